@@ -596,6 +596,50 @@ int simhand_augment_batch_ex(const uint8_t* images, const float* joints, const f
                              float* joints_aug, int32_t* rec, void* workspace, size_t workspace_bytes, sh_stream_t stream);
 
 /* ===========================================================================
+ * Row operators of an MLP / projection head: layer norm, linear (matrix product with bias, activation and residual in its epilogue) and 8-bit
+ * activation checkpoints, forward and backward.  All tensors are dense rows ([rows][cols], cols contiguous) in `dtype` = SH_F32 or SH_BF16 (the
+ * build's 16-bit type) unless a parameter says fp32; rows >= 0 and cols >= 1 are arbitrary (no multiple, element alignment suffices); sums,
+ * statistics and products accumulate in fp32, column sums over rows are folded in a fixed order (bit-reproducible).  Nothing is written beside the
+ * outputs and the workspace.  The reference has no such operators (its head is Linear -> BatchNorm1d -> ReLU -> Linear,
+ * src/models/unsupervised/simclr_model.py:22-39): parity is held against the formulas in 64 bits.
+ * =========================================================================== */
+enum sh_act { SH_ACT_NONE = 0, SH_ACT_RELU = 1, SH_ACT_GELU = 2 /* z Phi(z), by the error function */, SH_ACT_SILU = 3 /* z sigma(z) */ };
+
+/* y = h gamma + beta, h = (x - mean) rstd, mean / rstd [rows] fp32 over the cols of a row (rstd = 1 / sqrt(variance + eps)); relu: y = max(y, 0).
+ * gamma, beta fp32 [cols].  At most 16384 columns in 16 bits, 8192 in fp32. */
+int simhand_layer_norm_fwd(const void* x, const float* gamma, const float* beta, float eps, int relu, void* y, float* mean, float* rstd,
+                           int64_t rows, int cols, int dtype, sh_stream_t stream);
+/* u = dy (relu: where h gamma + beta > 0), g = u gamma: dx = rstd (g - mean_c(g) - h mean_c(g h)); dgamma_dbeta [2][cols] fp32 = sum_rows u h, sum_rows u.
+ * x is given as it is, or (x = NULL) as its 8-bit checkpoint x_codes / x_exps (simhand_act8_pack). */
+size_t simhand_layer_norm_bwd_workspace_bytes(int64_t rows, int cols, int dtype);
+int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, const float* gamma, const float* beta,
+                           const float* mean, const float* rstd, int relu, void* dx, float* dgamma_dbeta, int64_t rows, int cols, int dtype,
+                           void* workspace, size_t workspace_bytes, sh_stream_t stream);
+
+/* z = x w^T + bias, y = act(z) + residual; x [rows][in_dim], w [out_dim][in_dim], bias fp32 [out_dim] or NULL, residual [rows][out_dim] or NULL,
+ * pre [rows][out_dim] or NULL receives z (what simhand_linear_act_bwd takes).  residual may be y's own buffer. */
+int simhand_linear_fwd(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, void* pre, int64_t rows, int in_dim,
+                       int out_dim, int dtype, sh_stream_t stream);
+/* dz = dy act'(pre), db [cols] fp32 = sum_rows dz (before dz is rounded).  SH_ACT_NONE: pre and dz may be NULL (dz = dy; only db is computed).  dz may be dy's buffer. */
+size_t simhand_linear_act_bwd_workspace_bytes(int64_t rows, int cols, int dtype);
+int simhand_linear_act_bwd(const void* dy, const void* pre, int act, void* dz, float* db, int64_t rows, int cols, int dtype, void* workspace,
+                           size_t workspace_bytes, sh_stream_t stream);
+/* dx [rows][in_dim] = dz w (w [out_dim][in_dim] as in the forward call; its transposed copy lives in the workspace) */
+size_t simhand_linear_dgrad_workspace_bytes(int in_dim, int out_dim, int dtype);
+int simhand_linear_dgrad(const void* dz, const void* w, void* dx, int64_t rows, int in_dim, int out_dim, int dtype, void* workspace,
+                         size_t workspace_bytes, sh_stream_t stream);
+/* dw [out_dim][in_dim] fp32 = dz^T x; x as it is, or (x = NULL) as its 8-bit checkpoint, whose values enter the product rounded to dtype */
+size_t simhand_linear_wgrad_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype);
+int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, float* dw, int64_t rows, int in_dim,
+                         int out_dim, int dtype, void* workspace, size_t workspace_bytes, sh_stream_t stream);
+
+/* 8-bit activation checkpoint: codes [rows][cols] (OCP e4m3) and exps [rows][ceil(cols / 32)], value = e4m3(code) 2^(exp - 127) with one exponent for 32
+ * consecutive columns of a row: the least one with which the block's largest finite magnitude is at most 448 (never below 2^-126).  Rounded to nearest even;
+ * Inf and NaN are stored as NaN.  unpack rounds the values to dtype. */
+int simhand_act8_pack(const void* x, uint8_t* codes, uint8_t* exps, int64_t rows, int cols, int dtype, sh_stream_t stream);
+int simhand_act8_unpack(const uint8_t* codes, const uint8_t* exps, void* x, int64_t rows, int cols, int dtype, sh_stream_t stream);
+
+/* ===========================================================================
  * Thin RCCL wrappers behind an opaque communicator handle -- the exchange steps of the path for a caller
  * that does not go through torch.distributed: all-gather of the projection / joint rows into the reference row order,
  * all-reduce of the distance statistics (MAX / MIN / SUM) and of the parameter gradients (SUM).

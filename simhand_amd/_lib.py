@@ -43,6 +43,7 @@ DIST_MODES = {"mpjpe": 0, "w_abs": 1, "w_o_abs": 2, "l2": 3}
 WEIGHT_TYPES = {None: 0, "none": 0, "linear": 1, "non_linear": 2, "explicit": 3}
 PP_NORM_IN, PP_NORM_OUT, PP_ANGLE_AS_GIVEN = 1, 2, 4
 PP_FUSED = 3
+ACTS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
 PROF_CLASSES = ("conv_fwd", "conv_dgrad", "conv_wgrad", "bn", "pool", "loss", "misc", "optimizer")
 # enum sh_route: kernel the library dispatched a call to (index = counter slot)
 ROUTES = ("igemm128_fwd", "igemm128_dgrad", "igemm256_fwd", "igemm256_dgrad", "igemm256_tail", "gemm1x1_fwd", "gemm1x1_fwd_bnact",
@@ -241,6 +242,18 @@ SIGNATURES = {
     "simhand_augment_batch": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _S, _P]),
     "simhand_augment_workspace_bytes_ex": (_S, [_I, _I, _I, _I, _I]),
     "simhand_augment_batch_ex": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _S, _P]),
+    "simhand_layer_norm_fwd": (_I, [_P, _P, _P, _F, _I, _P, _P, _P, _L, _I, _I, _P]),
+    "simhand_layer_norm_bwd_workspace_bytes": (_S, [_L, _I, _I]),
+    "simhand_layer_norm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _L, _I, _I, _P, _S, _P]),
+    "simhand_linear_fwd": (_I, [_P, _P, _P, _I, _P, _P, _P, _L, _I, _I, _I, _P]),
+    "simhand_linear_act_bwd_workspace_bytes": (_S, [_L, _I, _I]),
+    "simhand_linear_act_bwd": (_I, [_P, _P, _I, _P, _P, _L, _I, _I, _P, _S, _P]),
+    "simhand_linear_dgrad_workspace_bytes": (_S, [_I, _I, _I]),
+    "simhand_linear_dgrad": (_I, [_P, _P, _P, _L, _I, _I, _I, _P, _S, _P]),
+    "simhand_linear_wgrad_workspace_bytes": (_S, [_L, _I, _I, _I]),
+    "simhand_linear_wgrad": (_I, [_P, _P, _P, _P, _P, _L, _I, _I, _I, _P, _S, _P]),
+    "simhand_act8_pack": (_I, [_P, _P, _P, _L, _I, _I, _P]),
+    "simhand_act8_unpack": (_I, [_P, _P, _P, _L, _I, _I, _P]),
     "simhand_comm_unique_id": (_I, [_P]),
     "simhand_comm_init": (_I, [_P, _I, _I, C.POINTER(_P)]),
     "simhand_comm_destroy": (_I, [_P]),

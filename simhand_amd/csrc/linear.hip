@@ -1,0 +1,530 @@
+// The linear operator of an MLP / projection head for any sizes:  y = act(x w^T + bias) + residual  and its gradients.
+//
+//   x [rows][in], w [out][in], y / pre / residual [rows][out] in fp32 or the build's 16-bit type; bias, db, dw fp32; products accumulate in fp32 on the matrix cores
+//   (fp32 operands on v_mfma_f32_16x16x4_f32: exact products, no reduced-precision mode), every output is rounded once.
+//   act backward: dz = dy act'(pre), db = sum_rows dz (of the unrounded dz);   dx = dz w;   dw = dz^T x, x possibly as its 8-bit checkpoint.
+//
+// linear_gemm_kernel (forward, and dx with w transposed first): out [M][N] = a [M][K] b[N][K]^T, tiles of 128 x 128, 128 bytes of K a step, both operands
+// global -> registers -> LDS with the next step's loads in flight under the MFMAs.  The operands are swapped (b is the MFMA's first one), and b's rows are permuted inside
+// the tile, so that a lane ends with 8 consecutive columns of one row: bias, residual, pre-activation and output move as 16-byte vectors.
+// linear_wgrad_kernel: dw [N][K] = dz^T x, the reduction runs over rows: tiles of 128 x 128 over a range of rows (split), 16-bit operands are read transposed from LDS
+// (ds_read_b64_tr_b16); the splits' fp32 partial sums are added in a fixed order by a second launch.
+#include "rows.h"
+
+namespace sh {
+
+template <typename T> __device__ __forceinline__ f32x4 mma16(const uint4& a, const uint4& b, f32x4 c) {
+  if constexpr (sizeof(T) == 2) {
+    return sh_mfma16(a, b, c);
+  } else {  // 16 bytes = 4 fp32: MFMA e takes element e of both operands (the same k order on both sides)
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
+  }
+}
+
+struct LinearArgs {
+  const void* a;        // [M][K]
+  const void* b;        // [N][ldb]
+  void* out;            // [M][N]
+  void* pre;            // [M][N] or null
+  const float* bias;    // [N] or null
+  const void* residual; // [M][N] or null
+  long long M;
+  int N, K, ldb, act;
+  unsigned n_tiles;
+};
+
+// tile column that row m of MFMA tile ni holds: lane group g of the tiles 2 j, 2 j + 1 ends with columns 32 j + 8 g .. + 7
+__device__ __forceinline__ int lin_col(int ni, int m) { return (ni >> 1) * 32 + (m >> 2) * 8 + (ni & 1) * 4 + (m & 3); }
+
+// the 8 finished sums of one row: z = acc + bias, pre <- z, out <- act(z) + residual
+template <typename T>
+__device__ __forceinline__ void linear_store8(const LinearArgs& p, long long row, int n, const float (&acc)[8]) {
+  constexpr int VE = Vec16<T>::N;
+  const int left = p.N - n;
+  if (left <= 0) return;
+  float z[8];
+  float b[8];
+  if (p.bias != nullptr) ld_f32<8>(p.bias + n, left, b);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) z[e] = p.bias != nullptr ? acc[e] + b[e] : acc[e];
+  const long long at = row * p.N + n;
+#pragma unroll
+  for (int h = 0; h < 8 / VE; ++h) {
+    const int l = left - h * VE;
+    if (l <= 0) break;
+    float o[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) o[e] = z[h * VE + e];
+    if (p.pre != nullptr) st_chunk<T>((T*)p.pre + at + h * VE, l, pack16<T>(o));
+    if (p.act != SH_ACT_NONE) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) o[e] = act_value(o[e], p.act);
+    }
+    if (p.residual != nullptr) {
+      float r[VE];
+      unpack16<T>(ld_chunk<T>((const T*)p.residual + at + h * VE, l), r);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) o[e] += r[e];
+    }
+    st_chunk<T>((T*)p.out + at + h * VE, l, pack16<T>(o));
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256, 2) void linear_gemm_kernel(LinearArgs p) {
+  constexpr int VE = Vec16<T>::N, KE = 128 / sizeof(T);  // elements per 16-byte chunk / per k-step (a tile row is 8 chunks)
+  __shared__ __attribute__((aligned(16))) char smem[2 * 128 * 128];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int li = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
+  const unsigned logical = xcd_order(blockIdx.x, gridDim.x);
+  const int n0 = (int)(logical % p.n_tiles) * 128;  // the n-tiles of a row tile are neighbours on one XCD: a is read from HBM once
+  const long long m0 = (long long)(logical / p.n_tiles) * 128;
+  const T* __restrict__ A = (const T*)p.a;
+  const T* __restrict__ B = (const T*)p.b;
+  // staging: thread = chunk tid & 7 of rows (tid >> 3) + 32 i of either operand; LDS chunk position = chunk ^ (row's key)
+  const int sc = tid & 7, sr = tid >> 3;
+  uint4 ra[4], rb[4];
+  auto load = [&](int k0) {
+    const int k = k0 + sc * VE, left = p.K - k;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long m = m0 + sr + 32 * i;
+      const int n = n0 + sr + 32 * i;
+      ra[i] = (m < p.M && left > 0) ? ld_chunk<T>(A + m * p.K + k, left) : make_uint4(0u, 0u, 0u, 0u);
+      rb[i] = (n < p.N && left > 0) ? ld_chunk<T>(B + (long long)n * p.ldb + k, left) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  auto key_b = [](int row) { return ((row >> 1) & 1) | (((row >> 3) & 3) << 1); };
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+    for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  load(0);
+  for (int k0 = 0; k0 < p.K; k0 += KE) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = sr + 32 * i;
+      *reinterpret_cast<uint4*>(smem + row * 128 + ((sc ^ ((row >> 1) & 7)) * 16)) = ra[i];
+      *reinterpret_cast<uint4*>(smem + 16384 + row * 128 + ((sc ^ key_b(row)) * 16)) = rb[i];
+    }
+    __syncthreads();
+    if (k0 + KE < p.K) load(k0 + KE);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      uint4 fa[4], fb[4];
+#pragma unroll
+      for (int mi = 0; mi < 4; ++mi) {
+        const int row = wm * 64 + mi * 16 + li;
+        fa[mi] = *reinterpret_cast<const uint4*>(smem + row * 128 + (((kk * 4 + g) ^ ((row >> 1) & 7)) * 16));
+      }
+#pragma unroll
+      for (int ni = 0; ni < 4; ++ni) {
+        const int row = wn * 64 + lin_col(ni, li);
+        fb[ni] = *reinterpret_cast<const uint4*>(smem + 16384 + row * 128 + (((kk * 4 + g) ^ key_b(row)) * 16));
+      }
+#pragma unroll
+      for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = mma16<T>(fb[ni], fa[mi], acc[mi][ni]);
+    }
+  }
+#pragma unroll
+  for (int mi = 0; mi < 4; ++mi) {
+    const long long row = m0 + wm * 64 + mi * 16 + li;
+    if (row >= p.M) continue;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float v[8];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        v[r] = acc[mi][2 * j][r];
+        v[4 + r] = acc[mi][2 * j + 1][r];
+      }
+      linear_store8<T>(p, row, n0 + wn * 64 + j * 32 + g * 8, v);
+    }
+  }
+}
+
+// w [n][k] -> wt [k][ldt], 32 x 32 tiles through LDS; columns n .. ldt - 1 are written as zeros
+template <typename T> __global__ __launch_bounds__(256) void linear_transpose_kernel(const T* __restrict__ w, T* __restrict__ wt, int n, int k, int ldt) {
+  __shared__ T tile[32][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int n0 = blockIdx.y * 32, k0 = blockIdx.x * 32;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    const int r = n0 + ty + i, c = k0 + tx;
+    tile[ty + i][tx] = (r < n && c < k) ? w[(long long)r * k + c] : (T)0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    const int r = k0 + ty + i, c = n0 + tx;
+    if (r < k && c < ldt) wt[(long long)r * ldt + c] = tile[tx][ty + i];
+  }
+}
+
+// ---- dz = dy act'(pre), db ----------------------------------------------------------------------------------------------------
+// A block covers TX 16-byte vectors of columns (TX = 8 .. 64, the power of two at or above a narrow row's vectors) and 256 / TX rows at a time over its range of rows;
+// part [row blocks][cols] = its column sums.
+template <typename T, int TX>
+__global__ __launch_bounds__(256) void linear_act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ pre, int act, T* __restrict__ dz,
+                                                             float* __restrict__ part, long long rows, int cols, long long per_block) {
+  constexpr int VE = Vec16<T>::N, TY = 256 / TX;
+  __shared__ float red[TY][TX * VE + 1];
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+  const int c = (blockIdx.x * TX + tx) * VE;
+  const long long r0 = (long long)blockIdx.y * per_block;
+  const long long r1 = r0 + per_block < rows ? r0 + per_block : rows;
+  float s[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) s[e] = 0.f;
+  if (c < cols) {
+    const int left = cols - c;
+    for (long long r = r0 + ty; r < r1; r += TY) {
+      float d[VE];
+      unpack16<T>(ld_chunk<T>(dy + r * cols + c, left), d);
+      if (act != SH_ACT_NONE) {
+        float z[VE];
+        unpack16<T>(ld_chunk<T>(pre + r * cols + c, left), z);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) d[e] *= act_slope(z[e], act);
+      }
+#pragma unroll
+      for (int e = 0; e < VE; ++e) s[e] += d[e];
+      if (dz != nullptr) st_chunk<T>(dz + r * cols + c, left, pack16<T>(d));
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VE; ++e) red[ty][tx * VE + e] = s[e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < TX * VE; i += 256) {
+    const int col = blockIdx.x * TX * VE + i;
+    if (col >= cols) continue;
+    float a = 0.f;
+#pragma unroll
+    for (int y = 0; y < TY; ++y) a += red[y][i];
+    part[(long long)blockIdx.y * cols + col] = a;
+  }
+}
+
+// ---- dw = dz^T x ---------------------------------------------------------------------------------------------------------------
+struct WgradArgsL {
+  const void* dz;         // [M][N]
+  const void* x;          // [M][K] (null: codes)
+  const uint8_t* codes;   // [M][K]
+  const uint8_t* exps;    // [M][ceil(K / 32)]
+  float* part;            // [splits][N][K]
+  long long M, per_split; // per_split: a multiple of the k-step
+  int N, K;
+  unsigned n_tiles, k_tiles;
+};
+
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+// 16-bit operand of 32 rows x 16 columns read transposed: lane gets rows {4g..4g+3, 16+4g..16+4g+3} of column cb + (lane & 15)
+__device__ __forceinline__ uint4 frag_tr16(const char* tile, int stride, int cb, int lane) {
+  typedef s16x4_t __attribute__((address_space(3))) * lds_ptr;
+  const int p = lane & 15, g = lane >> 4;
+  const char* a0 = tile + (4 * g + (p >> 2)) * stride + (cb + (p & 3) * 4) * 2;
+  const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(a0));
+  const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(a0 + 16 * stride));
+  uint4 r;
+  r.x = (unsigned)(unsigned short)lo[0] | ((unsigned)(unsigned short)lo[1] << 16);
+  r.y = (unsigned)(unsigned short)lo[2] | ((unsigned)(unsigned short)lo[3] << 16);
+  r.z = (unsigned)(unsigned short)hi[0] | ((unsigned)(unsigned short)hi[1] << 16);
+  r.w = (unsigned)(unsigned short)hi[2] | ((unsigned)(unsigned short)hi[3] << 16);
+  return r;
+}
+
+template <typename T, bool A8>
+__global__ __launch_bounds__(256, 2) void linear_wgrad_kernel(WgradArgsL p) {
+  constexpr int VE = Vec16<T>::N;
+  constexpr int KP = sizeof(T) == 2 ? 32 : 16;      // rows per step
+  constexpr int CH = 128 / VE;                      // 16-byte chunks of a 128-column tile row
+  constexpr int STRIDE = 128 * sizeof(T) + (sizeof(T) == 2 ? 32 : 64);  // padded: the rows a transpose read / a group of lanes touches fall on different banks
+  constexpr int NCH = KP * CH / 256;                // chunks per thread and operand
+  __shared__ __attribute__((aligned(16))) char smem[2 * KP * STRIDE];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int li = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
+  unsigned logical = xcd_order(blockIdx.x, gridDim.x);
+  const int k0 = (int)(logical % p.k_tiles) * 128; logical /= p.k_tiles;
+  const int n0 = (int)(logical % p.n_tiles) * 128;
+  const int split = (int)(logical / p.n_tiles);
+  const long long r0 = (long long)split * p.per_split;
+  const long long r1 = r0 + p.per_split < p.M ? r0 + p.per_split : p.M;
+  const int eb = (p.K + kAct8Block - 1) / kAct8Block;
+  uint4 rd[NCH], rx[NCH];
+  auto load = [&](long long r) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int q = tid + 256 * i;
+      const long long row = r + q / CH;
+      const int col = (q % CH) * VE;
+      const int ln = p.N - (n0 + col), lk = p.K - (k0 + col);
+      rd[i] = (row < r1 && ln > 0) ? ld_chunk<T>((const T*)p.dz + row * p.N + n0 + col, ln) : make_uint4(0u, 0u, 0u, 0u);
+      if constexpr (A8) {
+        float v[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) v[e] = 0.f;
+        if (row < r1 && lk > 0) {
+          unsigned w[VE / 4];
+          act8_ld_codes<VE>(p.codes + row * p.K + k0 + col, lk, w);
+          const float sc = act8_scale(p.exps[row * eb + (k0 + col) / kAct8Block]);
+#pragma unroll
+          for (int j = 0; j < VE / 4; ++j) act8_decode4(w[j], sc, v + 4 * j);
+        }
+        rx[i] = pack16<T>(v);
+      } else {
+        rx[i] = (row < r1 && lk > 0) ? ld_chunk<T>((const T*)p.x + row * p.K + k0 + col, lk) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  };
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+    for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  char* td = smem;
+  char* tx = smem + KP * STRIDE;
+  load(r0);
+  for (long long r = r0; r < r1; r += KP) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int q = tid + 256 * i;
+      const int at = (q / CH) * STRIDE + (q % CH) * 16;
+      *reinterpret_cast<uint4*>(td + at) = rd[i];
+      *reinterpret_cast<uint4*>(tx + at) = rx[i];
+    }
+    __syncthreads();
+    if (r + KP < r1) load(r + KP);
+    if constexpr (sizeof(T) == 2) {
+      uint4 fd[4], fx[4];
+#pragma unroll
+      for (int mi = 0; mi < 4; ++mi) fd[mi] = frag_tr16(td, STRIDE, wm * 64 + mi * 16, lane);
+#pragma unroll
+      for (int ni = 0; ni < 4; ++ni) fx[ni] = frag_tr16(tx, STRIDE, wn * 64 + ni * 16, lane);
+#pragma unroll
+      for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = mma16<T>(fd[mi], fx[ni], acc[mi][ni]);
+    } else {
+#pragma unroll
+      for (int s4 = 0; s4 < KP / 4; ++s4) {
+        float fd[4], fx[4];
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi) {
+          fd[mi] = *reinterpret_cast<const float*>(td + (s4 * 4 + g) * STRIDE + (wm * 64 + mi * 16 + li) * 4);
+          fx[mi] = *reinterpret_cast<const float*>(tx + (s4 * 4 + g) * STRIDE + (wn * 64 + mi * 16 + li) * 4);
+        }
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+          for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x4f32(fd[mi], fx[ni], acc[mi][ni], 0, 0, 0);
+      }
+    }
+  }
+  // lane: rows n = n0 + wm 64 + 16 mi + 4 g + r, column k = k0 + wn 64 + 16 ni + li
+  float* out = p.part + (long long)split * p.N * p.K;
+#pragma unroll
+  for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int n = n0 + wm * 64 + mi * 16 + 4 * g + r;
+      if (n >= p.N) continue;
+#pragma unroll
+      for (int ni = 0; ni < 4; ++ni) {
+        const int k = k0 + wn * 64 + ni * 16 + li;
+        if (k < p.K) out[(long long)n * p.K + k] = acc[mi][ni][r];
+      }
+    }
+}
+
+// the splits' partial sums in a fixed order
+__global__ __launch_bounds__(256) void linear_wgrad_reduce_kernel(const float* __restrict__ part, long long count, int splits, float* __restrict__ dw) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= count) return;
+  float a = 0.f;
+  for (int s = 0; s < splits; ++s) a += part[(long long)s * count + i];
+  dw[i] = a;
+}
+
+__global__ __launch_bounds__(256) void rows_zero_kernel(float* p, long long n) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = 0.f;
+}
+
+static int linear_bad(const char* what, int64_t rows, int in, int out, int dtype) {
+  SH_REQUIRE(dtype == SH_F32 || dtype == SH_BF16, "%s: dtype %d", what, dtype);
+  SH_REQUIRE(rows >= 0 && rows < (1ll << 31) && in >= 1 && out >= 1 && in <= (1 << 20) && out <= (1 << 20), "%s: rows=%lld in=%d out=%d", what, (long long)rows, in, out);
+  SH_REQUIRE((int64_t)((rows + 127) / 128) * ((in > out ? in : out) / 128 + 1) < (1ll << 31), "%s: rows=%lld in=%d out=%d: too many tiles", what,
+             (long long)rows, in, out);
+  return 0;
+}
+
+static int gemm_launch(const LinearArgs& base, int dtype, hipStream_t s, const char* what) {
+  LinearArgs p = base;
+  p.n_tiles = (unsigned)ceil_div(p.N, 128);
+  const unsigned grid = (unsigned)ceil_div(p.M, 128) * p.n_tiles;
+  if (dtype == SH_F32) linear_gemm_kernel<float><<<grid, 256, 0, s>>>(p);
+  else linear_gemm_kernel<bf16_t><<<grid, 256, 0, s>>>(p);
+  return check_launch(what);
+}
+
+static int act_bwd_tx(int cols, int dtype) {
+  const int nvec = (cols + (dtype == SH_F32 ? 4 : 8) - 1) / (dtype == SH_F32 ? 4 : 8);
+  return nvec <= 8 ? 8 : nvec <= 16 ? 16 : nvec <= 32 ? 32 : 64;
+}
+static void act_bwd_plan(int64_t rows, int cols, int dtype, int* gx, int* gy, int64_t* per) {
+  const int tx = act_bwd_tx(cols, dtype), ty = 256 / tx, ve = dtype == SH_F32 ? 4 : 8;
+  *gx = ceil_div(cols, tx * ve);
+  int64_t want = (2048 + *gx - 1) / *gx, most = (rows + ty - 1) / ty;
+  if (want > most) want = most;
+  if (want < 1) want = 1;
+  *per = ((rows + want - 1) / want + ty - 1) / ty * ty;
+  if (*per < 1) *per = ty;
+  *gy = (int)((rows + *per - 1) / *per);
+  if (*gy < 1) *gy = 1;
+}
+
+static void linear_wgrad_plan(int64_t rows, int in, int out, int dtype, int* splits, int64_t* per) {
+  const int kp = dtype == SH_F32 ? 16 : 32;
+  const int64_t tiles = (int64_t)ceil_div(in, 128) * ceil_div(out, 128);
+  const int64_t steps = rows > 0 ? (rows + kp - 1) / kp : 1;
+  int64_t sk = 512 / tiles;
+  if (sk > (steps + 15) / 16) sk = (steps + 15) / 16;  // at least 16 steps each
+  if (sk < 1) sk = 1;
+  const int64_t each = (steps + sk - 1) / sk;
+  *per = each * kp;
+  *splits = (int)((steps + each - 1) / each);
+}
+
+}  // namespace sh
+
+using namespace sh;
+
+extern "C" {
+
+int simhand_linear_fwd(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, void* pre, int64_t rows, int in_dim,
+                       int out_dim, int dtype, sh_stream_t stream) {
+  if (linear_bad("linear_fwd", rows, in_dim, out_dim, dtype)) return 1;
+  SH_REQUIRE(act >= SH_ACT_NONE && act <= SH_ACT_SILU, "linear_fwd: act %d", act);
+  if (rows == 0) return 0;
+  SH_REQUIRE(x && w && y, "linear_fwd: NULL argument");
+  hipStream_t s = (hipStream_t)stream;
+  const double eb = dtype == SH_F32 ? 4 : 2;
+  ProfScope ps(SH_PROF_MISC, s, 2.0 * rows * in_dim * out_dim, eb * ((double)rows * in_dim + (double)in_dim * out_dim + (double)rows * out_dim));
+  LinearArgs p = {x, w, y, pre, bias, residual, rows, out_dim, in_dim, in_dim, act, 0};
+  return gemm_launch(p, dtype, s, "linear_fwd");
+}
+
+size_t simhand_linear_act_bwd_workspace_bytes(int64_t rows, int cols, int dtype) {
+  if (rows < 0 || cols < 1) return 0;
+  int gx, gy;
+  int64_t per;
+  act_bwd_plan(rows, cols, dtype, &gx, &gy, &per);
+  return (size_t)gy * cols * sizeof(float);
+}
+
+int simhand_linear_act_bwd(const void* dy, const void* pre, int act, void* dz, float* db, int64_t rows, int cols, int dtype, void* workspace,
+                           size_t workspace_bytes, sh_stream_t stream) {
+  if (linear_bad("linear_act_bwd", rows, 1, cols, dtype)) return 1;
+  SH_REQUIRE(act >= SH_ACT_NONE && act <= SH_ACT_SILU, "linear_act_bwd: act %d", act);
+  SH_REQUIRE(db && (rows == 0 || dy), "linear_act_bwd: NULL argument");
+  SH_REQUIRE(rows == 0 || act == SH_ACT_NONE || (pre && dz), "linear_act_bwd: an activation needs pre and dz");
+  SH_REQUIRE(workspace && workspace_bytes >= simhand_linear_act_bwd_workspace_bytes(rows, cols, dtype), "linear_act_bwd: workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  ProfScope ps(SH_PROF_MISC, s, 0, (dtype == SH_F32 ? 4.0 : 2.0) * rows * cols * (act == SH_ACT_NONE ? 1 : 3));
+  int gx, gy;
+  int64_t per;
+  act_bwd_plan(rows, cols, dtype, &gx, &gy, &per);
+  float* part = (float*)workspace;
+  const dim3 grid(gx, gy);
+#define SH_ACT(T, TX) linear_act_bwd_kernel<T, TX><<<grid, 256, 0, s>>>((const T*)dy, (const T*)pre, act, (T*)dz, part, rows, cols, per)
+#define SH_ACT_TX(T)                       \
+  switch (act_bwd_tx(cols, dtype)) {       \
+    case 8: SH_ACT(T, 8); break;           \
+    case 16: SH_ACT(T, 16); break;         \
+    case 32: SH_ACT(T, 32); break;         \
+    default: SH_ACT(T, 64); break;         \
+  }
+  if (dtype == SH_F32) { SH_ACT_TX(float) }
+  else { SH_ACT_TX(bf16_t) }
+#undef SH_ACT_TX
+#undef SH_ACT
+  if (check_launch("linear_act_bwd")) return 1;
+  return fold_columns(part, gy, cols, db, s);
+}
+
+size_t simhand_linear_dgrad_workspace_bytes(int in_dim, int out_dim, int dtype) {
+  if (in_dim < 1 || out_dim < 1) return 0;
+  return (size_t)in_dim * ((out_dim + 7) / 8 * 8) * (dtype == SH_F32 ? 4 : 2);
+}
+
+int simhand_linear_dgrad(const void* dz, const void* w, void* dx, int64_t rows, int in_dim, int out_dim, int dtype, void* workspace,
+                         size_t workspace_bytes, sh_stream_t stream) {
+  if (linear_bad("linear_dgrad", rows, in_dim, out_dim, dtype)) return 1;
+  if (rows == 0) return 0;
+  SH_REQUIRE(dz && w && dx, "linear_dgrad: NULL argument");
+  SH_REQUIRE(workspace && workspace_bytes >= simhand_linear_dgrad_workspace_bytes(in_dim, out_dim, dtype), "linear_dgrad: workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  const double eb = dtype == SH_F32 ? 4 : 2;
+  ProfScope ps(SH_PROF_MISC, s, 2.0 * rows * in_dim * out_dim, eb * ((double)rows * in_dim + (double)in_dim * out_dim + (double)rows * out_dim));
+  const int ldt = (out_dim + 7) / 8 * 8;
+  const dim3 tg(ceil_div(in_dim, 32), ceil_div(ldt, 32));
+  if (dtype == SH_F32) linear_transpose_kernel<float><<<tg, 256, 0, s>>>((const float*)w, (float*)workspace, out_dim, in_dim, ldt);
+  else linear_transpose_kernel<bf16_t><<<tg, 256, 0, s>>>((const bf16_t*)w, (bf16_t*)workspace, out_dim, in_dim, ldt);
+  if (check_launch("linear_dgrad")) return 1;
+  LinearArgs p = {dz, workspace, dx, nullptr, nullptr, nullptr, rows, in_dim, out_dim, ldt, SH_ACT_NONE, 0};
+  return gemm_launch(p, dtype, s, "linear_dgrad");
+}
+
+size_t simhand_linear_wgrad_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype) {
+  if (rows < 0 || in_dim < 1 || out_dim < 1) return 0;
+  int splits;
+  int64_t per;
+  linear_wgrad_plan(rows, in_dim, out_dim, dtype, &splits, &per);
+  return splits > 1 ? (size_t)splits * in_dim * out_dim * sizeof(float) : 16;
+}
+
+int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, float* dw, int64_t rows, int in_dim, int out_dim,
+                         int dtype, void* workspace, size_t workspace_bytes, sh_stream_t stream) {
+  if (linear_bad("linear_wgrad", rows, in_dim, out_dim, dtype)) return 1;
+  const bool a8 = x_codes != nullptr;
+  SH_REQUIRE(!a8 || (x_exps && !x), "linear_wgrad: pass either x or its codes and exponents");
+  SH_REQUIRE(dw && (rows == 0 || (dz && (x || a8))), "linear_wgrad: NULL argument");
+  SH_REQUIRE(workspace && workspace_bytes >= simhand_linear_wgrad_workspace_bytes(rows, in_dim, out_dim, dtype), "linear_wgrad: workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  const double eb = dtype == SH_F32 ? 4 : 2;
+  ProfScope ps(SH_PROF_MISC, s, 2.0 * rows * in_dim * out_dim, eb * (double)rows * out_dim + (a8 ? 1.03125 : eb) * rows * in_dim + 4.0 * in_dim * out_dim);
+  const long long count = (long long)in_dim * out_dim;
+  if (rows == 0) {
+    rows_zero_kernel<<<(unsigned)((count + 255) / 256), 256, 0, s>>>(dw, count);
+    return check_launch("linear_wgrad");
+  }
+  int splits;
+  int64_t per;
+  linear_wgrad_plan(rows, in_dim, out_dim, dtype, &splits, &per);
+  WgradArgsL p = {dz, x, x_codes, x_exps, splits > 1 ? (float*)workspace : dw, rows, per, out_dim, in_dim, (unsigned)ceil_div(out_dim, 128),
+                  (unsigned)ceil_div(in_dim, 128)};
+  const unsigned grid = p.n_tiles * p.k_tiles * (unsigned)splits;
+  if (dtype == SH_F32) {
+    if (a8) linear_wgrad_kernel<float, true><<<grid, 256, 0, s>>>(p);
+    else linear_wgrad_kernel<float, false><<<grid, 256, 0, s>>>(p);
+  } else {
+    if (a8) linear_wgrad_kernel<bf16_t, true><<<grid, 256, 0, s>>>(p);
+    else linear_wgrad_kernel<bf16_t, false><<<grid, 256, 0, s>>>(p);
+  }
+  if (check_launch("linear_wgrad")) return 1;
+  if (splits > 1) {
+    linear_wgrad_reduce_kernel<<<(unsigned)((count + 255) / 256), 256, 0, s>>>((const float*)workspace, count, splits, dw);
+    return check_launch("linear_wgrad_reduce");
+  }
+  return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,146 @@
+// Row-vector helpers of the layer-norm / linear / 8-bit activation kernels: rows of any length at any element alignment, and the block-scaled e4m3 codes.
+#pragma once
+#include "common.h"
+
+namespace sh {
+
+// 16 bytes at an address that is only element-aligned (a row of odd length): gfx950 serves unaligned global accesses in hardware, the type tells
+// the compiler not to assume more
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned u32x4_any1 __attribute__((ext_vector_type(4), aligned(1)));
+
+__device__ __forceinline__ uint4 ld16_any(const void* p) {
+  const u32x4_any v = *reinterpret_cast<const u32x4_any*>(p);
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+__device__ __forceinline__ void st16_any(void* p, const uint4& v) {
+  const u32x4_any o = {v.x, v.y, v.z, v.w};
+  *reinterpret_cast<u32x4_any*>(p) = o;
+}
+
+// 16-byte chunk <-> fp32 lanes
+template <typename T> __device__ __forceinline__ void unpack16(const uint4& v, float (&o)[Vec16<T>::N]) {
+  const unsigned w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (Vec16<T>::N == 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[2 * i] = h16_lo(w[i]);
+      o[2 * i + 1] = h16_hi(w[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __uint_as_float(w[i]);
+  }
+}
+template <typename T> __device__ __forceinline__ uint4 pack16(const float (&o)[Vec16<T>::N]) {
+  unsigned w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (Vec16<T>::N == 8) w[i] = pack_bf16x2(o[2 * i], o[2 * i + 1]);
+    else w[i] = __float_as_uint(o[i]);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// the chunk at p of which `left` elements exist (left >= N: all); what is missing reads as zero and is not touched in memory
+template <typename T> __device__ __forceinline__ uint4 ld_chunk(const T* p, int left) {
+  constexpr int N = Vec16<T>::N;
+  if (left >= N) return ld16_any(p);
+  unsigned w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int e = 0; e < N - 1; ++e) {
+    if (e < left) {
+      if constexpr (N == 8) w[e >> 1] |= (unsigned)p[e] << ((e & 1) * 16);
+      else w[e] = __float_as_uint(p[e]);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T> __device__ __forceinline__ void st_chunk(T* p, int left, const uint4& v) {
+  constexpr int N = Vec16<T>::N;
+  if (left >= N) {
+    st16_any(p, v);
+    return;
+  }
+  const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < N - 1; ++e) {
+    if (e < left) {
+      if constexpr (N == 8) p[e] = (T)(w[e >> 1] >> ((e & 1) * 16));
+      else p[e] = __uint_as_float(w[e]);
+    }
+  }
+}
+// fp32 vectors beside a row (gamma, beta, bias): N floats at p, `left` of them existing; missing ones are zero
+template <int N> __device__ __forceinline__ void ld_f32(const float* p, int left, float (&o)[N]) {
+  typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+  if (left >= N) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const f32x4_any v = *reinterpret_cast<const f32x4_any*>(p + i);
+      o[i] = v.x; o[i + 1] = v.y; o[i + 2] = v.z; o[i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = i < left ? p[i] : 0.f;
+  }
+}
+
+// ---- 8-bit activations: value = e4m3(code) * 2^(exp - 127), one exp byte (1 .. 247) for 32 consecutive columns of a row ------------------
+constexpr int kAct8Block = 32;
+__device__ __forceinline__ float act8_scale(unsigned exp) { return __uint_as_float(exp << 23); }
+// four codes of one word
+__device__ __forceinline__ void act8_decode4(unsigned w, float scale, float* o) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  o[0] = lo[0] * scale; o[1] = lo[1] * scale; o[2] = hi[0] * scale; o[3] = hi[1] * scale;
+}
+// N (4, 8, 16) codes at p, `left` of them existing; missing ones decode to zero
+template <int N> __device__ __forceinline__ void act8_ld_codes(const uint8_t* p, int left, unsigned (&w)[N / 4]) {
+  if (left >= N) {
+    if constexpr (N == 16) {
+      const u32x4_any1 v = *reinterpret_cast<const u32x4_any1*>(p);
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else if constexpr (N == 8) {
+      const u32x2_any v = *reinterpret_cast<const u32x2_any*>(p);
+      w[0] = v.x; w[1] = v.y;
+    } else {
+      typedef unsigned u32_any __attribute__((aligned(1)));
+      w[0] = *reinterpret_cast<const u32_any*>(p);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) w[i] = 0u;
+#pragma unroll
+  for (int e = 0; e < N - 1; ++e)
+    if (e < left) w[e >> 2] |= (unsigned)p[e] << ((e & 3) * 8);
+}
+
+// xcd-aware order: the hardware puts block b on XCD b % 8; every XCD gets a contiguous range of logical tiles
+__device__ __forceinline__ unsigned xcd_order(unsigned bid, unsigned nblk) {
+  const unsigned q = nblk >> 3, r = nblk & 7, xcd = bid & 7, j = bid >> 3;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + j;
+}
+
+// activations of the linear operator (enum sh_act) and their derivatives, fp32.  NaN stays NaN (also through ReLU).
+__device__ __forceinline__ float act_value(float z, int act) {
+  if (act == SH_ACT_RELU) return z <= 0.f ? 0.f : z;
+  if (act == SH_ACT_GELU) return z * (0.5f * (1.f + erff(z * 0.70710678118654752f)));
+  if (act == SH_ACT_SILU) return z / (1.f + expf(-z));
+  return z;
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+  if (act == SH_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if (act == SH_ACT_GELU) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+  if (act == SH_ACT_SILU) {
+    const float s = 1.f / (1.f + expf(-z));
+    return s * (1.f + z * (1.f - s));
+  }
+  return 1.f;
+}
+
+// ---- column sums: part [nblk][n] -> out [n], folded in 64 bits in the order of the blocks (rows.hip) -----------------------------------
+int fold_columns(const float* part, int nblk, int n, float* out, hipStream_t s);
+}  // namespace sh

@@ -189,6 +189,181 @@ def proj_stats(P: torch.Tensor) -> torch.Tensor:
     return out
 
 
+# ------------------------------------------------------------------ row operators: layer norm, linear, 8-bit activations
+class Act8:
+    """An activation kept in 8 bits for the backward pass (act8_pack): e4m3 ``codes`` (uint8, the activation's shape), one power of two for every 32
+    consecutive values of a row in ``exps`` (uint8 [rows][ceil(cols / 32)]) and the ``dtype`` it was packed from.  value = e4m3(code) * 2^(exp - 127).
+    linear_bwd and layer_norm_bwd take it in the activation's place."""
+    __slots__ = ("codes", "exps", "dtype")
+
+    def __init__(self, codes: torch.Tensor, exps: torch.Tensor, dtype: torch.dtype):
+        cols = codes.shape[-1] if codes.dim() else 0
+        if codes.dtype != torch.uint8 or exps.dtype != torch.uint8 or cols < 1:
+            raise _lib.SimhandHipError("Act8: codes [..., cols >= 1] and exps must be uint8 tensors")
+        if exps.numel() != codes.numel() // cols * ((cols + 31) // 32) or exps.device != codes.device:
+            raise _lib.SimhandHipError(f"Act8: {tuple(codes.shape)} codes need one exponent per 32 columns of a row on their device, got {tuple(exps.shape)}")
+        self.codes, self.exps, self.dtype = codes, exps, dtype
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def _rows_of(x, what: str) -> Tuple[int, int]:
+    """(rows, cols) of a row tensor [..., cols] that lives on the current device (the launch goes to that device's current stream)."""
+    if x.device.type != "cuda":
+        raise _lib.SimhandHipError(f"{what}: simhand_amd ops need device tensors (there is no CPU path)")
+    if x.device.index != torch.cuda.current_device():
+        raise _lib.SimhandHipError(f"{what}: the tensor is on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise _lib.SimhandHipError(f"{what}: rows of at least one value, got shape {tuple(shape)}")
+    cols = shape[-1]
+    n = x.codes.numel() if isinstance(x, Act8) else x.numel()
+    return n // cols, cols
+
+
+def _like(t: Optional[torch.Tensor], x, shape, dtype: torch.dtype, what: str) -> C.c_void_p:
+    """Pointer of an operand that has to have this shape and type, on x's device (None: NULL)."""
+    if t is None:
+        return C.c_void_p(0)
+    if t.device != x.device or t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise _lib.SimhandHipError(f"{what}: expected {tuple(shape)} {dtype} on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return _ptr(t)
+
+
+def _saved(x, like: torch.Tensor, shape, what: str):
+    """(x, codes, exps) pointers of a saved activation: a tensor, or its 8-bit checkpoint."""
+    if isinstance(x, Act8):
+        if x.dtype != like.dtype:
+            raise _lib.SimhandHipError(f"{what}: checkpoint of a {x.dtype} activation next to a {like.dtype} gradient")
+        return C.c_void_p(0), _like(x.codes, like, shape, torch.uint8, what), _ptr(x.exps, torch.uint8)
+    return _like(x, like, shape, like.dtype, what), C.c_void_p(0), C.c_void_p(0)
+
+
+def _act_id(act: Optional[str], what: str) -> int:
+    if act not in _lib.ACTS:
+        raise _lib.SimhandHipError(f"{what}: act must be one of {sorted(k for k in _lib.ACTS if k)}, got {act!r}")
+    return _lib.ACTS[act]
+
+
+def layer_norm_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps: float = 1e-5, relu: bool = False):
+    """(y, mean, rstd): y = (x - mean) * rstd * gamma + beta over the last dimension (relu: max(y, 0)); gamma, beta fp32 [cols]; mean, rstd fp32,
+    one per row, for layer_norm_bwd."""
+    rows, cols = _rows_of(x, "layer_norm_fwd")
+    lib = _lib_dev()
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    stat = torch.empty(2, rows, dtype=torch.float32, device=x.device)
+    mean, rstd = stat[0], stat[1]
+    check(lib.simhand_layer_norm_fwd(_ptr(x), _like(gamma, x, (cols,), _F32, "layer_norm_fwd (gamma)"), _like(beta, x, (cols,), _F32, "layer_norm_fwd (beta)"),
+                                     float(eps), int(bool(relu)), _ptr(y), _ptr(mean), _ptr(rstd), rows, cols, dt(x.dtype), _stream()), "layer_norm_fwd")
+    return y, mean, rstd
+
+
+def layer_norm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, beta: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, relu: bool = False):
+    """(dx, dgamma, dbeta) of layer_norm_fwd.  x: its input, or the input's 8-bit checkpoint (act8_pack); mean, rstd: as returned there.  With relu the gate
+    is recomputed from x (bit for bit the forward's when x is the tensor itself)."""
+    rows, cols = _rows_of(dy, "layer_norm_bwd")
+    lib = _lib_dev()
+    what = "layer_norm_bwd"
+    px, pc, pe = _saved(x, dy, dy.shape, what + " (x)")
+    dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
+    dgb = torch.empty(2, cols, dtype=torch.float32, device=dy.device)
+    d = dt(dy.dtype)
+    nb = lib.simhand_layer_norm_bwd_workspace_bytes(rows, cols, d)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dy.device)
+    check(lib.simhand_layer_norm_bwd(_ptr(dy), px, pc, pe, _like(gamma, dy, (cols,), _F32, what + " (gamma)"), _like(beta, dy, (cols,), _F32, what + " (beta)"),
+                                     _like(mean, dy, (rows,), _F32, what + " (mean)"), _like(rstd, dy, (rows,), _F32, what + " (rstd)"), int(bool(relu)),
+                                     _ptr(dx), _ptr(dgb), rows, cols, d, _ptr(ws), nb, _stream()), what)
+    return dx, dgb[0], dgb[1]
+
+
+def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
+               residual: Optional[torch.Tensor] = None, want_pre: bool = False):
+    """y = act(x w^T + bias) + residual in one launch; x [..., in], w [out][in] in x's type, bias fp32 [out], residual [..., out]; act: none, relu, gelu
+    (by the error function) or silu.  want_pre: returns (y, pre), pre = x w^T + bias in x's type -- what linear_act_bwd takes."""
+    rows, cin = _rows_of(x, "linear_fwd")
+    lib = _lib_dev()
+    a = _act_id(act, "linear_fwd")
+    if w.dim() != 2 or w.shape[0] < 1:
+        raise _lib.SimhandHipError(f"linear_fwd: w must be [out][in], got {tuple(w.shape)}")
+    cout = w.shape[0]
+    shape = x.shape[:-1] + (cout,)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    pre = torch.empty_like(y) if want_pre else None
+    check(lib.simhand_linear_fwd(_ptr(x), _like(w, x, (cout, cin), x.dtype, "linear_fwd (w)"), _like(bias, x, (cout,), _F32, "linear_fwd (bias)"), a,
+                                 _like(residual, x, shape, x.dtype, "linear_fwd (residual)"), _ptr(y), _ptr(pre), rows, cin, cout, dt(x.dtype), _stream()),
+          "linear_fwd")
+    return (y, pre) if want_pre else y
+
+
+def linear_act_bwd(dy: torch.Tensor, pre: Optional[torch.Tensor] = None, act: Optional[str] = None):
+    """(dz, db): dz = dy * act'(pre) in dy's type, db fp32 = the sum of the unrounded dz over the rows (the bias gradient).  Without an activation dz is dy
+    itself.  (The residual's gradient is dy.)"""
+    rows, cols = _rows_of(dy, "linear_act_bwd")
+    lib = _lib_dev()
+    a = _act_id(act, "linear_act_bwd")
+    if a != 0 and pre is None:
+        raise _lib.SimhandHipError("linear_act_bwd: an activation needs the saved pre-activation")
+    d = dt(dy.dtype)
+    dz = torch.empty_like(dy, memory_format=torch.contiguous_format) if a else dy
+    db = torch.empty(cols, dtype=torch.float32, device=dy.device)
+    nb = lib.simhand_linear_act_bwd_workspace_bytes(rows, cols, d)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dy.device)
+    check(lib.simhand_linear_act_bwd(_ptr(dy), _like(pre if a else None, dy, dy.shape, dy.dtype, "linear_act_bwd (pre)"), a, _ptr(dz if a else None), _ptr(db),
+                                     rows, cols, d, _ptr(ws), nb, _stream()), "linear_act_bwd")
+    return dz, db
+
+
+def linear_bwd(dz: torch.Tensor, x, w: torch.Tensor, need_dx: bool = True):
+    """(dx, dw) of z = x w^T: dx = dz w in dz's type (None with need_dx=False), dw = dz^T x fp32 [out][in].  x: the forward's input, or its 8-bit
+    checkpoint (act8_pack) -- the weight gradient then reads the codes."""
+    rows, cout = _rows_of(dz, "linear_bwd")
+    lib = _lib_dev()
+    if w.dim() != 2:
+        raise _lib.SimhandHipError(f"linear_bwd: w must be [out][in], got {tuple(w.shape)}")
+    cin = w.shape[1]
+    d = dt(dz.dtype)
+    pw = _like(w, dz, (cout, cin), dz.dtype, "linear_bwd (w)")
+    xshape = dz.shape[:-1] + (cin,)
+    px, pc, pe = _saved(x, dz, xshape, "linear_bwd (x)")
+    pz = _ptr(dz)
+    dx = None
+    if need_dx:
+        dx = torch.empty(xshape, dtype=dz.dtype, device=dz.device)
+        nb = lib.simhand_linear_dgrad_workspace_bytes(cin, cout, d)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dz.device)
+        check(lib.simhand_linear_dgrad(pz, pw, _ptr(dx), rows, cin, cout, d, _ptr(ws), nb, _stream()), "linear_dgrad")
+    dw = torch.empty(cout, cin, dtype=torch.float32, device=dz.device)
+    nb = lib.simhand_linear_wgrad_workspace_bytes(rows, cin, cout, d)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dz.device)
+    check(lib.simhand_linear_wgrad(pz, px, pc, pe, _ptr(dw), rows, cin, cout, d, _ptr(ws), nb, _stream()), "linear_wgrad")
+    return dx, dw
+
+
+def act8_pack(x: torch.Tensor) -> Act8:
+    """x [..., cols] -> its 8-bit checkpoint (1.03 bytes a value): see Act8.  Inf and NaN are kept as NaN."""
+    rows, cols = _rows_of(x, "act8_pack")
+    lib = _lib_dev()
+    codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+    exps = torch.empty(rows, (cols + 31) // 32, dtype=torch.uint8, device=x.device)
+    check(lib.simhand_act8_pack(_ptr(x), _ptr(codes), _ptr(exps), rows, cols, dt(x.dtype), _stream()), "act8_pack")
+    return Act8(codes, exps, x.dtype)
+
+
+def act8_unpack(a: Act8) -> torch.Tensor:
+    """The values an 8-bit checkpoint stands for, in the type it was packed from."""
+    rows, cols = _rows_of(a, "act8_unpack")
+    lib = _lib_dev()
+    x = torch.empty(a.shape, dtype=a.dtype, device=a.device)
+    check(lib.simhand_act8_unpack(_ptr(a.codes), _ptr(a.exps), _ptr(x), rows, cols, dt(a.dtype), _stream()), "act8_unpack")
+    return x
+
+
 # ------------------------------------------------------------------------ conv
 def conv_desc(n, h, w, cin, cout, r, s, stride, pad, dtype: torch.dtype) -> ConvDesc:
     ho = (h + 2 * pad - r) // stride + 1
