@@ -83,7 +83,8 @@ def build_parser(description: str = "Script for training baseline supervised mod
     return p
 
 
-BUILD_ONLY_FLAGS = ("synthetic", "synthetic_raw", "synthetic_samples", "precision", "image_size", "max_steps", "out_dir", "sync_batchnorm")
+BUILD_ONLY_FLAGS = ("synthetic", "synthetic_raw", "synthetic_samples", "precision", "image_size", "max_steps", "out_dir", "sync_batchnorm",
+                    "projection_head_norm", "act8")
 
 
 def add_build_flags(p: argparse.ArgumentParser) -> argparse.ArgumentParser:
@@ -99,6 +100,10 @@ def add_build_flags(p: argparse.ArgumentParser) -> argparse.ArgumentParser:
     p.add_argument("--out_dir", type=str, default=None, help="where checkpoints go (default $SAVED_MODELS_BASE_PATH or ./runs)")
     p.add_argument("--sync_batchnorm", action="store_true",
                    help="multi-GPU: BatchNorm statistics over the global batch instead of per rank (PL's Trainer(sync_batchnorm=True))")
+    p.add_argument("--projection_head_norm", type=str, default=None, choices=["batch", "layer"],
+                   help="normalisation inside the projection head: batch = the reference's BatchNorm1d (default), layer = LayerNorm (each row by itself)")
+    p.add_argument("--act8", action="store_true",
+                   help="keep saved activations in 8 bits: the encoder's block inputs, and a layer-norm head's (less memory per image)")
     return p
 
 

@@ -90,6 +90,8 @@ def main(argv=None):
         data = SyntheticPairs(samples, train_param.batch_size, size, rank, world, train_param.seed, device)
 
     model_param = update_model_params(model_param, args, samples, train_param)
+    model_param.projection_head_norm = args.projection_head_norm or "batch"
+    model_param.act8 = args.act8
     model_param.augmentation = [k for k, v in train_param.augmentation_flags.items() if v]
     say(f"Model parameters {pformat(dict(model_param))}")
     mode = "train" if not args.resume and not args.eval else "eval"

@@ -91,6 +91,82 @@ def projection_stats(head_out_view: Tensor, name: str) -> dict:
 
 
 # --------------------------------------------------------------------------
+# row operators with their gradients: linear, layer norm, 8-bit checkpoints
+# --------------------------------------------------------------------------
+def _keep(ctx, x: Tensor, act8: bool, *others):
+    """Saves x -- as it is, or its 8-bit codes -- and whatever else the backward pass reads."""
+    ctx.x_dtype = x.dtype
+    ctx.act8 = act8
+    if act8:
+        c = ops.act8_pack(x)
+        ctx.save_for_backward(c.codes, c.exps, *others)
+    else:
+        ctx.save_for_backward(x, *others)
+
+
+def _kept(ctx):
+    t = ctx.saved_tensors
+    return (ops.Act8(t[0], t[1], ctx.x_dtype), t[2:]) if ctx.act8 else (t[0], t[1:])
+
+
+class _LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, act, residual, act8):
+        x = x.contiguous()
+        wc = w.detach().to(x.dtype).contiguous()
+        b = None if bias is None else bias.detach().float().contiguous()
+        plain = act in (None, "none")
+        out = ops.linear_fwd(x, wc, b, act=act, residual=None if residual is None else residual.contiguous(), want_pre=not plain)
+        y, pre = (out, None) if plain else out
+        _keep(ctx, x, act8, wc, *(() if plain else (pre,)))
+        ctx.act, ctx.dtypes = act, (w.dtype, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, rest = _kept(ctx)
+        need_x, need_w, need_b, _, need_r, _ = ctx.needs_input_grad
+        dy = dy.to(ctx.x_dtype).contiguous()
+        pre = rest[1] if len(rest) > 1 else None
+        dz, db = ops.linear_act_bwd(dy, pre, ctx.act) if (need_b or pre is not None) else (dy, None)
+        dx = dw = None
+        if need_x or need_w:
+            dx, dw = ops.linear_bwd(dz, x, rest[0], need_dx=need_x)
+        return (dx, dw.to(ctx.dtypes[0]) if need_w else None, db.to(ctx.dtypes[1]) if need_b else None, None, dy if need_r else None, None)
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps, relu, act8):
+        x = x.contiguous()
+        g, b = gamma.detach().float().contiguous(), beta.detach().float().contiguous()
+        y, mean, rstd = ops.layer_norm_fwd(x, g, b, eps, relu)
+        _keep(ctx, x, act8, g, b, mean, rstd)
+        ctx.relu, ctx.dtypes = relu, (gamma.dtype, beta.dtype)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, (g, b, mean, rstd) = _kept(ctx)
+        dx, dg, db = ops.layer_norm_bwd(dy.to(ctx.x_dtype).contiguous(), x, g, b, mean, rstd, ctx.relu)
+        return dx, dg.to(ctx.dtypes[0]), db.to(ctx.dtypes[1]), None, None, None
+
+
+def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: Optional[str] = None, residual: Optional[Tensor] = None,
+           act8: bool = False) -> Tensor:
+    """act(x weight^T + bias) + residual (act: none, relu, gelu, silu) with gradients of every tensor argument; x [..., in] in fp32 or the library's 16-bit type, weight
+    [out][in] (a fp32 master is rounded to x's type for the product, its gradient stays fp32).  act8: x is kept for the backward pass in 8 bits."""
+    return _LinearFn.apply(x, weight, bias, act, residual, bool(act8) and torch.is_grad_enabled())
+
+
+def layer_norm(x: Tensor, weight: Tensor, bias: Tensor, eps: float = 1e-5, relu: bool = False, act8: bool = False) -> Tensor:
+    """Layer norm over the last dimension (relu: with the ReLU behind it) with gradients of x, weight and bias.  act8: x is kept in 8 bits."""
+    return _LayerNormFn.apply(x, weight, bias, eps, bool(relu), bool(act8) and torch.is_grad_enabled())
+
+
+# --------------------------------------------------------------------------
 # adaptive weights, explicit surface (a10)
 # --------------------------------------------------------------------------
 def _joint_rows(j1: Tensor, j2: Tensor) -> Tuple[Tensor, int, str]:

@@ -187,6 +187,10 @@ class ResNetEngine:
         # bn1 + ReLU of a Bottleneck applied inside conv2's launch where that 3x3 kernel keeps its activation rows in an LDS ring (the
         # 64- and 128-channel stride-1 layers): the bn_apply pass of those units disappears (attribute: A/B timing only)
         self.bn_on_load = True
+        # saved activations in 8 bits (ops.act8_pack): the input of every block without a shortcut convolution -- the widest tensor its backward pass
+        # reads, and there only for its first convolution's weight gradient -- is kept as codes once its block's forward has run: 1.03 instead of 2 (fp32: 4) bytes
+        # a value.  A 1x1 convolution's weight gradient reads the codes themselves (ops.linear_wgrad), a 3x3's a transient copy.
+        self.act8 = False
         # multi-GPU: host.dist.OverlappedGradReducer -- finished parameter gradients go out block by block during backward
         self.grad_reducer = None
 
@@ -508,6 +512,10 @@ class ResNetEngine:
                 x = self._conv_bn(conv, bn, t, True, idn, training, saved, chain_conv=chain_conv)
                 if want_ctx:
                     ctx["blocks"].append((saved, dsaved[0] if dsaved else None))
+                    if self.act8 and blk.downsample is None:
+                        saved[0].x = ops.act8_pack(inp)
+                        if len(ctx["blocks"]) > 1 and ctx["blocks"][-2][0][-1].mask is not None:
+                            ctx["blocks"][-2][0][-1].a = None  # the last holder of inp (the backward pass gates by the mask alone)
         enc = ops.avgpool_fwd(x)
         if want_ctx:
             ctx["last_shape"] = tuple(x.shape)
@@ -625,6 +633,16 @@ class ResNetEngine:
         ops.scatter2_add(dsub, dx, below.mask if masked_store else None)
         return dx
 
+    @staticmethod
+    def _wgrad(u: _Unit, dy):
+        """Weight gradient in OIHW from the unit's saved input, which may be its 8-bit checkpoint."""
+        w, x = u.conv.weight, u.x
+        if isinstance(x, ops.Act8):
+            if u.conv.kernel_size == (1, 1) and u.conv.stride == (1, 1) and u.conv.padding == (0, 0):
+                return ops.linear_wgrad(dy, x).view(w.shape)
+            x = ops.act8_unpack(x)
+        return ops.conv2d_wgrad_oihw(u.desc, x, dy, tuple(w.shape))  # split-K reduce writes weight.grad's layout
+
     def _unit_bwd(self, u: _Unit, da, grads: dict, need_dx: bool, dx_into=None, relu_mask=None, res_grad=None, res_mask=None,
                   raw_partial=None, prev: Optional[_Unit] = None, prev_masked_store: bool = False, sub_grad=None):
         """BN bwd -> wgrad (+ dgrad).  relu_mask: bit mask that gates `da` (residual units: their own output mask;
@@ -640,7 +658,7 @@ class ResNetEngine:
             raise RuntimeError("this unit ran the folded forward (its raw conv output was never stored): its backward must be folded too")
         w = u.conv.weight
         fuse_apply = (self.fuse_bwd_apply_wgrad and self.dtype in _H16 and not u.stem and relu_mask is None and not u.has_res
-                      and u.conv.kernel_size == (1, 1) and u.conv.stride == (1, 1) and u.conv.padding == (0, 0))
+                      and u.conv.kernel_size == (1, 1) and u.conv.stride == (1, 1) and u.conv.padding == (0, 0) and not isinstance(u.x, ops.Act8))
         fuse_dg = (self.fuse_bwd_apply_dgrad and not fuse_apply and self.dtype in _H16 and not u.stem and relu_mask is None
                    and not u.has_res and need_dx and prev is not None and prev_masked_store and u.conv.kernel_size == (1, 1)
                    and u.conv.stride == (1, 1) and u.conv.padding == (0, 0) and ops.conv2d_dgrad_dysrc_ok(d))
@@ -666,7 +684,7 @@ class ResNetEngine:
             dxm, _ = ops.conv2d_dgrad_ex(d, None, pk.crsk, dx=dx_into, accumulate=dx_into is not None, res_grad=res_grad, res_mask=res_mask,
                                          fuse_mode=4, prev_mask=prev.mask, want_sums=False,
                                          dy_src=(da.contiguous(), u.y, u.st, coefs, u.relu, dy), sub_grad=sub_grad)
-            grads[w] = ops.conv2d_wgrad_oihw(d, u.x, dy, tuple(w.shape))
+            grads[w] = self._wgrad(u, dy)
             return dxm, None
         if fuse_apply:
             grads[w], dy = ops.conv2d_wgrad_bnbwd(d, u.x, da, u.y, u.st, coefs, u.relu, tuple(w.shape))
@@ -676,7 +694,7 @@ class ResNetEngine:
             # fp8 configuration: both operands already exist as e4m3 codes (x from the forward's BatchNorm-apply, dy from the pass above)
             grads[w] = ops.conv2d_wgrad_fp8(d, u.xq[0], dyq, u.xq[1], f8[0].state)
         else:
-            grads[w] = ops.conv2d_wgrad_oihw(d, u.x, dy, tuple(w.shape))  # split-K reduce writes weight.grad's layout
+            grads[w] = self._wgrad(u, dy)
         if not need_dx:
             return None, None
         pk = self._pack(u.conv, need_t=True)
@@ -810,7 +828,12 @@ class ResNetModel(nn.Module):
                                       nn.AdaptiveAvgPool2d((1, 1)))
         self.final_layer = nn.Sequential(nn.Linear(m.fc.in_features, 21 * 3 + 1))
         self.out_features = m.fc.in_features
+        self.act8 = False
         self.engine = ResNetEngine(self.features, compute_dtype)
+
+    def set_act8(self, on: bool) -> None:
+        """Keep the blocks' saved inputs in 8 bits (ResNetEngine.act8)."""
+        self.act8 = self.engine.act8 = bool(on)
 
     def set_compute_dtype(self, dtype: torch.dtype, fp8: bool = False) -> None:
         """torch.float32 (exact-fp32 parity mode), torch.bfloat16, or torch.float16 (the reference's precision=16 storage type: selects
@@ -818,6 +841,7 @@ class ResNetModel(nn.Module):
         if dtype in _H16:
             _lib.use_half("f16" if dtype == torch.float16 else "bf16")
         self.engine = ResNetEngine(self.features, dtype, fp8=fp8)
+        self.engine.act8 = self.act8
 
     def forward(self, x) -> Tensor:
         """x: image batch, or a tuple of batches (the two views) encoded as their concatenation -- the stem reads each

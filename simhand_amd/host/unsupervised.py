@@ -82,6 +82,10 @@ class SimCLR(BaseModel):
         super().__init__(config, logger_debug, mode)
         self.save_hyperparameters()
         self.projection_head = self.get_projection_head()
+        # act8 (not in the reference; default off): saved activations in 8 bits -- the encoder's block inputs, and a layer-norm head's
+        self.act8 = bool(getattr(self.config, "act8", False))
+        if self.act8:
+            self.encoder.set_act8(True)
         self.mode = mode
         self.process_group = None  # torch.distributed group for the global negative set (None = default / single)
 
@@ -89,9 +93,14 @@ class SimCLR(BaseModel):
         # quirk honoured: for resnet 18/34 the JSON's projection_head_input_dim (2048) is wrong and
         # nothing in the reference fixes it -> follow the encoder's width
         in_dim = getattr(self.encoder, "out_features", self.config.projection_head_input_dim)
+        # projection_head_norm (not in the reference; default "batch" = its head): "layer" normalises every row by itself -- the projections of an image
+        # then depend on no other image, so they are the same on any number of ranks without a collective
+        norm = getattr(self.config, "projection_head_norm", None) or "batch"
+        if norm not in ("batch", "layer"):
+            raise ValueError(f"projection_head_norm must be 'batch' or 'layer', got {norm!r}")
         return nn.Sequential(
             nn.Linear(in_dim, self.config.projection_head_hidden_dim, bias=True),
-            nn.BatchNorm1d(self.config.projection_head_hidden_dim),
+            (nn.BatchNorm1d if norm == "batch" else nn.LayerNorm)(self.config.projection_head_hidden_dim),
             nn.ReLU(),
             nn.Linear(self.config.projection_head_hidden_dim, self.config.output_dim, bias=False),
         )
@@ -102,6 +111,10 @@ class SimCLR(BaseModel):
 
     def _head(self, enc: Tensor) -> Tensor:
         ph = self.projection_head
+        if isinstance(ph[1], nn.LayerNorm):
+            h = mu.linear(enc, ph[0].weight, ph[0].bias, act8=self.act8)
+            h = mu.layer_norm(h, ph[1].weight, ph[1].bias, ph[1].eps, relu=True, act8=self.act8)
+            return mu.linear(h, ph[3].weight, act8=self.act8)
         return _HeadFn.apply(enc, ph, self.training, ph[0].weight, ph[0].bias, ph[1].weight, ph[1].bias, ph[3].weight)
 
     def get_projection_stats(self, projection: Tensor, name: str) -> dict:

@@ -330,19 +330,32 @@ def linear_bwd(dz: torch.Tensor, x, w: torch.Tensor, need_dx: bool = True):
     d = dt(dz.dtype)
     pw = _like(w, dz, (cout, cin), dz.dtype, "linear_bwd (w)")
     xshape = dz.shape[:-1] + (cin,)
-    px, pc, pe = _saved(x, dz, xshape, "linear_bwd (x)")
-    pz = _ptr(dz)
+    if tuple(x.shape) != tuple(xshape):
+        raise _lib.SimhandHipError(f"linear_bwd: x must be {tuple(xshape)}, got {tuple(x.shape)}")
     dx = None
     if need_dx:
         dx = torch.empty(xshape, dtype=dz.dtype, device=dz.device)
         nb = lib.simhand_linear_dgrad_workspace_bytes(cin, cout, d)
         ws = torch.empty(nb, dtype=torch.uint8, device=dz.device)
-        check(lib.simhand_linear_dgrad(pz, pw, _ptr(dx), rows, cin, cout, d, _ptr(ws), nb, _stream()), "linear_dgrad")
+        check(lib.simhand_linear_dgrad(_ptr(dz), pw, _ptr(dx), rows, cin, cout, d, _ptr(ws), nb, _stream()), "linear_dgrad")
+    return dx, linear_wgrad(dz, x)
+
+
+def linear_wgrad(dz: torch.Tensor, x) -> torch.Tensor:
+    """dw = dz^T x fp32 [out][in] alone; dz [..., out], x [..., in] or its 8-bit checkpoint.  Also the weight gradient of a 1x1 / stride-1 convolution whose
+    input was kept in 8 bits: dz and x with pixels as rows."""
+    rows, cout = _rows_of(dz, "linear_wgrad")
+    lib = _lib_dev()
+    d = dt(dz.dtype)
+    if len(x.shape) < 1 or x.shape[-1] < 1:
+        raise _lib.SimhandHipError(f"linear_wgrad: rows of at least one value, got x of shape {tuple(x.shape)}")
+    cin = x.shape[-1]
+    px, pc, pe = _saved(x, dz, dz.shape[:-1] + (cin,), "linear_wgrad (x)")
     dw = torch.empty(cout, cin, dtype=torch.float32, device=dz.device)
     nb = lib.simhand_linear_wgrad_workspace_bytes(rows, cin, cout, d)
     ws = torch.empty(nb, dtype=torch.uint8, device=dz.device)
-    check(lib.simhand_linear_wgrad(pz, px, pc, pe, _ptr(dw), rows, cin, cout, d, _ptr(ws), nb, _stream()), "linear_wgrad")
-    return dx, dw
+    check(lib.simhand_linear_wgrad(_ptr(dz), px, pc, pe, _ptr(dw), rows, cin, cout, d, _ptr(ws), nb, _stream()), "linear_wgrad")
+    return dw
 
 
 def act8_pack(x: torch.Tensor) -> Act8:
