@@ -1,0 +1,71 @@
+// What the linear operator's kernels share (linear.hip, linear256.hip).
+#pragma once
+#include "rows.h"
+
+namespace sh {
+
+template <typename T> __device__ __forceinline__ f32x4 mma16(const uint4& a, const uint4& b, f32x4 c) {
+  if constexpr (sizeof(T) == 2) {
+    return sh_mfma16(a, b, c);
+  } else {  // 16 bytes = 4 fp32: MFMA e takes element e of both operands (the same k order on both sides)
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
+  }
+}
+
+struct LinearArgs {
+  const void* a;        // [M][K]
+  const void* b;        // [N][ldb]
+  void* out;            // [M][N]
+  void* pre;            // [M][N] or null
+  const float* bias;    // [N] or null
+  const void* residual; // [M][N] or null
+  long long M;
+  int N, K, ldb, act;
+  unsigned n_tiles;
+};
+
+// tile column that row m of MFMA tile ni holds: lane group g of the tiles 2 j, 2 j + 1 ends with columns 32 j + 8 g .. + 7
+__device__ __forceinline__ int lin_col(int ni, int m) { return (ni >> 1) * 32 + (m >> 2) * 8 + (ni & 1) * 4 + (m & 3); }
+
+// the 8 finished sums of one row: z = acc + bias, pre <- z, out <- act(z) + residual
+template <typename T>
+__device__ __forceinline__ void linear_store8(const LinearArgs& p, long long row, int n, const float (&acc)[8]) {
+  constexpr int VE = Vec16<T>::N;
+  const int left = p.N - n;
+  if (left <= 0) return;
+  float z[8];
+  float b[8];
+  if (p.bias != nullptr) ld_f32<8>(p.bias + n, left, b);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) z[e] = p.bias != nullptr ? acc[e] + b[e] : acc[e];
+  const long long at = row * p.N + n;
+#pragma unroll
+  for (int h = 0; h < 8 / VE; ++h) {
+    const int l = left - h * VE;
+    if (l <= 0) break;
+    float o[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) o[e] = z[h * VE + e];
+    if (p.pre != nullptr) st_chunk<T>((T*)p.pre + at + h * VE, l, pack16<T>(o));
+    if (p.act != SH_ACT_NONE) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) o[e] = act_value(o[e], p.act);
+    }
+    if (p.residual != nullptr) {
+      float r[VE];
+      unpack16<T>(ld_chunk<T>((const T*)p.residual + at + h * VE, l), r);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) o[e] += r[e];
+    }
+    st_chunk<T>((T*)p.out + at + h * VE, l, pack16<T>(o));
+  }
+}
+
+// 256 x 256 tiles, 16-bit operands (linear256.hip)
+bool linear256_takes(const LinearArgs& p, int dtype);
+int linear256_launch(const LinearArgs& p, hipStream_t s, const char* what);
+
+}  // namespace sh

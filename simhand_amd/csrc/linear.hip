@@ -9,144 +9,156 @@
 // the tile, so that a lane ends with 8 consecutive columns of one row: bias, residual, pre-activation and output move as 16-byte vectors.
 // linear_wgrad_kernel: dw [N][K] = dz^T x, the reduction runs over rows: tiles of 128 x 128 over a range of rows (split), 16-bit operands are read transposed from LDS
 // (ds_read_b64_tr_b16); the splits' fp32 partial sums are added in a fixed order by a second launch.
-#include "rows.h"
+#include "linear.h"
 
 namespace sh {
 
-template <typename T> __device__ __forceinline__ f32x4 mma16(const uint4& a, const uint4& b, f32x4 c) {
-  if constexpr (sizeof(T) == 2) {
-    return sh_mfma16(a, b, c);
-  } else {  // 16 bytes = 4 fp32: MFMA e takes element e of both operands (the same k order on both sides)
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
-  }
-}
-
-struct LinearArgs {
-  const void* a;        // [M][K]
-  const void* b;        // [N][ldb]
-  void* out;            // [M][N]
-  void* pre;            // [M][N] or null
-  const float* bias;    // [N] or null
-  const void* residual; // [M][N] or null
-  long long M;
-  int N, K, ldb, act;
-  unsigned n_tiles;
-};
-
-// tile column that row m of MFMA tile ni holds: lane group g of the tiles 2 j, 2 j + 1 ends with columns 32 j + 8 g .. + 7
-__device__ __forceinline__ int lin_col(int ni, int m) { return (ni >> 1) * 32 + (m >> 2) * 8 + (ni & 1) * 4 + (m & 3); }
-
-// the 8 finished sums of one row: z = acc + bias, pre <- z, out <- act(z) + residual
-template <typename T>
-__device__ __forceinline__ void linear_store8(const LinearArgs& p, long long row, int n, const float (&acc)[8]) {
-  constexpr int VE = Vec16<T>::N;
-  const int left = p.N - n;
-  if (left <= 0) return;
-  float z[8];
-  float b[8];
-  if (p.bias != nullptr) ld_f32<8>(p.bias + n, left, b);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) z[e] = p.bias != nullptr ? acc[e] + b[e] : acc[e];
-  const long long at = row * p.N + n;
-#pragma unroll
-  for (int h = 0; h < 8 / VE; ++h) {
-    const int l = left - h * VE;
-    if (l <= 0) break;
-    float o[VE];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) o[e] = z[h * VE + e];
-    if (p.pre != nullptr) st_chunk<T>((T*)p.pre + at + h * VE, l, pack16<T>(o));
-    if (p.act != SH_ACT_NONE) {
-#pragma unroll
-      for (int e = 0; e < VE; ++e) o[e] = act_value(o[e], p.act);
-    }
-    if (p.residual != nullptr) {
-      float r[VE];
-      unpack16<T>(ld_chunk<T>((const T*)p.residual + at + h * VE, l), r);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) o[e] += r[e];
-    }
-    st_chunk<T>((T*)p.out + at + h * VE, l, pack16<T>(o));
-  }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256, 2) void linear_gemm_kernel(LinearArgs p) {
+// TILE = 128: each of the 4 waves a 64 x 64 quarter; 64: a 32 x 32 quarter
+template <typename T, int TILE>
+__global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_gemm_kernel(LinearArgs p) {
   constexpr int VE = Vec16<T>::N, KE = 128 / sizeof(T);  // elements per 16-byte chunk / per k-step (a tile row is 8 chunks)
-  __shared__ __attribute__((aligned(16))) char smem[2 * 128 * 128];
+  constexpr int Q = TILE / 32, HALF = TILE / 2;          // MFMA tiles per wave and direction, also staging rounds
+  __shared__ __attribute__((aligned(16))) char smem[2 * TILE * 128];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int li = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
   const unsigned logical = xcd_order(blockIdx.x, gridDim.x);
-  const int n0 = (int)(logical % p.n_tiles) * 128;  // the n-tiles of a row tile are neighbours on one XCD: a is read from HBM once
-  const long long m0 = (long long)(logical / p.n_tiles) * 128;
-  const T* __restrict__ A = (const T*)p.a;
-  const T* __restrict__ B = (const T*)p.b;
-  // staging: thread = chunk tid & 7 of rows (tid >> 3) + 32 i of either operand; LDS chunk position = chunk ^ (row's key)
+  const int n0 = (int)(logical % p.n_tiles) * TILE;  // the n-tiles of a row tile are neighbours on one XCD: a is read from HBM once
+  const long long m0 = (long long)(logical / p.n_tiles) * TILE;
+  // staging: thread = chunk tid & 7 of rows (tid >> 3) + 32 i of either operand; LDS chunk position = chunk ^ (row's key).  Rows past the end repeat the last one (their
+  // sums are never stored).
   const int sc = tid & 7, sr = tid >> 3;
-  uint4 ra[4], rb[4];
-  auto load = [&](int k0) {
-    const int k = k0 + sc * VE, left = p.K - k;
+  const T* pa[Q];
+  const T* pb[Q];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long long m = m0 + sr + 32 * i;
-      const int n = n0 + sr + 32 * i;
-      ra[i] = (m < p.M && left > 0) ? ld_chunk<T>(A + m * p.K + k, left) : make_uint4(0u, 0u, 0u, 0u);
-      rb[i] = (n < p.N && left > 0) ? ld_chunk<T>(B + (long long)n * p.ldb + k, left) : make_uint4(0u, 0u, 0u, 0u);
+  for (int i = 0; i < Q; ++i) {
+    const long long m = m0 + sr + 32 * i;
+    const int n = n0 + sr + 32 * i;
+    pa[i] = (const T*)p.a + (m < p.M ? m : p.M - 1) * p.K;
+    pb[i] = (const T*)p.b + (long long)(n < p.N ? n : p.N - 1) * p.ldb;
+  }
+  uint4 ra[Q], rb[Q];
+  auto load = [&](int k0) {
+    const int k = k0 + sc * VE;
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      ra[i] = ld_kchunk<T>(pa[i], k, p.K);
+      rb[i] = ld_kchunk<T>(pb[i], k, p.K);
     }
   };
   auto key_b = [](int row) { return ((row >> 1) & 1) | (((row >> 3) & 3) << 1); };
-  f32x4 acc[4][4];
+  f32x4 acc[Q][Q];
 #pragma unroll
-  for (int mi = 0; mi < 4; ++mi)
+  for (int mi = 0; mi < Q; ++mi)
 #pragma unroll
-    for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
   load(0);
   for (int k0 = 0; k0 < p.K; k0 += KE) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < Q; ++i) {
       const int row = sr + 32 * i;
       *reinterpret_cast<uint4*>(smem + row * 128 + ((sc ^ ((row >> 1) & 7)) * 16)) = ra[i];
-      *reinterpret_cast<uint4*>(smem + 16384 + row * 128 + ((sc ^ key_b(row)) * 16)) = rb[i];
+      *reinterpret_cast<uint4*>(smem + TILE * 128 + row * 128 + ((sc ^ key_b(row)) * 16)) = rb[i];
     }
     __syncthreads();
     if (k0 + KE < p.K) load(k0 + KE);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      uint4 fa[4], fb[4];
+      uint4 fa[Q], fb[Q];
 #pragma unroll
-      for (int mi = 0; mi < 4; ++mi) {
-        const int row = wm * 64 + mi * 16 + li;
+      for (int mi = 0; mi < Q; ++mi) {
+        const int row = wm * HALF + mi * 16 + li;
         fa[mi] = *reinterpret_cast<const uint4*>(smem + row * 128 + (((kk * 4 + g) ^ ((row >> 1) & 7)) * 16));
       }
 #pragma unroll
-      for (int ni = 0; ni < 4; ++ni) {
-        const int row = wn * 64 + lin_col(ni, li);
-        fb[ni] = *reinterpret_cast<const uint4*>(smem + 16384 + row * 128 + (((kk * 4 + g) ^ key_b(row)) * 16));
+      for (int ni = 0; ni < Q; ++ni) {
+        const int row = wn * HALF + lin_col(ni, li);
+        fb[ni] = *reinterpret_cast<const uint4*>(smem + TILE * 128 + row * 128 + (((kk * 4 + g) ^ key_b(row)) * 16));
       }
 #pragma unroll
-      for (int mi = 0; mi < 4; ++mi)
+      for (int mi = 0; mi < Q; ++mi)
 #pragma unroll
-        for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = mma16<T>(fb[ni], fa[mi], acc[mi][ni]);
+        for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = mma16<T>(fb[ni], fa[mi], acc[mi][ni]);
     }
   }
 #pragma unroll
-  for (int mi = 0; mi < 4; ++mi) {
-    const long long row = m0 + wm * 64 + mi * 16 + li;
+  for (int mi = 0; mi < Q; ++mi) {
+    const long long row = m0 + wm * HALF + mi * 16 + li;
     if (row >= p.M) continue;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < Q / 2; ++j) {
       float v[8];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         v[r] = acc[mi][2 * j][r];
         v[4 + r] = acc[mi][2 * j + 1][r];
       }
-      linear_store8<T>(p, row, n0 + wn * 64 + j * 32 + g * 8, v);
+      linear_store8<T>(p, row, n0 + wn * HALF + j * 32 + g * 8, v);
     }
+  }
+}
+
+// Few rows: a block of 8 waves makes 16 columns of up to 16 MT rows; every wave takes each eighth 64-byte piece of K, both operands go from memory straight into MFMA
+// operands (no LDS: nothing is used twice), and the waves' sums meet in LDS.  What counts here is latency and the number of CUs that read w: 16 columns a block
+// put 32 blocks on 512 columns.
+template <typename T, int MT>
+__global__ __launch_bounds__(512) void linear_skinny_kernel(LinearArgs p) {
+  constexpr int VE = Vec16<T>::N, KE = 4 * VE, W = 8;  // elements of a lane group's four chunks
+  __shared__ float red[W][MT][16][17];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const long long m0 = (long long)blockIdx.y * (16 * MT);
+  const T* pb = (const T*)p.b + (long long)(n0 + li < p.N ? n0 + li : p.N - 1) * p.ldb;
+  const T* pa[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const long long m = m0 + 16 * t + li;
+    pa[t] = (const T*)p.a + (m < p.M ? m : p.M - 1) * p.K;
+  }
+  f32x4 acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  const int k_first = wave * KE + g * VE;
+  constexpr int U = MT >= 4 ? 2 : 4;  // pieces in flight
+  int k0 = k_first;
+  for (; k0 - g * VE + (U - 1) * W * KE + KE <= p.K; k0 += U * W * KE) {  // U whole pieces
+    uint4 b[U], a[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      b[u] = ld16_any(pb + k0 + u * W * KE);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) a[u][t] = ld16_any(pa[t] + k0 + u * W * KE);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) acc[t] = mma16<T>(a[u][t], b[u], acc[t]);
+  }
+  for (; k0 - g * VE < p.K; k0 += W * KE) {
+    const uint4 b = ld_kchunk<T>(pb, k0, p.K);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = mma16<T>(ld_kchunk<T>(pa[t], k0, p.K), b, acc[t]);
+  }
+  // D[row m = 4 g + r][column n = li]
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) red[wave][t][4 * g + r][li] = acc[t][r];
+  __syncthreads();
+  for (int i = tid; i < MT * 16 * 16; i += 512) {
+    const int n = i & 15, m = (i >> 4) & 15, t = i >> 8;
+    const long long row = m0 + 16 * t + m;
+    const int col = n0 + n;
+    if (row >= p.M || col >= p.N) continue;
+    float z = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) z += red[w][t][m][n];
+    if (p.bias != nullptr) z += p.bias[col];
+    const long long at = row * p.N + col;
+    if (p.pre != nullptr) Elem<T>::store((T*)p.pre + at, z);
+    z = act_value(z, p.act);
+    if (p.residual != nullptr) z += Elem<T>::load((const T*)p.residual + at);
+    Elem<T>::store((T*)p.out + at, z);
   }
 }
 
@@ -366,12 +378,37 @@ static int linear_bad(const char* what, int64_t rows, int in, int out, int dtype
   return 0;
 }
 
+// Which kernel: few rows -> the skinny one (rows <= 64 and so little work that tiles would leave most CUs idle); 64-wide tiles while 128-wide ones would not put two
+// blocks on each of the 256 CUs; else 128-wide ones.
 static int gemm_launch(const LinearArgs& base, int dtype, hipStream_t s, const char* what) {
   LinearArgs p = base;
-  p.n_tiles = (unsigned)ceil_div(p.N, 128);
-  const unsigned grid = (unsigned)ceil_div(p.M, 128) * p.n_tiles;
-  if (dtype == SH_F32) linear_gemm_kernel<float><<<grid, 256, 0, s>>>(p);
-  else linear_gemm_kernel<bf16_t><<<grid, 256, 0, s>>>(p);
+  if (p.M <= 64 && ceil_div(p.N, 64) < 256) {
+    const int mt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
+    const dim3 grid(ceil_div(p.N, 16), 1);
+#define SH_SKINNY(T, MT) linear_skinny_kernel<T, MT><<<grid, 512, 0, s>>>(p)
+    if (dtype == SH_F32) {
+      if (mt == 1) SH_SKINNY(float, 1);
+      else if (mt == 2) SH_SKINNY(float, 2);
+      else SH_SKINNY(float, 4);
+    } else {
+      if (mt == 1) SH_SKINNY(bf16_t, 1);
+      else if (mt == 2) SH_SKINNY(bf16_t, 2);
+      else SH_SKINNY(bf16_t, 4);
+    }
+#undef SH_SKINNY
+    return check_launch(what);
+  }
+  if (linear256_takes(p, dtype)) return linear256_launch(p, s, what);
+  const int tile = (int64_t)ceil_div(p.M, 128) * ceil_div(p.N, 128) >= 512 ? 128 : 64;
+  p.n_tiles = (unsigned)ceil_div(p.N, tile);
+  const unsigned grid = (unsigned)ceil_div(p.M, tile) * p.n_tiles;
+  if (tile == 128) {
+    if (dtype == SH_F32) linear_gemm_kernel<float, 128><<<grid, 256, 0, s>>>(p);
+    else linear_gemm_kernel<bf16_t, 128><<<grid, 256, 0, s>>>(p);
+  } else {
+    if (dtype == SH_F32) linear_gemm_kernel<float, 64><<<grid, 256, 0, s>>>(p);
+    else linear_gemm_kernel<bf16_t, 64><<<grid, 256, 0, s>>>(p);
+  }
   return check_launch(what);
 }
 

@@ -57,6 +57,31 @@ template <typename T> __device__ __forceinline__ uint4 ld_chunk(const T* p, int 
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+// v with its first `gone` elements zeroed
+template <typename T> __device__ __forceinline__ uint4 drop_first(const uint4& v, int gone) {
+  constexpr int N = Vec16<T>::N;
+  unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (N == 8) {
+      if (gone >= 2 * i + 2) w[i] = 0u;
+      else if (gone == 2 * i + 1) w[i] &= 0xffff0000u;
+    } else {
+      if (gone > i) w[i] = 0u;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// One chunk of a reduction row (the product's K): `k` its first element, `len` the row's length.  The ragged last chunk of a row is read as the row's last N elements with
+// those that the chunk before it holds zeroed -- both operands of a product are read like this, so element e of either is the same k, and no element is
+// loaded by itself.  Rows shorter than a chunk go element by element.
+template <typename T> __device__ __forceinline__ uint4 ld_kchunk(const T* row, int k, int len) {
+  constexpr int N = Vec16<T>::N;
+  if (k + N <= len) return ld16_any(row + k);
+  if (k >= len) return make_uint4(0u, 0u, 0u, 0u);
+  if (len < N) return ld_chunk<T>(row, len);
+  return drop_first<T>(ld16_any(row + len - N), k - (len - N));
+}
 template <typename T> __device__ __forceinline__ void st_chunk(T* p, int left, const uint4& v) {
   constexpr int N = Vec16<T>::N;
   if (left >= N) {
@@ -124,19 +149,46 @@ __device__ __forceinline__ unsigned xcd_order(unsigned bid, unsigned nblk) {
   return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + j;
 }
 
-// activations of the linear operator (enum sh_act) and their derivatives, fp32.  NaN stays NaN (also through ReLU).
+// ---- activations of the linear operator (enum sh_act) and their derivatives, fp32.  NaN stays NaN (also through ReLU). ------------------------
+// exp(-z^2 / 2) and the normal distribution function Phi(z) = erfc(-z / sqrt 2) / 2.  erfc(x) = t P(t) exp(-x^2), t = 1 / (1 + x / 2), x >= 0, with P the degree-8
+// Chebyshev fit of exp(x^2) erfc(x) / t over t in [1/16, 1] (x <= 30; exp(-x^2) is zero in fp32 long before): 4e-7 relative in fp32 arithmetic over the whole
+// range, on both tails, in 17 instructions.  The library's erff costs about three times that, and an epilogue of 256 x 256 of them took as long as the
+// product it follows.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+  const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.35355339059327376f, 1.f));
+  float p = -0.05634250491857529f;
+  p = fmaf(p, t, 0.2723356783390045f);
+  p = fmaf(p, t, -0.4642637073993683f);
+  p = fmaf(p, t, 0.2548193037509918f);
+  p = fmaf(p, t, -0.01282817404717207f);
+  p = fmaf(p, t, 0.1978423148393631f);
+  p = fmaf(p, t, 0.2440689206123352f);
+  p = fmaf(p, t, 0.2822780907154083f);
+  p = fmaf(p, t, 0.28209006786346436f);
+  const float q = p * t * e * 0.5f;
+  return z < 0.f ? q : 1.f - q;
+}
+__device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }
 __device__ __forceinline__ float act_value(float z, int act) {
   if (act == SH_ACT_RELU) return z <= 0.f ? 0.f : z;
-  if (act == SH_ACT_GELU) return z * (0.5f * (1.f + erff(z * 0.70710678118654752f)));
-  if (act == SH_ACT_SILU) return z / (1.f + expf(-z));
+  if (act == SH_ACT_GELU) {
+    float e;
+    return z * normal_cdf(z, e);
+  }
+  if (act == SH_ACT_SILU) return z * logistic(z);
   return z;
 }
 __device__ __forceinline__ float act_slope(float z, int act) {
   if (act == SH_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-  if (act == SH_ACT_GELU) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+  if (act == SH_ACT_GELU) {
+    float e;
+    const float c = normal_cdf(z, e);
+    return fmaf(z * 0.39894228040143268f, e, c);
+  }
   if (act == SH_ACT_SILU) {
-    const float s = 1.f / (1.f + expf(-z));
-    return s * (1.f + z * (1.f - s));
+    const float s = logistic(z);
+    return s * fmaf(z, 1.f - s, 1.f);
   }
   return 1.f;
 }

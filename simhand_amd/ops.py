@@ -215,10 +215,11 @@ class Act8:
 
 def _rows_of(x, what: str) -> Tuple[int, int]:
     """(rows, cols) of a row tensor [..., cols] that lives on the current device (the launch goes to that device's current stream)."""
-    if x.device.type != "cuda":
+    dev = x.device
+    if dev.type != "cuda":
         raise _lib.SimhandHipError(f"{what}: simhand_amd ops need device tensors (there is no CPU path)")
-    if x.device.index != torch.cuda.current_device():
-        raise _lib.SimhandHipError(f"{what}: the tensor is on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if dev.index != torch.cuda.current_device():
+        raise _lib.SimhandHipError(f"{what}: the tensor is on {dev}, the current device is cuda:{torch.cuda.current_device()}")
     shape = x.shape
     if len(shape) < 1 or shape[-1] < 1:
         raise _lib.SimhandHipError(f"{what}: rows of at least one value, got shape {tuple(shape)}")
@@ -227,28 +228,44 @@ def _rows_of(x, what: str) -> Tuple[int, int]:
     return n // cols, cols
 
 
-def _like(t: Optional[torch.Tensor], x, shape, dtype: torch.dtype, what: str) -> C.c_void_p:
-    """Pointer of an operand that has to have this shape and type, on x's device (None: NULL)."""
+# Small batches are bound by the host: the row operators pass addresses and the stream as plain integers (what ctypes makes of a c_void_p anyway; 0 = NULL)
+def _row_stream(x) -> int:
+    return torch._C._cuda_getCurrentRawStream(x.device.index)
+
+
+def _at(t: torch.Tensor) -> int:
+    if not t.is_contiguous():
+        raise _lib.SimhandHipError("simhand_amd ops need contiguous tensors")
+    return t.data_ptr()
+
+
+def _like(t: Optional[torch.Tensor], x, shape, dtype: torch.dtype, what: str) -> int:
+    """Address of an operand that has to have this shape and type, on x's device (None: NULL)."""
     if t is None:
-        return C.c_void_p(0)
-    if t.device != x.device or t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        return 0
+    if t.shape != shape or t.dtype != dtype or t.device != x.device:
         raise _lib.SimhandHipError(f"{what}: expected {tuple(shape)} {dtype} on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    return _ptr(t)
+    return _at(t)
 
 
 def _saved(x, like: torch.Tensor, shape, what: str):
-    """(x, codes, exps) pointers of a saved activation: a tensor, or its 8-bit checkpoint."""
+    """(x, codes, exps) addresses of a saved activation: a tensor, or its 8-bit checkpoint."""
     if isinstance(x, Act8):
         if x.dtype != like.dtype:
             raise _lib.SimhandHipError(f"{what}: checkpoint of a {x.dtype} activation next to a {like.dtype} gradient")
-        return C.c_void_p(0), _like(x.codes, like, shape, torch.uint8, what), _ptr(x.exps, torch.uint8)
-    return _like(x, like, shape, like.dtype, what), C.c_void_p(0), C.c_void_p(0)
+        return 0, _like(x.codes, like, shape, torch.uint8, what), _at(x.exps)
+    return _like(x, like, shape, like.dtype, what), 0, 0
 
 
 def _act_id(act: Optional[str], what: str) -> int:
-    if act not in _lib.ACTS:
+    a = _lib.ACTS.get(act)
+    if a is None:
         raise _lib.SimhandHipError(f"{what}: act must be one of {sorted(k for k in _lib.ACTS if k)}, got {act!r}")
-    return _lib.ACTS[act]
+    return a
+
+
+def _scratch(nbytes: int, x) -> torch.Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=x.device)
 
 
 def layer_norm_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps: float = 1e-5, relu: bool = False):
@@ -256,11 +273,12 @@ def layer_norm_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps
     one per row, for layer_norm_bwd."""
     rows, cols = _rows_of(x, "layer_norm_fwd")
     lib = _lib_dev()
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    stat = torch.empty(2, rows, dtype=torch.float32, device=x.device)
-    mean, rstd = stat[0], stat[1]
-    check(lib.simhand_layer_norm_fwd(_ptr(x), _like(gamma, x, (cols,), _F32, "layer_norm_fwd (gamma)"), _like(beta, x, (cols,), _F32, "layer_norm_fwd (beta)"),
-                                     float(eps), int(bool(relu)), _ptr(y), _ptr(mean), _ptr(rstd), rows, cols, dt(x.dtype), _stream()), "layer_norm_fwd")
+    px, shape = _at(x), (cols,)
+    y = torch.empty_like(x)
+    mean = torch.empty(rows, dtype=_F32, device=x.device)
+    rstd = torch.empty_like(mean)
+    check(lib.simhand_layer_norm_fwd(px, _like(gamma, x, shape, _F32, "layer_norm_fwd (gamma)"), _like(beta, x, shape, _F32, "layer_norm_fwd (beta)"), eps,
+                                     1 if relu else 0, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), rows, cols, dt(x.dtype), _row_stream(x)), "layer_norm_fwd")
     return y, mean, rstd
 
 
@@ -269,17 +287,19 @@ def layer_norm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, beta: torch.Tensor,
     is recomputed from x (bit for bit the forward's when x is the tensor itself)."""
     rows, cols = _rows_of(dy, "layer_norm_bwd")
     lib = _lib_dev()
-    what = "layer_norm_bwd"
+    what, shape, stats = "layer_norm_bwd", (cols,), (rows,)
+    pdy = _at(dy)
     px, pc, pe = _saved(x, dy, dy.shape, what + " (x)")
-    dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
-    dgb = torch.empty(2, cols, dtype=torch.float32, device=dy.device)
+    dx = torch.empty_like(dy)
+    dgb = torch.empty((2, cols), dtype=_F32, device=dy.device)
     d = dt(dy.dtype)
     nb = lib.simhand_layer_norm_bwd_workspace_bytes(rows, cols, d)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dy.device)
-    check(lib.simhand_layer_norm_bwd(_ptr(dy), px, pc, pe, _like(gamma, dy, (cols,), _F32, what + " (gamma)"), _like(beta, dy, (cols,), _F32, what + " (beta)"),
-                                     _like(mean, dy, (rows,), _F32, what + " (mean)"), _like(rstd, dy, (rows,), _F32, what + " (rstd)"), int(bool(relu)),
-                                     _ptr(dx), _ptr(dgb), rows, cols, d, _ptr(ws), nb, _stream()), what)
-    return dx, dgb[0], dgb[1]
+    ws = _scratch(nb, dy)
+    check(lib.simhand_layer_norm_bwd(pdy, px, pc, pe, _like(gamma, dy, shape, _F32, what + " (gamma)"), _like(beta, dy, shape, _F32, what + " (beta)"),
+                                     _like(mean, dy, stats, _F32, what + " (mean)"), _like(rstd, dy, stats, _F32, what + " (rstd)"), 1 if relu else 0,
+                                     dx.data_ptr(), dgb.data_ptr(), rows, cols, d, ws.data_ptr(), nb, _row_stream(dy)), what)
+    dgamma, dbeta = dgb.unbind(0)
+    return dx, dgamma, dbeta
 
 
 def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
@@ -293,11 +313,12 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
         raise _lib.SimhandHipError(f"linear_fwd: w must be [out][in], got {tuple(w.shape)}")
     cout = w.shape[0]
     shape = x.shape[:-1] + (cout,)
+    px = _at(x)
+    pw, pb = _like(w, x, (cout, cin), x.dtype, "linear_fwd (w)"), _like(bias, x, (cout,), _F32, "linear_fwd (bias)")
+    pr = _like(residual, x, shape, x.dtype, "linear_fwd (residual)")
     y = torch.empty(shape, dtype=x.dtype, device=x.device)
     pre = torch.empty_like(y) if want_pre else None
-    check(lib.simhand_linear_fwd(_ptr(x), _like(w, x, (cout, cin), x.dtype, "linear_fwd (w)"), _like(bias, x, (cout,), _F32, "linear_fwd (bias)"), a,
-                                 _like(residual, x, shape, x.dtype, "linear_fwd (residual)"), _ptr(y), _ptr(pre), rows, cin, cout, dt(x.dtype), _stream()),
-          "linear_fwd")
+    check(lib.simhand_linear_fwd(px, pw, pb, a, pr, y.data_ptr(), pre.data_ptr() if want_pre else 0, rows, cin, cout, dt(x.dtype), _row_stream(x)), "linear_fwd")
     return (y, pre) if want_pre else y
 
 
@@ -310,12 +331,12 @@ def linear_act_bwd(dy: torch.Tensor, pre: Optional[torch.Tensor] = None, act: Op
     if a != 0 and pre is None:
         raise _lib.SimhandHipError("linear_act_bwd: an activation needs the saved pre-activation")
     d = dt(dy.dtype)
-    dz = torch.empty_like(dy, memory_format=torch.contiguous_format) if a else dy
-    db = torch.empty(cols, dtype=torch.float32, device=dy.device)
+    pdy, ppre = _at(dy), _like(pre if a else None, dy, dy.shape, dy.dtype, "linear_act_bwd (pre)")
+    dz = torch.empty_like(dy) if a else dy
+    db = torch.empty(cols, dtype=_F32, device=dy.device)
     nb = lib.simhand_linear_act_bwd_workspace_bytes(rows, cols, d)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dy.device)
-    check(lib.simhand_linear_act_bwd(_ptr(dy), _like(pre if a else None, dy, dy.shape, dy.dtype, "linear_act_bwd (pre)"), a, _ptr(dz if a else None), _ptr(db),
-                                     rows, cols, d, _ptr(ws), nb, _stream()), "linear_act_bwd")
+    ws = _scratch(nb, dy)
+    check(lib.simhand_linear_act_bwd(pdy, ppre, a, dz.data_ptr() if a else 0, db.data_ptr(), rows, cols, d, ws.data_ptr(), nb, _row_stream(dy)), "linear_act_bwd")
     return dz, db
 
 
@@ -330,14 +351,15 @@ def linear_bwd(dz: torch.Tensor, x, w: torch.Tensor, need_dx: bool = True):
     d = dt(dz.dtype)
     pw = _like(w, dz, (cout, cin), dz.dtype, "linear_bwd (w)")
     xshape = dz.shape[:-1] + (cin,)
-    if tuple(x.shape) != tuple(xshape):
+    if x.shape != xshape:
         raise _lib.SimhandHipError(f"linear_bwd: x must be {tuple(xshape)}, got {tuple(x.shape)}")
     dx = None
     if need_dx:
+        pz = _at(dz)
         dx = torch.empty(xshape, dtype=dz.dtype, device=dz.device)
         nb = lib.simhand_linear_dgrad_workspace_bytes(cin, cout, d)
-        ws = torch.empty(nb, dtype=torch.uint8, device=dz.device)
-        check(lib.simhand_linear_dgrad(_ptr(dz), pw, _ptr(dx), rows, cin, cout, d, _ptr(ws), nb, _stream()), "linear_dgrad")
+        ws = _scratch(nb, dz)
+        check(lib.simhand_linear_dgrad(pz, pw, dx.data_ptr(), rows, cin, cout, d, ws.data_ptr(), nb, _row_stream(dz)), "linear_dgrad")
     return dx, linear_wgrad(dz, x)
 
 
@@ -350,11 +372,12 @@ def linear_wgrad(dz: torch.Tensor, x) -> torch.Tensor:
     if len(x.shape) < 1 or x.shape[-1] < 1:
         raise _lib.SimhandHipError(f"linear_wgrad: rows of at least one value, got x of shape {tuple(x.shape)}")
     cin = x.shape[-1]
+    pz = _at(dz)
     px, pc, pe = _saved(x, dz, dz.shape[:-1] + (cin,), "linear_wgrad (x)")
-    dw = torch.empty(cout, cin, dtype=torch.float32, device=dz.device)
+    dw = torch.empty((cout, cin), dtype=_F32, device=dz.device)
     nb = lib.simhand_linear_wgrad_workspace_bytes(rows, cin, cout, d)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dz.device)
-    check(lib.simhand_linear_wgrad(_ptr(dz), px, pc, pe, _ptr(dw), rows, cin, cout, d, _ptr(ws), nb, _stream()), "linear_wgrad")
+    ws = _scratch(nb, dz)
+    check(lib.simhand_linear_wgrad(pz, px, pc, pe, dw.data_ptr(), rows, cin, cout, d, ws.data_ptr(), nb, _row_stream(dz)), "linear_wgrad")
     return dw
 
 
@@ -362,9 +385,10 @@ def act8_pack(x: torch.Tensor) -> Act8:
     """x [..., cols] -> its 8-bit checkpoint (1.03 bytes a value): see Act8.  Inf and NaN are kept as NaN."""
     rows, cols = _rows_of(x, "act8_pack")
     lib = _lib_dev()
+    px, d = _at(x), dt(x.dtype)
     codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
-    exps = torch.empty(rows, (cols + 31) // 32, dtype=torch.uint8, device=x.device)
-    check(lib.simhand_act8_pack(_ptr(x), _ptr(codes), _ptr(exps), rows, cols, dt(x.dtype), _stream()), "act8_pack")
+    exps = torch.empty((rows, (cols + 31) // 32), dtype=torch.uint8, device=x.device)
+    check(lib.simhand_act8_pack(px, codes.data_ptr(), exps.data_ptr(), rows, cols, d, _row_stream(x)), "act8_pack")
     return Act8(codes, exps, x.dtype)
 
 
@@ -372,8 +396,9 @@ def act8_unpack(a: Act8) -> torch.Tensor:
     """The values an 8-bit checkpoint stands for, in the type it was packed from."""
     rows, cols = _rows_of(a, "act8_unpack")
     lib = _lib_dev()
+    pc, pe, d = _at(a.codes), _at(a.exps), dt(a.dtype)
     x = torch.empty(a.shape, dtype=a.dtype, device=a.device)
-    check(lib.simhand_act8_unpack(_ptr(a.codes), _ptr(a.exps), _ptr(x), rows, cols, dt(a.dtype), _stream()), "act8_unpack")
+    check(lib.simhand_act8_unpack(pc, pe, x.data_ptr(), rows, cols, d, _row_stream(a)), "act8_unpack")
     return x
 
 

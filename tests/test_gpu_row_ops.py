@@ -189,6 +189,38 @@ def test_linear_forward(dtype, m, k, n, act, bias, residual, pre):
         close(zp, z, half_step(dtype) * z.abs() + 1.01 * fz + tiny(dtype), "pre")
 
 
+# the kernel for many rows (16 bits, rows of 16-byte chunks, at least 192 tiles of 256 x 256): whole tiles, ragged rows / columns / K, one to five k-steps, the smallest N, several
+# tiles per block
+SHAPES_MANY = [(49152, 64, 256), (49100, 72, 136), (24600, 128, 520), (6200, 320, 2048), (30011, 8, 384), (131072 + 40, 200, 128), (16640, 136, 1032)]
+
+
+@pytest.mark.parametrize("m,k,n", SHAPES_MANY)
+@pytest.mark.parametrize("act,bias,residual,pre", [("none", False, False, False), ("relu", True, True, False), ("gelu", True, True, True), ("silu", False, False, True)])
+def test_linear_forward_many_rows(dtype, m, k, n, act, bias, residual, pre):
+    from simhand_amd import ops
+
+    if dtype == torch.float32:
+        m = m // 16 + 5  # the tile kernel's own sizes are covered above; its 128-wide tiles start at 512 of them
+    x, w = randn(m, k, dtype=dtype), randn(n, k, seed=1, scale=k ** -0.5, dtype=dtype)
+    b = randn(n, seed=2) if bias else None
+    res = randn(m, n, seed=3, dtype=dtype) if residual else None
+    out = ops.linear_fwd(x.cuda(), w.cuda(), b.cuda() if bias else None, act=act, residual=res.cuda() if residual else None, want_pre=pre)
+    y, zp = out if pre else (out, None)
+    xd, wd = x.cuda().double(), w.cuda().double()  # 64-bit products on the GPU (plain torch): too many for the CPU
+    z, mag = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    if bias:
+        z, mag = z + b.cuda().double(), mag + b.cuda().double().abs()
+    fz = 2 * (k + 2) * U * mag
+    want = act_ref(z, act)
+    fy = 1.13 * fz + 8 * U * (z.abs() + 1e-30)
+    if residual:
+        want = want + res.cuda().double()
+        fy = fy + U * (want.abs() + z.abs())
+    assert bool(((y.double() - want).abs() <= half_step(dtype) * want.abs() + 1.01 * fy + tiny(dtype)).all())
+    if pre:
+        assert bool(((zp.double() - z).abs() <= half_step(dtype) * z.abs() + 1.01 * fz + tiny(dtype)).all())
+
+
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 9), (7, 64), (100, 33), (513, 128), (129, 512), (2050, 77), (64, 2048)])
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
 def test_linear_act_backward(dtype, rows, cols, act):
