@@ -64,8 +64,22 @@ __device__ __forceinline__ void linear_store8(const LinearArgs& p, long long row
   }
 }
 
-// 256 x 256 tiles, 16-bit operands (linear256.hip)
+struct WgradArgsL {
+  const void* dz;         // [M][N]
+  const void* x;          // [M][K] (null: codes)
+  const uint8_t* codes;   // [M][K]
+  const uint8_t* exps;    // [M][ceil(K / 32)]
+  float* part;            // [splits][N][K]
+  long long M, per_split; // per_split: a multiple of the k-step
+  int N, K;
+  unsigned n_tiles, k_tiles;
+};
+
+// 256 x 256 tiles, 16-bit operands (linear256.hip, linear_wgrad256.hip)
 bool linear256_takes(const LinearArgs& p, int dtype);
 int linear256_launch(const LinearArgs& p, hipStream_t s, const char* what);
+bool linear_wgrad256_takes(const void* dz, const void* x, const uint8_t* codes, const uint8_t* exps, int64_t rows, int in_dim, int out_dim, int dtype);
+void linear_wgrad256_plan(int64_t rows, int in_dim, int out_dim, int* splits, int64_t* per);
+int linear_wgrad256_launch(const WgradArgsL& p, int splits, hipStream_t s);
 
 }  // namespace sh

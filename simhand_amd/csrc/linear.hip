@@ -225,17 +225,6 @@ __global__ __launch_bounds__(256) void linear_act_bwd_kernel(const T* __restrict
 }
 
 // ---- dw = dz^T x ---------------------------------------------------------------------------------------------------------------
-struct WgradArgsL {
-  const void* dz;         // [M][N]
-  const void* x;          // [M][K] (null: codes)
-  const uint8_t* codes;   // [M][K]
-  const uint8_t* exps;    // [M][ceil(K / 32)]
-  float* part;            // [splits][N][K]
-  long long M, per_split; // per_split: a multiple of the k-step
-  int N, K;
-  unsigned n_tiles, k_tiles;
-};
-
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 // 16-bit operand of 32 rows x 16 columns read transposed: lane gets rows {4g..4g+3, 16+4g..16+4g+3} of column cb + (lane & 15)
 __device__ __forceinline__ uint4 frag_tr16(const char* tile, int stride, int cb, int lane) {
@@ -522,9 +511,12 @@ int simhand_linear_dgrad(const void* dz, const void* w, void* dx, int64_t rows, 
 
 size_t simhand_linear_wgrad_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype) {
   if (rows < 0 || in_dim < 1 || out_dim < 1) return 0;
-  int splits;
+  // the call's alignment decides between two kernels (below): enough for either
+  int splits, wide = 1;
   int64_t per;
   linear_wgrad_plan(rows, in_dim, out_dim, dtype, &splits, &per);
+  if (linear_wgrad256_takes(nullptr, nullptr, nullptr, nullptr, rows, in_dim, out_dim, dtype)) linear_wgrad256_plan(rows, in_dim, out_dim, &wide, &per);
+  if (wide > splits) splits = wide;
   return splits > 1 ? (size_t)splits * in_dim * out_dim * sizeof(float) : 16;
 }
 
@@ -545,18 +537,24 @@ int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, 
   }
   int splits;
   int64_t per;
-  linear_wgrad_plan(rows, in_dim, out_dim, dtype, &splits, &per);
+  const bool wide = linear_wgrad256_takes(dz, x, x_codes, x_exps, rows, in_dim, out_dim, dtype);
+  if (wide) linear_wgrad256_plan(rows, in_dim, out_dim, &splits, &per);
+  else linear_wgrad_plan(rows, in_dim, out_dim, dtype, &splits, &per);
   WgradArgsL p = {dz, x, x_codes, x_exps, splits > 1 ? (float*)workspace : dw, rows, per, out_dim, in_dim, (unsigned)ceil_div(out_dim, 128),
                   (unsigned)ceil_div(in_dim, 128)};
-  const unsigned grid = p.n_tiles * p.k_tiles * (unsigned)splits;
-  if (dtype == SH_F32) {
-    if (a8) linear_wgrad_kernel<float, true><<<grid, 256, 0, s>>>(p);
-    else linear_wgrad_kernel<float, false><<<grid, 256, 0, s>>>(p);
+  if (wide) {
+    if (linear_wgrad256_launch(p, splits, s)) return 1;
   } else {
-    if (a8) linear_wgrad_kernel<bf16_t, true><<<grid, 256, 0, s>>>(p);
-    else linear_wgrad_kernel<bf16_t, false><<<grid, 256, 0, s>>>(p);
+    const unsigned grid = p.n_tiles * p.k_tiles * (unsigned)splits;
+    if (dtype == SH_F32) {
+      if (a8) linear_wgrad_kernel<float, true><<<grid, 256, 0, s>>>(p);
+      else linear_wgrad_kernel<float, false><<<grid, 256, 0, s>>>(p);
+    } else {
+      if (a8) linear_wgrad_kernel<bf16_t, true><<<grid, 256, 0, s>>>(p);
+      else linear_wgrad_kernel<bf16_t, false><<<grid, 256, 0, s>>>(p);
+    }
+    if (check_launch("linear_wgrad")) return 1;
   }
-  if (check_launch("linear_wgrad")) return 1;
   if (splits > 1) {
     linear_wgrad_reduce_kernel<<<(unsigned)((count + 255) / 256), 256, 0, s>>>((const float*)workspace, count, splits, dw);
     return check_launch("linear_wgrad_reduce");

@@ -251,6 +251,23 @@ def test_linear_backward(dtype, m, k, n, act8):
     assert ops.linear_bwd(dz.cuda(), xs, w.cuda(), need_dx=False)[0] is None
 
 
+# the kernels for many rows (weight gradient: at least 4096 rows and 192 columns on both sides; input gradient: 192 tiles): whole and ragged tiles, rows that end inside a step,
+# one and several tiles, ranges of rows that leave some blocks with less
+@pytest.mark.parametrize("m,k,n", [(4096, 256, 256), (49152, 256, 256), (49157, 200, 328), (8195, 512, 200), (6001, 384, 1024), (20000, 1024, 264), (33333, 640, 192)])
+@pytest.mark.parametrize("act8", [False, True])
+def test_linear_backward_many_rows(dtype, m, k, n, act8):
+    from simhand_amd import ops
+
+    x, w, dz = randn(m, k, dtype=dtype).cuda(), randn(n, k, seed=1, dtype=dtype).cuda(), randn(m, n, seed=2, dtype=dtype).cuda()
+    xs = ops.act8_pack(x) if act8 else x
+    xv = ops.act8_unpack(xs).double() if act8 else x.double()
+    dx, dw = ops.linear_bwd(dz, xs, w)
+    zd, wd = dz.double(), w.double()
+    want = zd @ wd
+    assert bool(((dx.double() - want).abs() <= half_step(dtype) * want.abs() + 1.01 * 2 * (n + 2) * U * (zd.abs() @ wd.abs()) + tiny(dtype)).all())
+    assert bool(((dw.double() - zd.t() @ xv).abs() <= 2 * (m + 40) * U * (zd.abs().t() @ xv.abs()) + 1e-30).all())
+
+
 def test_linear_gradient_against_differences():
     """fp32: dz, db, dx, dw against central differences of the 64-bit formula along random directions."""
     from simhand_amd import ops
