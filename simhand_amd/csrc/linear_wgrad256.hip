@@ -17,7 +17,7 @@ template <bool A8>
 __global__ __launch_bounds__(512, 1) void linear_wgrad256_kernel(WgradArgsL p) {
   typedef bf16_t T;
   constexpr int KP = 32, SUB = KP * 128, HALF = 4 * SUB;    // rows per step, bytes of a sub-tile / of one operand's tile
-  constexpr int NS = A8 ? 5 : 4, D = NS - 1;                // stages; steps the DMAs run ahead
+  constexpr int NS = 5, D = NS - 1;                         // stages; steps the DMAs run ahead
   constexpr int RAW = KP * 256, RAWE = KP * 8;              // codes and exponents of a step
   constexpr int XS = A8 ? 2 : NS;                           // stages of the 16-bit x tile
   constexpr int X0 = NS * HALF, R0 = X0 + XS * HALF, E0 = R0 + (A8 ? NS * RAW : 0), BYTES = E0 + (A8 ? NS * RAWE : 0);
@@ -59,12 +59,13 @@ __global__ __launch_bounds__(512, 1) void linear_wgrad256_kernel(WgradArgsL p) {
     inside[i] = col < width;
     ptr[i] = reinterpret_cast<const char*>(src0 + (r0 + row) * width + (inside[i] ? col : 0));
   }
-  // A8: lane = row 4 wave + (lane >> 4) of the step, codes k0 + 16 (lane & 15) .. + 15; exponents: row lane >> 1, 4 of the tile's 8 bytes
+  // A8: lane = row 4 wave + (lane >> 4) of the step, codes k0 + 16 (lane & 15) .. + 15; exponents of the wave's four rows: lanes 0 .. 7, half a row's 8 bytes each (all 32 rows by
+  // every wave would be 256 cache lines a step, three times what the operands take)
   const int crow = 4 * wave + (lane >> 4), ccol = 16 * li;
   const long long eb = (p.K + kAct8Block - 1) / kAct8Block;
   const bool cin = A8 && k0 + ccol < p.K, ein = A8 && k0 / 32 + 4 * (lane & 1) < eb;
   const uint8_t* cptr = A8 ? p.codes + (r0 + crow) * p.K + (cin ? k0 + ccol : 0) : nullptr;
-  const uint8_t* eptr = A8 ? p.exps + (r0 + (lane >> 1)) * eb + (ein ? k0 / 32 + 4 * (lane & 1) : 0) : nullptr;
+  const uint8_t* eptr = A8 ? p.exps + (r0 + 4 * wave + (lane >> 1)) * eb + (ein ? k0 / 32 + 4 * (lane & 1) : 0) : nullptr;
   unsigned fill = 0;  // stage the next DMAs go to
   auto dma_step = [&](int c) __attribute__((always_inline)) {
     const int left = rows - c * KP;  // rows of step c (<= 0: none, zeros)
@@ -76,27 +77,26 @@ __global__ __launch_bounds__(512, 1) void linear_wgrad256_kernel(WgradArgsL p) {
     }
     if constexpr (A8) {
       dma16(cin && crow < left ? (const void*)cptr : (const void*)zero, lds0 + R0 + fill * RAW + wave * 1024);
-      dma4(ein && (lane >> 1) < left ? (const void*)eptr : (const void*)zero, lds0 + E0 + fill * RAWE);  // every wave fetches the same 256 bytes
+      if (lane < 8) dma4(ein && 4 * wave + (lane >> 1) < left ? (const void*)eptr : (const void*)zero, lds0 + E0 + fill * RAWE + wave * 32);
       cptr += (long long)KP * p.K;
       eptr += KP * eb;
     }
     fill = fill == NS - 1 ? 0 : fill + 1;
   };
-  // the thread's own 16 codes of the step in stage `from` -> its 32 bytes of the 16-bit tile `to`
-  auto decode = [&](unsigned from, unsigned to) __attribute__((always_inline)) {
-    const uint4 q = *reinterpret_cast<const uint4*>(smem + R0 + from * RAW + wave * 1024 + lane * 16);
-    const float sc = act8_scale(*reinterpret_cast<const uint8_t*>(smem + E0 + from * RAWE + crow * 8 + (li >> 1)));
-    float v[16];
-    act8_decode4(q.x, sc, v);
-    act8_decode4(q.y, sc, v + 4);
-    act8_decode4(q.z, sc, v + 8);
-    act8_decode4(q.w, sc, v + 12);
-    float lo[8], hi[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) lo[e] = v[e], hi[e] = v[8 + e];
-    char* at = smem + X0 + to * HALF + (li >> 2) * SUB + crow * 128 + (((li & 3) + (crow >> 1)) & 3) * 32;
-    *reinterpret_cast<uint4*>(at) = pack16<T>(lo);
-    *reinterpret_cast<uint4*>(at + 16) = pack16<T>(hi);
+  // the thread's own 16 codes of the step in stage `from`: fetched from LDS, then decoded into their 32 bytes of the 16-bit tile `to`.  The halves of a 32-byte group change places in
+  // the odd sub-tiles: eight neighbouring lanes then write 128 different bytes of the banks.
+  uint4 cq;
+  unsigned ce;
+  auto codes_get = [&](unsigned from) __attribute__((always_inline)) {
+    cq = *reinterpret_cast<const uint4*>(smem + R0 + from * RAW + wave * 1024 + lane * 16);
+    ce = *reinterpret_cast<const uint8_t*>(smem + E0 + from * RAWE + crow * 8 + (li >> 1));
+  };
+  const int put_at = X0 + (li >> 2) * SUB + crow * 128 + (((li & 3) + (crow >> 1)) & 3) * 32 + ((li >> 2) & 1) * 16;
+  auto codes_put = [&](unsigned to) __attribute__((always_inline)) {
+    const float sc = act8_scale(ce);
+    char* at = smem + to * HALF;
+    *reinterpret_cast<uint4*>(at + put_at) = act8_decode8_h16(cq.x, cq.y, sc);
+    *reinterpret_cast<uint4*>(at + (put_at ^ 16)) = act8_decode8_h16(cq.z, cq.w, sc);
   };
 
   f32x4 acc[8][4];
@@ -120,31 +120,55 @@ __global__ __launch_bounds__(512, 1) void linear_wgrad256_kernel(WgradArgsL p) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) offs[q] = frow * 128 + (((q + (frow >> 1)) & 3) * 32) + (li & 3) * 8;
 
+  const int xhalf = A8 ? (wn & 1) * 16 : 0;
+  // The barrier stands in the MIDDLE of a step: it says that step j + 1 has landed (and, A8, is decoded) while half of step j's MFMAs are still to come, and under those the
+  // first fragments of step j + 1 are read.  With the barrier at the top all eight waves read fragments at once and the matrix cores waited for them: 44 % busy.
+  uint4 fa[4], fb[2][4];
+  auto read_a = [&](unsigned stage, int mi) __attribute__((always_inline)) {
+    fa[mi & 3] = tr2(smem + stage * HALF + (wm * 2 + (mi >> 2)) * SUB + offs[mi & 3]);
+  };
+  auto x_tile = [&](int j, unsigned stage) __attribute__((always_inline)) { return smem + X0 + (A8 ? (unsigned)(j & 1) : stage) * HALF + wn * SUB; };
   if constexpr (A8) {  // the first step's x tile (its codes are this thread's own)
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * (D - 1)) : "memory");
-    decode(0, 0);
+    codes_get(0);
+    codes_put(0);
   }
-  unsigned use = 0;  // stage of step j
-  for (int j = 0; j < nk; ++j) {
-    // !A8: step j has landed (D - 1 steps of 4 instructions may be in flight).  A8: step j + 1 has, too -- its codes are decoded below.
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(A8 ? 4 * (D - 2) : 4 * (D - 1)) : "memory");
-    dma_step(j + D);  // into the stage that step j - 1 was read from
-    const unsigned nxt = use == NS - 1 ? 0 : use + 1;
-    const char* ta = smem + use * HALF + wm * 2 * SUB;
-    const char* tb = smem + X0 + (A8 ? (unsigned)(j & 1) : use) * HALF + wn * SUB;
-    uint4 fb[4];
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 * (D - 1)) : "memory");
 #pragma unroll
-    for (int ni = 0; ni < 4; ++ni) fb[ni] = tr2(tb + offs[ni]);
+  for (int ni = 0; ni < 4; ++ni) fb[0][ni] = tr2(x_tile(0, 0) + (offs[ni] ^ xhalf));
+  read_a(0, 0);
+  read_a(0, 1);
+  unsigned use = 0;  // stage of step j
+  auto step = [&](int j, auto parity) __attribute__((always_inline)) {
+    constexpr int P = decltype(parity)::value;
+    const unsigned nxt = use == NS - 1 ? 0 : use + 1;
+    if constexpr (A8) {  // step j + 1 has landed as far as this wave's own DMAs go: steps j + 2 .. j + D - 1 may be in flight
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * (D - 2)) : "memory");
+      codes_get(nxt);
+    }
 #pragma unroll
     for (int mi = 0; mi < 8; ++mi) {
-      const uint4 fa = tr2(ta + (mi >> 2) * SUB + offs[mi & 3]);
+      if (mi < 6) read_a(use, mi + 2);
+      if (mi == 5) {
 #pragma unroll
-      for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = sh_mfma16(fa, fb[ni], acc[mi][ni]);
+        for (int ni = 0; ni < 4; ++ni) fb[P ^ 1][ni] = tr2(x_tile(j + 1, nxt) + (offs[ni] ^ xhalf));
+      }
+      if (mi >= 6) read_a(nxt, mi - 6);
+#pragma unroll
+      for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = sh_mfma16(fa[mi & 3], fb[P][ni], acc[mi][ni]);
       if constexpr (A8) {
-        if (mi == 3) decode(nxt, (unsigned)((j + 1) & 1));
+        if (mi == 1) codes_put((unsigned)((j + 1) & 1));  // read last in the second half of step j - 2
+      }
+      if (mi == 3) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 * (D - 2)) : "memory");
+        dma_step(j + D);  // into the stage of step j - 1, which every wave has read
       }
     }
     use = nxt;
+  };
+  for (int j = 0; j < nk; j += 2) {
+    step(j, std::integral_constant<int, 0>());
+    if (j + 1 < nk) step(j + 1, std::integral_constant<int, 1>());
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 
