@@ -145,11 +145,17 @@ __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(const T* __restrict
 
 // A8: x comes as its 8-bit checkpoint (codes + exponents).  part [gridDim.x][2][cols]: sums of u h and u over the block's rows.
 // A row group walks its rows with the next row's loads in flight; gamma and beta wait in LDS (G < 256), which the column sums reuse at the end.
-template <typename T, int G, int NV, bool A8, bool RAG>
-__global__ __launch_bounds__(256) void layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
+// blocks of the backward kernel per CU, by the values a lane holds (registers); the grid is as many as run at once
+__host__ __device__ constexpr int ln_bwd_occupancy(int nv, bool fp32, bool rag) {
+  if (fp32) return nv <= 1 ? 8 : nv <= 2 ? 5 : nv <= 4 ? 3 : 1;
+  return nv <= 1 ? 6 : nv <= 2 ? (rag ? 3 : 4) : nv <= 4 ? 2 : 1;
+}
+
+template <typename T, int G, int NV, bool A8, bool RAG, bool GATE>
+__global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG)) void layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
                                                              const uint8_t* __restrict__ exps, const float* __restrict__ gamma,
                                                              const float* __restrict__ beta, const float* __restrict__ mean,
-                                                             const float* __restrict__ rstd, int relu, T* __restrict__ dx,
+                                                             const float* __restrict__ rstd, T* __restrict__ dx,
                                                              float* __restrict__ part, long long rows, int cols) {
   constexpr int VE = Vec16<T>::N, RB = 256 / G, W8 = VE / 4;
   constexpr bool GLOBAL = G == 256;  // wide rows: gamma / beta come from the caches
@@ -163,9 +169,9 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(const T* __restrict
 #pragma unroll
     for (int e = 0; e < VE; ++e) ag[i][e] = ab[i][e] = 0.f;
   if constexpr (!GLOBAL) {
-    for (int c = threadIdx.x; c < cols; c += 256) {
-      fold[0][c] = gamma[c];
-      fold[1][c] = beta[c];
+    for (int c = threadIdx.x; c < cols || c < VE; c += 256) {  // (a row shorter than a vector: zeros behind it)
+      fold[0][c] = c < cols ? gamma[c] : 0.f;
+      fold[1][c] = c < cols ? beta[c] : 0.f;
     }
     __syncthreads();
   }
@@ -229,6 +235,8 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(const T* __restrict
     }
     if (row0 + stride < rows) fetch(row + stride);
     float s1 = 0.f, s2 = 0.f;
+    // The pass is bound by its arithmetic once the loads are hidden (25 instructions a value took 35 us of 33001 x 777 alone): the gate is a variant of its own, and
+    // only a row's ragged last vector -- never in the first half of the lane's vectors -- masks what its neighbour counts.
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const LnVec<VE, RAG> w((i * G + t) * VE, cols);
@@ -236,24 +244,28 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(const T* __restrict
       float ga[VE], be[VE];
       if constexpr (GLOBAL) {
         w.load_f32(gamma, ga);
-        w.load_f32(beta, be);
+        if constexpr (GATE) w.load_f32(beta, be);
       } else {
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           ga[e] = fold[0][w.at + e];
-          be[e] = fold[1][w.at + e];
+          if constexpr (GATE) be[e] = fold[1][w.at + e];
         }
       }
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const float z = ln_affine(h[i][e], m, r, ga[e], be[e], h[i][e]);
-        if (relu && !(z > 0.f)) u[i][e] = 0.f;
-        const float uc = w.counts(e) ? u[i][e] : 0.f, hc = w.counts(e) ? h[i][e] : 0.f;
-        ag[i][e] += uc * hc;
+        if constexpr (GATE) {
+          if (!(ln_affine(h[i][e], m, r, ga[e], be[e], h[i][e]) > 0.f)) u[i][e] = 0.f;
+        } else {
+          h[i][e] = (h[i][e] - m) * r;
+        }
+        const float uc = RAG && 2 * i >= NV - 1 ? (w.counts(e) ? u[i][e] : 0.f) : u[i][e];
+        const float gc = uc * ga[e];
+        ag[i][e] += uc * h[i][e];
         ab[i][e] += uc;
-        u[i][e] *= ga[e];
-        s1 += w.counts(e) ? u[i][e] : 0.f;
-        s2 += w.counts(e) ? u[i][e] * h[i][e] : 0.f;
+        s1 += gc;
+        s2 += gc * h[i][e];
+        u[i][e] = RAG && 2 * i >= NV - 1 ? u[i][e] * ga[e] : gc;
       }
     }
     group_sum2<G>(s1, s2, red);
@@ -342,10 +354,14 @@ int fold_columns(const float* part, int nblk, int n, float* out, hipStream_t s) 
 static int ln_nvec(int cols, int dtype) { return (cols + (dtype == SH_F32 ? 4 : 8) - 1) / (dtype == SH_F32 ? 4 : 8); }
 constexpr int kLnMaxVec = 2048;
 static int ln_rows_per_block(int nvec) { return nvec <= 16 ? 16 : nvec <= 256 ? 4 : 1; }
-// backward blocks: enough to fill the chip twice, few enough that the partial sums stay small beside the rows
-static int ln_bwd_blocks(int64_t rows, int nvec) {
+static int ln_nv(int nvec) { return nvec <= 64 ? 1 : nvec <= 128 ? 2 : nvec <= 256 ? 4 : nvec <= 512 ? 2 : nvec <= 1024 ? 4 : 8; }
+// backward blocks: one round of what the CUs hold (each then walks its share of the rows with the next row in flight; a second, part-empty round cost a third of the
+// pass over 33001 x 777), and no more partial sums than that
+static int ln_bwd_blocks(int64_t rows, int cols, int dtype) {
+  const int nvec = ln_nvec(cols, dtype);
   const int64_t need = (rows + ln_rows_per_block(nvec) - 1) / ln_rows_per_block(nvec);
-  return (int)(need < 1 ? 1 : need > 1024 ? 1024 : need);
+  const int64_t most = 256 * ln_bwd_occupancy(ln_nv(nvec), dtype == SH_F32, cols % (dtype == SH_F32 ? 4 : 8) != 0);
+  return (int)(need < 1 ? 1 : need > most ? most : need);
 }
 
 #define SH_LN_DISPATCH(CALL)          \
@@ -394,7 +410,7 @@ int simhand_layer_norm_fwd(const void* x, const float* gamma, const float* beta,
 
 size_t simhand_layer_norm_bwd_workspace_bytes(int64_t rows, int cols, int dtype) {
   if (rows < 0 || cols < 1) return 0;
-  return (size_t)ln_bwd_blocks(rows, ln_nvec(cols, dtype)) * 2 * cols * sizeof(float);
+  return (size_t)ln_bwd_blocks(rows, cols, dtype) * 2 * cols * sizeof(float);
 }
 
 int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, const float* gamma, const float* beta,
@@ -407,23 +423,26 @@ int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes
   SH_REQUIRE(!a8 || (x_exps && !x), "layer_norm_bwd: pass either x or its codes and exponents");
   SH_REQUIRE(gamma && beta && dgamma_dbeta && (rows == 0 || (dy && (x || a8) && mean && rstd && dx)), "layer_norm_bwd: NULL argument");
   const int nvec = ln_nvec(cols, dtype);
-  const int grid = ln_bwd_blocks(rows, nvec);
+  const int grid = ln_bwd_blocks(rows, cols, dtype);
   SH_REQUIRE(workspace && workspace_bytes >= simhand_layer_norm_bwd_workspace_bytes(rows, cols, dtype), "layer_norm_bwd: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   const double eb = dtype == SH_F32 ? 4 : 2;
   ProfScope ps(SH_PROF_BN, s, 0, (double)rows * cols * (2 * eb + (a8 ? 1.03125 : eb)));
   float* part = (float*)workspace;
   const bool rag = cols % (dtype == SH_F32 ? 4 : 8) != 0;
-#define SH_ONE(T, G, NV, A8, RAG)                                                                                                                    \
-  layer_norm_bwd_kernel<T, G, NV, A8, RAG><<<grid, 256, 0, s>>>((const T*)dy, (const T*)x, x_codes, x_exps, gamma, beta, mean, rstd, relu, (T*)dx, part, \
-                                                                rows, cols)
-#define SH_TYPE(T, G, NV)                     \
-  if (a8) {                                   \
-    if (rag) SH_ONE(T, G, NV, true, true);    \
-    else SH_ONE(T, G, NV, true, false);       \
-  } else {                                    \
-    if (rag) SH_ONE(T, G, NV, false, true);   \
-    else SH_ONE(T, G, NV, false, false);      \
+#define SH_LAUNCH(T, G, NV, A8, RAG, GATE)                                                                                                           \
+  layer_norm_bwd_kernel<T, G, NV, A8, RAG, GATE><<<grid, 256, 0, s>>>((const T*)dy, (const T*)x, x_codes, x_exps, gamma, beta, mean, rstd, (T*)dx, part, \
+                                                                      rows, cols)
+#define SH_ONE(T, G, NV, A8, RAG)               \
+  if (relu) SH_LAUNCH(T, G, NV, A8, RAG, true); \
+  else SH_LAUNCH(T, G, NV, A8, RAG, false)
+#define SH_TYPE(T, G, NV)                       \
+  if (a8) {                                     \
+    if (rag) { SH_ONE(T, G, NV, true, true); }  \
+    else { SH_ONE(T, G, NV, true, false); }     \
+  } else {                                      \
+    if (rag) { SH_ONE(T, G, NV, false, true); } \
+    else { SH_ONE(T, G, NV, false, false); }    \
   }
 #define SH_CALL(G, NV)                        \
   if (dtype == SH_F32) {                      \
@@ -435,6 +454,7 @@ int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes
 #undef SH_CALL
 #undef SH_TYPE
 #undef SH_ONE
+#undef SH_LAUNCH
   if (check_launch("layer_norm_bwd")) return 1;
   return fold_columns(part, grid, 2 * cols, dgamma_dbeta, s);
 }
