@@ -628,7 +628,8 @@ int simhand_linear_act_bwd(const void* dy, const void* pre, int act, void* dz, f
 size_t simhand_linear_dgrad_workspace_bytes(int in_dim, int out_dim, int dtype);
 int simhand_linear_dgrad(const void* dz, const void* w, void* dx, int64_t rows, int in_dim, int out_dim, int dtype, void* workspace,
                          size_t workspace_bytes, sh_stream_t stream);
-/* dw [out_dim][in_dim] fp32 = dz^T x; x as it is, or (x = NULL) as its 8-bit checkpoint, whose values enter the product rounded to dtype */
+/* dw [out_dim][in_dim] fp32 = dz^T x; x as it is, or (x = NULL) as its 8-bit checkpoint, whose values enter the product rounded to dtype.
+ * A workspace query of 0: NULL will do. */
 size_t simhand_linear_wgrad_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype);
 int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, float* dw, int64_t rows, int in_dim,
                          int out_dim, int dtype, void* workspace, size_t workspace_bytes, sh_stream_t stream);

@@ -98,6 +98,178 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_gemm_kernel(L
   }
 }
 
+// The same product with both operands by LDS-DMA, for rows of whole 16-byte chunks: two k-steps ahead, one barrier per step and nothing staged in registers.  Waves as 2 x 2, each
+// QM x QN MFMA tiles: 128 x 128 (80 KB of LDS, weights only one step ahead: two blocks per CU), 128 x 64 (two), 64 x 64 (three) -- the largest that still puts two blocks on every
+// CU.  One block's epilogue runs under the others' k-loops.
+// BT: b is stored [K][N] (dx = dz w reads w as it is, without a transposed copy): its tile is sub-tiles of 64 columns by K rows, 16-bit operands are read transposed
+// (ds_read_b64_tr_b16; the activations' chunks are then read in the halves that match its row order), fp32 ones element by element.
+__device__ uint4 g_lin_zero[8];  // read-only zeros
+
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+
+template <typename T, int QM, int QN, bool BT>
+__global__ __launch_bounds__(256, QM == 2 ? 3 : 2) void linear_dma_kernel(LinearArgs p) {
+  constexpr int VE = Vec16<T>::N, KE = 128 / sizeof(T), BM = 32 * QM, BN = 32 * QN;
+  constexpr int NB = QN == 4 ? 2 : 3;  // stages of b
+  constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, B0 = 3 * A_BYTES;
+  __shared__ __attribute__((aligned(16))) char smem[3 * A_BYTES + NB * B_BYTES];
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
+  // inline asm: hipcc's wait-count pass would drain every outstanding LDS-DMA in front of each LDS read; the loop counts them itself
+  auto dma16 = [](const void* src, unsigned lds_addr) __attribute__((always_inline)) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_addr), "v"(src));
+  };
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int li = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
+  const unsigned logical = xcd_order(blockIdx.x, gridDim.x);
+  const int n0 = (int)(logical % p.n_tiles) * BN;
+  const long long m0 = (long long)(logical / p.n_tiles) * BM;
+  // instruction i of a wave fills tile rows 32 i + 8 wave .. + 7; lane = row lane >> 3, slot lane & 7; slot s holds chunk s ^ key(row)
+  const int slot = lane & 7, lrow = wave * 8 + (lane >> 3);
+  auto key_b = [](int row) __attribute__((always_inline)) -> int { return ((row >> 1) & 1) | (((row >> 3) & 3) << 1); };
+  const int ka = (slot ^ ((lrow >> 1) & 7)) * VE;
+  const char* zero = reinterpret_cast<const char*>(g_lin_zero) + slot * 16;
+  const char* pa[QM];
+#pragma unroll
+  for (int i = 0; i < QM; ++i) {
+    const long long m = m0 + lrow + 32 * i;
+    pa[i] = reinterpret_cast<const char*>((const T*)p.a + (m < p.M ? m : p.M - 1) * p.K + ka);
+  }
+  // b [N][K]: as a.  b [K][N]: instruction i of a wave = number q = QN wave + i of the tile's; sub-tile q / 8, rows 8 (q % 8) (16 bits) or 4 (q % 8) (fp32) and following; the columns of
+  // a row are rotated (16 bits: 32-byte groups by row / 2; fp32: 16-byte slots by 0, 1, 8, 9 for row / 4) so that what a read touches falls on different banks
+  auto rot32 = [](int row) __attribute__((always_inline)) -> int { return ((row >> 2) & 1) + ((row >> 3) & 1) * 8; };
+  const char* pb[QN];
+  int kb[QN];       // the lane's first k of the chunk (b [N][K]) or its row (b [K][N]) inside a step
+  bool inside[QN];
+#pragma unroll
+  for (int i = 0; i < QN; ++i) {
+    if constexpr (BT) {
+      const int q = QN * wave + i, sub = q >> 3;
+      int col;
+      if constexpr (sizeof(T) == 2) {
+        kb[i] = 8 * (q & 7) + (lane >> 3);
+        col = n0 + sub * 64 + ((((slot >> 1) - (kb[i] >> 1)) & 3) * 16) + (slot & 1) * 8;
+      } else {
+        kb[i] = 4 * (q & 7) + (lane >> 4);
+        col = n0 + sub * 64 + (((lane & 15) - rot32(kb[i])) & 15) * 4;
+      }
+      inside[i] = col < p.N;
+      pb[i] = reinterpret_cast<const char*>((const T*)p.b + (long long)kb[i] * p.ldb + (inside[i] ? col : 0));
+    } else {
+      const int n = n0 + lrow + 32 * i;
+      kb[i] = (slot ^ key_b(lrow)) * VE;
+      inside[i] = true;
+      pb[i] = reinterpret_cast<const char*>((const T*)p.b + (long long)(n < p.N ? n : p.N - 1) * p.ldb + kb[i]);
+    }
+  }
+  const long long b_step = BT ? (long long)KE * p.ldb * (int)sizeof(T) : 128;
+  auto issue_a = [&](int kt) __attribute__((always_inline)) {
+    const bool ok = kt * KE + ka < p.K;
+    const unsigned dst = lds0 + (kt % 3) * A_BYTES + wave * 1024;
+#pragma unroll
+    for (int i = 0; i < QM; ++i) dma16(ok ? pa[i] + kt * 128 : zero, dst + i * 4096);
+  };
+  auto issue_b = [&](int kt) __attribute__((always_inline)) {
+    const unsigned dst = lds0 + B0 + (kt % NB) * B_BYTES;
+#pragma unroll
+    for (int i = 0; i < QN; ++i)
+      dma16(inside[i] && kt * KE + kb[i] < p.K ? pb[i] + kt * b_step : zero, dst + (BT ? (QN * wave + i) * 1024 : wave * 1024 + i * 4096));
+  };
+  f32x4 acc[QM][QN];
+#pragma unroll
+  for (int mi = 0; mi < QM; ++mi)
+#pragma unroll
+    for (int ni = 0; ni < QN; ++ni) acc[mi][ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  const int nk = (p.K + KE - 1) / KE;
+  const int akey = (li >> 1) & 7, fa0 = (wm * 16 * QM + li) * 128;
+  const int rowb = wn * 16 * QN + lin_col(0, li);
+  const int fb0 = rowb * 128 + ((g ^ key_b(rowb)) * 16);
+  int bt[QN];  // BT: the lane's place in b's tile
+#pragma unroll
+  for (int ni = 0; ni < QN; ++ni) {
+    if constexpr (sizeof(T) == 2) {
+      const int row = 4 * g + (li >> 2), c = wn * 16 * QN + (ni >> 1) * 32 + (li & 3) * 8 + (ni & 1) * 4;
+      bt[ni] = (c >> 6) * (KE * 128) + row * 128 + ((((c & 63) >> 4) + (row >> 1)) & 3) * 32 + (c & 15) * 2;
+    } else {
+      const int row = 4 * g, c = wn * 16 * QN + lin_col(ni, li);
+      bt[ni] = (c >> 6) * (KE * 256) + row * 256 + ((((c & 63) >> 2) + rot32(row)) & 15) * 16 + (c & 3) * 4;
+    }
+  }
+  issue_a(0);
+  issue_b(0);
+  if constexpr (NB == 3) issue_b(1);
+  issue_a(1);
+  for (int kt = 0; kt < nk; ++kt) {
+    // all but what belongs to step kt + 1 alone has landed; every wave is past step kt - 1
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NB == 3 ? QM + QN : QM) : "memory");
+    issue_b(kt + NB - 1);
+    issue_a(kt + 2);
+    const char* sa = smem + (kt % 3) * A_BYTES;
+    const char* sb = smem + B0 + (kt % NB) * B_BYTES;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      uint4 fa[QM], fb[QN];
+#pragma unroll
+      for (int ni = 0; ni < QN; ++ni) {
+        if constexpr (!BT) {
+          fb[ni] = *reinterpret_cast<const uint4*>(sb + (kk ? fb0 ^ 64 : fb0) + (lin_col(ni, 0) - lin_col(0, 0)) * 128);
+        } else if constexpr (sizeof(T) == 2) {
+          typedef s16x4_t __attribute__((address_space(3))) * lds_ptr;
+          const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(sb + bt[ni] + kk * 4096)));
+          const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(sb + bt[ni] + kk * 4096 + 2048)));
+          fb[ni] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        } else {
+          const char* at = sb + bt[ni] + kk * 4096;
+          fb[ni] = make_uint4(*reinterpret_cast<const unsigned*>(at), *reinterpret_cast<const unsigned*>(at + 256), *reinterpret_cast<const unsigned*>(at + 512),
+                              *reinterpret_cast<const unsigned*>(at + 768));
+        }
+      }
+#pragma unroll
+      for (int mi = 0; mi < QM; ++mi) {
+        const char* at = sa + fa0 + mi * 2048;
+        if constexpr (BT && sizeof(T) == 2) {  // k = 32 kk + 4 g .. + 3 and 16 further: halves of chunks
+          const uint2 lo = *reinterpret_cast<const uint2*>(at + (((kk * 4 + (g >> 1)) ^ akey) * 16) + (g & 1) * 8);
+          const uint2 hi = *reinterpret_cast<const uint2*>(at + (((kk * 4 + 2 + (g >> 1)) ^ akey) * 16) + (g & 1) * 8);
+          fa[mi] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        } else {
+          fa[mi] = *reinterpret_cast<const uint4*>(at + (((kk * 4 + g) ^ akey) * 16));
+        }
+      }
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int mi = 0; mi < QM; ++mi)
+#pragma unroll
+          for (int ni = 0; ni < QN; ++ni) acc[mi][ni] = mma16<T>(fb[ni], fa[mi], acc[mi][ni]);
+      } else {  // element by element over all tiles: consecutive MFMAs do not wait for each other's sums
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int mi = 0; mi < QM; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < QN; ++ni) {
+              const unsigned b4[4] = {fb[ni].x, fb[ni].y, fb[ni].z, fb[ni].w}, a4[4] = {fa[mi].x, fa[mi].y, fa[mi].z, fa[mi].w};
+              acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(b4[e]), __uint_as_float(a4[e]), acc[mi][ni], 0, 0, 0);
+            }
+      }
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the DMAs past the end have landed before the LDS is given back
+#pragma unroll
+  for (int mi = 0; mi < QM; ++mi) {
+    const long long row = m0 + wm * 16 * QM + mi * 16 + li;
+    if (row >= p.M) continue;
+#pragma unroll
+    for (int j = 0; j < QN / 2; ++j) {
+      float v[8];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        v[r] = acc[mi][2 * j][r];
+        v[4 + r] = acc[mi][2 * j + 1][r];
+      }
+      linear_store8<T>(p, row, n0 + wn * 16 * QN + j * 32 + g * 8, v);
+    }
+  }
+}
+
 // Few rows: a block of 8 waves makes 16 columns of up to 16 MT rows; every wave takes each eighth 64-byte piece of K, both operands go from memory straight into MFMA
 // operands (no LDS: nothing is used twice), and the waves' sums meet in LDS.  What counts here is latency and the number of CUs that read w: 16 columns a block
 // put 32 blocks on 512 columns.
@@ -225,7 +397,6 @@ __global__ __launch_bounds__(256) void linear_act_bwd_kernel(const T* __restrict
 }
 
 // ---- dw = dz^T x ---------------------------------------------------------------------------------------------------------------
-typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 // 16-bit operand of 32 rows x 16 columns read transposed: lane gets rows {4g..4g+3, 16+4g..16+4g+3} of column cb + (lane & 15)
 __device__ __forceinline__ uint4 frag_tr16(const char* tile, int stride, int cb, int lane) {
   typedef s16x4_t __attribute__((address_space(3))) * lds_ptr;
@@ -241,19 +412,22 @@ __device__ __forceinline__ uint4 frag_tr16(const char* tile, int stride, int cb,
   return r;
 }
 
-template <typename T, bool A8>
-__global__ __launch_bounds__(256, 2) void linear_wgrad_kernel(WgradArgsL p) {
-  constexpr int VE = Vec16<T>::N;
-  constexpr int KP = sizeof(T) == 2 ? 32 : 16;      // rows per step
-  constexpr int CH = 128 / VE;                      // 16-byte chunks of a 128-column tile row
-  constexpr int STRIDE = 128 * sizeof(T) + (sizeof(T) == 2 ? 32 : 64);  // padded: the rows a transpose read / a group of lanes touches fall on different banks
+// TILE = 128 or 64 columns of either operand; waves as 2 x 2
+template <typename T, bool A8, int TILE>
+__global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_wgrad_kernel(WgradArgsL p) {
+  constexpr int VE = Vec16<T>::N, Q = TILE / 32;
+  constexpr int KP = sizeof(T) == 2 ? 32 : TILE == 128 ? 16 : 32;  // rows per step
+  constexpr int CH = TILE / VE;                     // 16-byte chunks of a tile row
+  constexpr int STRIDE = TILE * sizeof(T) + (sizeof(T) == 2 ? 32 : 64);  // padded: the rows a transpose read / a group of lanes touches fall on different banks
   constexpr int NCH = KP * CH / 256;                // chunks per thread and operand
-  __shared__ __attribute__((aligned(16))) char smem[2 * KP * STRIDE];
+  static_assert(NCH >= 1, "a chunk for every thread");
+  // two stages: a step's operands are written while the other stage is still being read, one barrier per step
+  __shared__ __attribute__((aligned(16))) char smem[4 * KP * STRIDE];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int li = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
   unsigned logical = xcd_order(blockIdx.x, gridDim.x);
-  const int k0 = (int)(logical % p.k_tiles) * 128; logical /= p.k_tiles;
-  const int n0 = (int)(logical % p.n_tiles) * 128;
+  const int k0 = (int)(logical % p.k_tiles) * TILE; logical /= p.k_tiles;
+  const int n0 = (int)(logical % p.n_tiles) * TILE;
   const int split = (int)(logical / p.n_tiles);
   const long long r0 = (long long)split * p.per_split;
   const long long r1 = r0 + p.per_split < p.M ? r0 + p.per_split : p.M;
@@ -284,16 +458,17 @@ __global__ __launch_bounds__(256, 2) void linear_wgrad_kernel(WgradArgsL p) {
       }
     }
   };
-  f32x4 acc[4][4];
+  f32x4 acc[Q][Q];
 #pragma unroll
-  for (int mi = 0; mi < 4; ++mi)
+  for (int mi = 0; mi < Q; ++mi)
 #pragma unroll
-    for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  char* td = smem;
-  char* tx = smem + KP * STRIDE;
+    for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
   load(r0);
+  int stage = 0;
   for (long long r = r0; r < r1; r += KP) {
-    __syncthreads();
+    char* td = smem + stage * (2 * KP * STRIDE);
+    char* tx = td + KP * STRIDE;
+    stage ^= 1;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int q = tid + 256 * i;
@@ -304,42 +479,42 @@ __global__ __launch_bounds__(256, 2) void linear_wgrad_kernel(WgradArgsL p) {
     __syncthreads();
     if (r + KP < r1) load(r + KP);
     if constexpr (sizeof(T) == 2) {
-      uint4 fd[4], fx[4];
+      uint4 fd[Q], fx[Q];
 #pragma unroll
-      for (int mi = 0; mi < 4; ++mi) fd[mi] = frag_tr16(td, STRIDE, wm * 64 + mi * 16, lane);
+      for (int mi = 0; mi < Q; ++mi) fd[mi] = frag_tr16(td, STRIDE, wm * 16 * Q + mi * 16, lane);
 #pragma unroll
-      for (int ni = 0; ni < 4; ++ni) fx[ni] = frag_tr16(tx, STRIDE, wn * 64 + ni * 16, lane);
+      for (int ni = 0; ni < Q; ++ni) fx[ni] = frag_tr16(tx, STRIDE, wn * 16 * Q + ni * 16, lane);
 #pragma unroll
-      for (int mi = 0; mi < 4; ++mi)
+      for (int mi = 0; mi < Q; ++mi)
 #pragma unroll
-        for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = mma16<T>(fd[mi], fx[ni], acc[mi][ni]);
+        for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = mma16<T>(fd[mi], fx[ni], acc[mi][ni]);
     } else {
 #pragma unroll
       for (int s4 = 0; s4 < KP / 4; ++s4) {
-        float fd[4], fx[4];
+        float fd[Q], fx[Q];
 #pragma unroll
-        for (int mi = 0; mi < 4; ++mi) {
-          fd[mi] = *reinterpret_cast<const float*>(td + (s4 * 4 + g) * STRIDE + (wm * 64 + mi * 16 + li) * 4);
-          fx[mi] = *reinterpret_cast<const float*>(tx + (s4 * 4 + g) * STRIDE + (wn * 64 + mi * 16 + li) * 4);
+        for (int mi = 0; mi < Q; ++mi) {
+          fd[mi] = *reinterpret_cast<const float*>(td + (s4 * 4 + g) * STRIDE + (wm * 16 * Q + mi * 16 + li) * 4);
+          fx[mi] = *reinterpret_cast<const float*>(tx + (s4 * 4 + g) * STRIDE + (wn * 16 * Q + mi * 16 + li) * 4);
         }
 #pragma unroll
-        for (int mi = 0; mi < 4; ++mi)
+        for (int mi = 0; mi < Q; ++mi)
 #pragma unroll
-          for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x4f32(fd[mi], fx[ni], acc[mi][ni], 0, 0, 0);
+          for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x4f32(fd[mi], fx[ni], acc[mi][ni], 0, 0, 0);
       }
     }
   }
   // lane: rows n = n0 + wm 64 + 16 mi + 4 g + r, column k = k0 + wn 64 + 16 ni + li
   float* out = p.part + (long long)split * p.N * p.K;
 #pragma unroll
-  for (int mi = 0; mi < 4; ++mi)
+  for (int mi = 0; mi < Q; ++mi)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int n = n0 + wm * 64 + mi * 16 + 4 * g + r;
+      const int n = n0 + wm * 16 * Q + mi * 16 + 4 * g + r;
       if (n >= p.N) continue;
 #pragma unroll
-      for (int ni = 0; ni < 4; ++ni) {
-        const int k = k0 + wn * 64 + ni * 16 + li;
+      for (int ni = 0; ni < Q; ++ni) {
+        const int k = k0 + wn * 16 * Q + ni * 16 + li;
         if (k < p.K) out[(long long)n * p.K + k] = acc[mi][ni][r];
       }
     }
@@ -367,6 +542,21 @@ static int linear_bad(const char* what, int64_t rows, int in, int out, int dtype
   return 0;
 }
 
+template <bool BT> static int dma_launch(LinearArgs p, int dtype, hipStream_t s, const char* what) {
+  auto count = [&](int bm, int bn) { return (int64_t)ceil_div(p.M, bm) * ceil_div(p.N, bn); };
+  const int bm = count(128, 64) >= 512 ? 128 : 64, bn = count(128, 128) >= 512 && p.N > 64 ? 128 : 64;
+  p.n_tiles = (unsigned)ceil_div(p.N, bn);
+  const unsigned grid = (unsigned)ceil_div(p.M, bm) * p.n_tiles;
+#define SH_DMA(T)                                                                  \
+  if (bn == 128) linear_dma_kernel<T, 4, 4, BT><<<grid, 256, 0, s>>>(p);           \
+  else if (bm == 128) linear_dma_kernel<T, 4, 2, BT><<<grid, 256, 0, s>>>(p);      \
+  else linear_dma_kernel<T, 2, 2, BT><<<grid, 256, 0, s>>>(p);
+  if (dtype == SH_F32) { SH_DMA(float) }
+  else { SH_DMA(bf16_t) }
+#undef SH_DMA
+  return check_launch(what);
+}
+
 // Which kernel: few rows -> the skinny one (rows <= 64 and so little work that tiles would leave most CUs idle); 64-wide tiles while 128-wide ones would not put two
 // blocks on each of the 256 CUs; else 128-wide ones.
 static int gemm_launch(const LinearArgs& base, int dtype, hipStream_t s, const char* what) {
@@ -388,6 +578,8 @@ static int gemm_launch(const LinearArgs& base, int dtype, hipStream_t s, const c
     return check_launch(what);
   }
   if (linear256_takes(p, dtype)) return linear256_launch(p, s, what);
+  const int ve = dtype == SH_F32 ? 4 : 8;
+  if (p.K % ve == 0 && p.ldb % ve == 0 && !(((size_t)p.a | (size_t)p.b) & 15)) return dma_launch<false>(p, dtype, s, what);
   const int tile = (int64_t)ceil_div(p.M, 128) * ceil_div(p.N, 128) >= 512 ? 128 : 64;
   p.n_tiles = (unsigned)ceil_div(p.N, tile);
   const unsigned grid = (unsigned)ceil_div(p.M, tile) * p.n_tiles;
@@ -417,16 +609,21 @@ static void act_bwd_plan(int64_t rows, int cols, int dtype, int* gx, int* gy, in
   if (*gy < 1) *gy = 1;
 }
 
-static void linear_wgrad_plan(int64_t rows, int in, int out, int dtype, int* splits, int64_t* per) {
-  const int kp = dtype == SH_F32 ? 16 : 32;
-  const int64_t tiles = (int64_t)ceil_div(in, 128) * ceil_div(out, 128);
+// Tile and splits over the rows: 128-wide tiles while they are enough for two blocks per CU with at most 8 splits (every split writes and re-reads its own dw), else 64-wide ones
+// (four blocks per CU).
+static int linear_wgrad_plan(int64_t rows, int in, int out, int dtype, int* splits, int64_t* per) {
+  const int64_t t128 = (int64_t)ceil_div(in, 128) * ceil_div(out, 128);
+  const int tile = t128 * 8 >= 512 || rows > 65536 ? 128 : 64, blocks = tile == 128 ? 512 : 1024;
+  const int kp = dtype == SH_F32 && tile == 128 ? 16 : 32;
+  const int64_t tiles = (int64_t)ceil_div(in, tile) * ceil_div(out, tile);
   const int64_t steps = rows > 0 ? (rows + kp - 1) / kp : 1;
-  int64_t sk = 512 / tiles;
-  if (sk > (steps + 15) / 16) sk = (steps + 15) / 16;  // at least 16 steps each
+  int64_t sk = blocks / tiles;
+  if (sk > (steps + 7) / 8) sk = (steps + 7) / 8;  // at least 8 steps each
   if (sk < 1) sk = 1;
   const int64_t each = (steps + sk - 1) / sk;
   *per = each * kp;
   *splits = (int)((steps + each - 1) / each);
+  return tile;
 }
 
 }  // namespace sh
@@ -500,13 +697,18 @@ int simhand_linear_dgrad(const void* dz, const void* w, void* dx, int64_t rows, 
   hipStream_t s = (hipStream_t)stream;
   const double eb = dtype == SH_F32 ? 4 : 2;
   ProfScope ps(SH_PROF_MISC, s, 2.0 * rows * in_dim * out_dim, eb * ((double)rows * in_dim + (double)in_dim * out_dim + (double)rows * out_dim));
+  // dx = dz w with w as it is, unless the product is large enough for the 256-wide tiles (whose transposed copy of w is then small change) or w's rows are no whole chunks
+  const int ve = dtype == SH_F32 ? 4 : 8;
+  LinearArgs direct = {dz, w, dx, nullptr, nullptr, nullptr, rows, in_dim, out_dim, in_dim, SH_ACT_NONE, 0};
+  LinearArgs wide = {dz, workspace, dx, nullptr, nullptr, nullptr, rows, in_dim, out_dim, (out_dim + 7) / 8 * 8, SH_ACT_NONE, 0};
+  if (in_dim % ve == 0 && out_dim % ve == 0 && !(((size_t)dz | (size_t)w) & 15) && !linear256_takes(wide, dtype))
+    return dma_launch<true>(direct, dtype, s, "linear_dgrad");
   const int ldt = (out_dim + 7) / 8 * 8;
   const dim3 tg(ceil_div(in_dim, 32), ceil_div(ldt, 32));
   if (dtype == SH_F32) linear_transpose_kernel<float><<<tg, 256, 0, s>>>((const float*)w, (float*)workspace, out_dim, in_dim, ldt);
   else linear_transpose_kernel<bf16_t><<<tg, 256, 0, s>>>((const bf16_t*)w, (bf16_t*)workspace, out_dim, in_dim, ldt);
   if (check_launch("linear_dgrad")) return 1;
-  LinearArgs p = {dz, workspace, dx, nullptr, nullptr, nullptr, rows, in_dim, out_dim, ldt, SH_ACT_NONE, 0};
-  return gemm_launch(p, dtype, s, "linear_dgrad");
+  return gemm_launch(wide, dtype, s, "linear_dgrad");
 }
 
 size_t simhand_linear_wgrad_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype) {
@@ -517,7 +719,7 @@ size_t simhand_linear_wgrad_workspace_bytes(int64_t rows, int in_dim, int out_di
   linear_wgrad_plan(rows, in_dim, out_dim, dtype, &splits, &per);
   if (linear_wgrad256_takes(nullptr, nullptr, nullptr, nullptr, rows, in_dim, out_dim, dtype)) linear_wgrad256_plan(rows, in_dim, out_dim, &wide, &per);
   if (wide > splits) splits = wide;
-  return splits > 1 ? (size_t)splits * in_dim * out_dim * sizeof(float) : 16;
+  return splits > 1 ? (size_t)splits * in_dim * out_dim * sizeof(float) : 0;
 }
 
 int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, float* dw, int64_t rows, int in_dim, int out_dim,
@@ -526,7 +728,8 @@ int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, 
   const bool a8 = x_codes != nullptr;
   SH_REQUIRE(!a8 || (x_exps && !x), "linear_wgrad: pass either x or its codes and exponents");
   SH_REQUIRE(dw && (rows == 0 || (dz && (x || a8))), "linear_wgrad: NULL argument");
-  SH_REQUIRE(workspace && workspace_bytes >= simhand_linear_wgrad_workspace_bytes(rows, in_dim, out_dim, dtype), "linear_wgrad: workspace too small");
+  const size_t need = simhand_linear_wgrad_workspace_bytes(rows, in_dim, out_dim, dtype);
+  SH_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "linear_wgrad: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   const double eb = dtype == SH_F32 ? 4 : 2;
   ProfScope ps(SH_PROF_MISC, s, 2.0 * rows * in_dim * out_dim, eb * (double)rows * out_dim + (a8 ? 1.03125 : eb) * rows * in_dim + 4.0 * in_dim * out_dim);
@@ -538,21 +741,26 @@ int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, 
   int splits;
   int64_t per;
   const bool wide = linear_wgrad256_takes(dz, x, x_codes, x_exps, rows, in_dim, out_dim, dtype);
+  int tile = 256;
   if (wide) linear_wgrad256_plan(rows, in_dim, out_dim, &splits, &per);
-  else linear_wgrad_plan(rows, in_dim, out_dim, dtype, &splits, &per);
-  WgradArgsL p = {dz, x, x_codes, x_exps, splits > 1 ? (float*)workspace : dw, rows, per, out_dim, in_dim, (unsigned)ceil_div(out_dim, 128),
-                  (unsigned)ceil_div(in_dim, 128)};
+  else tile = linear_wgrad_plan(rows, in_dim, out_dim, dtype, &splits, &per);
+  WgradArgsL p = {dz, x, x_codes, x_exps, splits > 1 ? (float*)workspace : dw, rows, per, out_dim, in_dim, (unsigned)ceil_div(out_dim, tile),
+                  (unsigned)ceil_div(in_dim, tile)};
   if (wide) {
     if (linear_wgrad256_launch(p, splits, s)) return 1;
   } else {
     const unsigned grid = p.n_tiles * p.k_tiles * (unsigned)splits;
+#define SH_WGRAD(T, A8)                                                             \
+  if (tile == 128) linear_wgrad_kernel<T, A8, 128><<<grid, 256, 0, s>>>(p);         \
+  else linear_wgrad_kernel<T, A8, 64><<<grid, 256, 0, s>>>(p)
     if (dtype == SH_F32) {
-      if (a8) linear_wgrad_kernel<float, true><<<grid, 256, 0, s>>>(p);
-      else linear_wgrad_kernel<float, false><<<grid, 256, 0, s>>>(p);
+      if (a8) { SH_WGRAD(float, true); }
+      else { SH_WGRAD(float, false); }
     } else {
-      if (a8) linear_wgrad_kernel<bf16_t, true><<<grid, 256, 0, s>>>(p);
-      else linear_wgrad_kernel<bf16_t, false><<<grid, 256, 0, s>>>(p);
+      if (a8) { SH_WGRAD(bf16_t, true); }
+      else { SH_WGRAD(bf16_t, false); }
     }
+#undef SH_WGRAD
     if (check_launch("linear_wgrad")) return 1;
   }
   if (splits > 1) {

@@ -353,14 +353,23 @@ def linear_bwd(dz: torch.Tensor, x, w: torch.Tensor, need_dx: bool = True):
     xshape = dz.shape[:-1] + (cin,)
     if x.shape != xshape:
         raise _lib.SimhandHipError(f"linear_bwd: x must be {tuple(xshape)}, got {tuple(x.shape)}")
+    pz = _at(dz)
+    px, pc, pe = _saved(x, dz, xshape, "linear_bwd (x)")
     dx = None
     if need_dx:
-        pz = _at(dz)
         dx = torch.empty(xshape, dtype=dz.dtype, device=dz.device)
         nb = lib.simhand_linear_dgrad_workspace_bytes(cin, cout, d)
         ws = _scratch(nb, dz)
         check(lib.simhand_linear_dgrad(pz, pw, dx.data_ptr(), rows, cin, cout, d, ws.data_ptr(), nb, _row_stream(dz)), "linear_dgrad")
-    return dx, linear_wgrad(dz, x)
+    return dx, _wgrad(lib, dz, pz, px, pc, pe, rows, cin, cout, d)
+
+
+def _wgrad(lib, dz, pz, px, pc, pe, rows, cin, cout, d) -> torch.Tensor:
+    dw = torch.empty((cout, cin), dtype=_F32, device=dz.device)
+    nb = lib.simhand_linear_wgrad_workspace_bytes(rows, cin, cout, d)
+    ws = _scratch(nb, dz) if nb else None
+    check(lib.simhand_linear_wgrad(pz, px, pc, pe, dw.data_ptr(), rows, cin, cout, d, ws.data_ptr() if nb else 0, nb, _row_stream(dz)), "linear_wgrad")
+    return dw
 
 
 def linear_wgrad(dz: torch.Tensor, x) -> torch.Tensor:
@@ -368,17 +377,11 @@ def linear_wgrad(dz: torch.Tensor, x) -> torch.Tensor:
     input was kept in 8 bits: dz and x with pixels as rows."""
     rows, cout = _rows_of(dz, "linear_wgrad")
     lib = _lib_dev()
-    d = dt(dz.dtype)
     if len(x.shape) < 1 or x.shape[-1] < 1:
         raise _lib.SimhandHipError(f"linear_wgrad: rows of at least one value, got x of shape {tuple(x.shape)}")
     cin = x.shape[-1]
-    pz = _at(dz)
     px, pc, pe = _saved(x, dz, dz.shape[:-1] + (cin,), "linear_wgrad (x)")
-    dw = torch.empty((cout, cin), dtype=_F32, device=dz.device)
-    nb = lib.simhand_linear_wgrad_workspace_bytes(rows, cin, cout, d)
-    ws = _scratch(nb, dz)
-    check(lib.simhand_linear_wgrad(pz, px, pc, pe, dw.data_ptr(), rows, cin, cout, d, ws.data_ptr(), nb, _row_stream(dz)), "linear_wgrad")
-    return dw
+    return _wgrad(lib, dz, _at(dz), px, pc, pe, rows, cin, cout, dt(dz.dtype))
 
 
 def act8_pack(x: torch.Tensor) -> Act8:

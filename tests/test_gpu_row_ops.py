@@ -236,7 +236,7 @@ def test_linear_act_backward(dtype, rows, cols, act):
     close(db, want.sum(dim=0), (rows + 4) * U * want.abs().sum(dim=0) + fp.sum(dim=0) + 1e-30, "db")
 
 
-@pytest.mark.parametrize("m,k,n", SHAPES_LIN + [(5000, 64, 64), (4097, 40, 72), (1000, 256, 512)])
+@pytest.mark.parametrize("m,k,n", SHAPES_LIN + [(5000, 64, 64), (4097, 40, 72), (1000, 256, 512), (2048, 520, 264), (70, 264, 1032), (5, 128, 136), (8200, 72, 200)])
 @pytest.mark.parametrize("act8", [False, True])
 def test_linear_backward(dtype, m, k, n, act8):
     from simhand_amd import ops
@@ -528,7 +528,7 @@ def test_nothing_is_written_beside_the_outputs(dtype):
     ws = torch.empty(lib.simhand_linear_dgrad_workspace_bytes(k, n, d), dtype=torch.uint8, device="cuda")
     assert lib.simhand_linear_dgrad(p(dz), p(w), p(dxv), m, k, n, d, p(ws), ws.numel(), st) == 0
     dw, dwv = guarded(n * k, torch.float32)
-    ws2 = torch.empty(lib.simhand_linear_wgrad_workspace_bytes(m, k, n, d), dtype=torch.uint8, device="cuda")
+    ws2 = torch.empty(lib.simhand_linear_wgrad_workspace_bytes(m, k, n, d) + 16, dtype=torch.uint8, device="cuda")
     assert lib.simhand_linear_wgrad(p(dz), p(x), None, None, p(dwv), m, k, n, d, p(ws2), ws2.numel(), st) == 0
     codes, cv = guarded(m * k, torch.uint8); exps, ev = guarded(m * 2, torch.uint8)
     assert lib.simhand_act8_pack(p(x), p(cv), p(ev), m, k, d, st) == 0

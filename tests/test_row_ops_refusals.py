@@ -36,6 +36,7 @@ def test_c_entry_points_refuse_bad_arguments():
     assert refused(lib.simhand_linear_dgrad(P, P, P, 4, 8, 8, 0, P, 8, N))                         # workspace
     assert refused(lib.simhand_linear_wgrad(P, P, N, N, N, 4, 8, 8, 0, P, 1 << 20, N))             # dw
     assert refused(lib.simhand_linear_wgrad(P, P, N, N, P, 4, 8, 8, 2, P, 1 << 20, N))             # dtype
+    assert refused(lib.simhand_linear_wgrad(P, P, N, N, P, 100000, 512, 512, 1, N, 0, N))          # workspace
     assert refused(lib.simhand_act8_pack(P, P, N, 4, 8, 0, N))                                     # exps
     assert refused(lib.simhand_act8_pack(P, P, P, 4, 0, 0, N))                                     # cols
     assert refused(lib.simhand_act8_unpack(P, P, P, -4, 8, 0, N))                                  # rows
@@ -57,7 +58,7 @@ def test_workspace_queries():
     for rows in (0, 1, 1000, 401408, (1 << 31) - 1):
         for cols in (1, 77, 2048):
             assert 0 < lib.simhand_linear_act_bwd_workspace_bytes(rows, cols, 1) < 1 << 28
-            assert 0 < lib.simhand_linear_wgrad_workspace_bytes(rows, cols, 512, 1) < 1 << 30
+            assert 0 <= lib.simhand_linear_wgrad_workspace_bytes(rows, cols, 512, 1) < 1 << 30
 
 
 def test_python_layer_refuses_host_tensors():
