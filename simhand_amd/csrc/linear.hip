@@ -98,9 +98,9 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_gemm_kernel(L
   }
 }
 
-// The same product with both operands by LDS-DMA, for rows of whole 16-byte chunks: two k-steps ahead, one barrier per step and nothing staged in registers.  Waves as 2 x 2, each
-// QM x QN MFMA tiles: 128 x 128 (80 KB of LDS, weights only one step ahead: two blocks per CU), 128 x 64 (two), 64 x 64 (three) -- the largest that still puts two blocks on every
-// CU.  One block's epilogue runs under the others' k-loops.
+// The same product with both operands by LDS-DMA, for rows of whole 16-byte chunks: several k-steps ahead, one barrier per step and nothing staged in registers.  Waves as 2 x 2, each
+// QM x QN MFMA tiles: 128 x 128 (80 KB of LDS: activations two steps ahead, weights one), 128 x 64 (72 KB, two steps), 64 x 64 (80 KB, four steps: so small a tile is all
+// latency) -- the largest that still puts two blocks on every CU.  One block's epilogue runs under the other's k-loop.
 // BT: b is stored [K][N] (dx = dz w reads w as it is, without a transposed copy): its tile is sub-tiles of 64 columns by K rows, 16-bit operands are read transposed
 // (ds_read_b64_tr_b16; the activations' chunks are then read in the halves that match its row order), fp32 ones element by element.
 __device__ uint4 g_lin_zero[8];  // read-only zeros
@@ -108,11 +108,11 @@ __device__ uint4 g_lin_zero[8];  // read-only zeros
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 
 template <typename T, int QM, int QN, bool BT>
-__global__ __launch_bounds__(256, QM == 2 ? 3 : 2) void linear_dma_kernel(LinearArgs p) {
+__global__ __launch_bounds__(256, 2) void linear_dma_kernel(LinearArgs p) {
   constexpr int VE = Vec16<T>::N, KE = 128 / sizeof(T), BM = 32 * QM, BN = 32 * QN;
-  constexpr int NB = QN == 4 ? 2 : 3;  // stages of b
-  constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, B0 = 3 * A_BYTES;
-  __shared__ __attribute__((aligned(16))) char smem[3 * A_BYTES + NB * B_BYTES];
+  constexpr int NA = QM == 2 ? 5 : 3, NB = QN == 4 ? 2 : NA;  // stages
+  constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, B0 = NA * A_BYTES;
+  __shared__ __attribute__((aligned(16))) char smem[NA * A_BYTES + NB * B_BYTES];
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
   // inline asm: hipcc's wait-count pass would drain every outstanding LDS-DMA in front of each LDS read; the loop counts them itself
   auto dma16 = [](const void* src, unsigned lds_addr) __attribute__((always_inline)) {
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256, QM == 2 ? 3 : 2) void linear_dma_kernel(Linear
   const long long b_step = BT ? (long long)KE * p.ldb * (int)sizeof(T) : 128;
   auto issue_a = [&](int kt) __attribute__((always_inline)) {
     const bool ok = kt * KE + ka < p.K;
-    const unsigned dst = lds0 + (kt % 3) * A_BYTES + wave * 1024;
+    const unsigned dst = lds0 + (kt % NA) * A_BYTES + wave * 1024;
 #pragma unroll
     for (int i = 0; i < QM; ++i) dma16(ok ? pa[i] + kt * 128 : zero, dst + i * 4096);
   };
@@ -194,16 +194,17 @@ __global__ __launch_bounds__(256, QM == 2 ? 3 : 2) void linear_dma_kernel(Linear
       bt[ni] = (c >> 6) * (KE * 256) + row * 256 + ((((c & 63) >> 2) + rot32(row)) & 15) * 16 + (c & 3) * 4;
     }
   }
-  issue_a(0);
-  issue_b(0);
-  if constexpr (NB == 3) issue_b(1);
-  issue_a(1);
+#pragma unroll
+  for (int i = 0; i < NA - 1; ++i) {
+    if (i < NB - 1) issue_b(i);
+    issue_a(i);
+  }
   for (int kt = 0; kt < nk; ++kt) {
-    // all but what belongs to step kt + 1 alone has landed; every wave is past step kt - 1
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NB == 3 ? QM + QN : QM) : "memory");
+    // all but what belongs to the steps behind kt alone has landed (NB = 2: the activations of step kt + 1); every wave is past step kt - 1
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NB == 2 ? QM : (NA - 2) * (QM + QN)) : "memory");
     issue_b(kt + NB - 1);
-    issue_a(kt + 2);
-    const char* sa = smem + (kt % 3) * A_BYTES;
+    issue_a(kt + NA - 1);
+    const char* sa = smem + (kt % NA) * A_BYTES;
     const char* sb = smem + B0 + (kt % NB) * B_BYTES;
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
@@ -291,7 +292,7 @@ __global__ __launch_bounds__(512) void linear_skinny_kernel(LinearArgs p) {
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const int k_first = wave * KE + g * VE;
-  constexpr int U = MT >= 4 ? 2 : 4;  // pieces in flight
+  constexpr int U = MT >= 4 ? 2 : MT == 2 ? 4 : 8;  // pieces in flight
   int k0 = k_first;
   for (; k0 - g * VE + (U - 1) * W * KE + KE <= p.K; k0 += U * W * KE) {  // U whole pieces
     uint4 b[U], a[U][MT];
@@ -412,9 +413,10 @@ __device__ __forceinline__ uint4 frag_tr16(const char* tile, int stride, int cb,
   return r;
 }
 
-// TILE = 128 or 64 columns of either operand; waves as 2 x 2
-template <typename T, bool A8, int TILE>
-__global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_wgrad_kernel(WgradArgsL p) {
+// TILE = 128 or 64 columns of either operand; waves as 2 x 2.  GR = 2: two such groups of waves in a block take the steps in turn and add their sums in LDS at the end -- for
+// about as many tiles as CUs, where splits over blocks would write, re-read and add several copies of dw to keep two waves on every SIMD.
+template <typename T, bool A8, int TILE, int GR>
+__global__ __launch_bounds__(256 * GR, TILE == 128 ? 2 : 4 / GR) void linear_wgrad_kernel(WgradArgsL p) {
   constexpr int VE = Vec16<T>::N, Q = TILE / 32;
   constexpr int KP = sizeof(T) == 2 ? 32 : TILE == 128 ? 16 : 32;  // rows per step
   constexpr int CH = TILE / VE;                     // 16-byte chunks of a tile row
@@ -422,8 +424,9 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_wgrad_kernel(
   constexpr int NCH = KP * CH / 256;                // chunks per thread and operand
   static_assert(NCH >= 1, "a chunk for every thread");
   // two stages: a step's operands are written while the other stage is still being read, one barrier per step
-  __shared__ __attribute__((aligned(16))) char smem[4 * KP * STRIDE];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  constexpr int GROUP = 4 * KP * STRIDE;
+  __shared__ __attribute__((aligned(16))) char smem[GR * GROUP];
+  const int tid = threadIdx.x & 255, grp = GR == 1 ? 0 : threadIdx.x >> 8, wave = tid >> 6, lane = tid & 63;
   const int li = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
   unsigned logical = xcd_order(blockIdx.x, gridDim.x);
   const int k0 = (int)(logical % p.k_tiles) * TILE; logical /= p.k_tiles;
@@ -463,10 +466,10 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_wgrad_kernel(
   for (int mi = 0; mi < Q; ++mi)
 #pragma unroll
     for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  load(r0);
+  load(r0 + grp * KP);
   int stage = 0;
-  for (long long r = r0; r < r1; r += KP) {
-    char* td = smem + stage * (2 * KP * STRIDE);
+  for (long long r = r0; r < r1; r += KP * GR) {  // (rows past r1 are zeros: the groups take as many turns)
+    char* td = smem + grp * GROUP + stage * (2 * KP * STRIDE);
     char* tx = td + KP * STRIDE;
     stage ^= 1;
 #pragma unroll
@@ -477,7 +480,7 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_wgrad_kernel(
       *reinterpret_cast<uint4*>(tx + at) = rx[i];
     }
     __syncthreads();
-    if (r + KP < r1) load(r + KP);
+    if (r + KP * GR < r1) load(r + KP * GR + grp * KP);
     if constexpr (sizeof(T) == 2) {
       uint4 fd[Q], fx[Q];
 #pragma unroll
@@ -503,6 +506,27 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_wgrad_kernel(
           for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x4f32(fd[mi], fx[ni], acc[mi][ni], 0, 0, 0);
       }
     }
+  }
+  if constexpr (GR == 2) {
+    static_assert(GR * GROUP >= TILE * TILE * 4, "the second group's sums fit");
+    float* sums = reinterpret_cast<float*>(smem);
+    __syncthreads();
+    if (grp == 1) {
+#pragma unroll
+      for (int mi = 0; mi < Q; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < Q; ++ni)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sums[((mi * Q + ni) * 4 + r) * 256 + tid] = acc[mi][ni][r];
+    }
+    __syncthreads();
+    if (grp == 1) return;
+#pragma unroll
+    for (int mi = 0; mi < Q; ++mi)
+#pragma unroll
+      for (int ni = 0; ni < Q; ++ni)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[mi][ni][r] += sums[((mi * Q + ni) * 4 + r) * 256 + tid];
   }
   // lane: rows n = n0 + wm 64 + 16 mi + 4 g + r, column k = k0 + wn 64 + 16 ni + li
   float* out = p.part + (long long)split * p.N * p.K;
@@ -577,6 +601,7 @@ static int gemm_launch(const LinearArgs& base, int dtype, hipStream_t s, const c
 #undef SH_SKINNY
     return check_launch(what);
   }
+  if (linear_rows_takes(p, dtype)) return linear_rows_launch(p, s, what);
   if (linear256_takes(p, dtype)) return linear256_launch(p, s, what);
   const int ve = dtype == SH_F32 ? 4 : 8;
   if (p.K % ve == 0 && p.ldb % ve == 0 && !(((size_t)p.a | (size_t)p.b) & 15)) return dma_launch<false>(p, dtype, s, what);
@@ -609,13 +634,18 @@ static void act_bwd_plan(int64_t rows, int cols, int dtype, int* gx, int* gy, in
   if (*gy < 1) *gy = 1;
 }
 
-// Tile and splits over the rows: 128-wide tiles while they are enough for two blocks per CU with at most 8 splits (every split writes and re-reads its own dw), else 64-wide ones
-// (four blocks per CU).
+// Tile and splits over the rows: two groups of waves per 64-wide tile where there are about as many tiles as CUs (no splits: tile code 65); else 128-wide tiles while they are
+// enough for two blocks per CU with at most 8 splits (every split writes and re-reads its own dw), else 64-wide ones (four blocks per CU).
 static int linear_wgrad_plan(int64_t rows, int in, int out, int dtype, int* splits, int64_t* per) {
-  const int64_t t128 = (int64_t)ceil_div(in, 128) * ceil_div(out, 128);
+  const int64_t t128 = (int64_t)ceil_div(in, 128) * ceil_div(out, 128), t64 = (int64_t)ceil_div(in, 64) * ceil_div(out, 64);
+  if (t64 >= 192 && t64 <= 256 && rows >= 256 && rows <= 16384) {
+    *splits = 1;
+    *per = rows;
+    return 65;
+  }
   const int tile = t128 * 8 >= 512 || rows > 65536 ? 128 : 64, blocks = tile == 128 ? 512 : 1024;
   const int kp = dtype == SH_F32 && tile == 128 ? 16 : 32;
-  const int64_t tiles = (int64_t)ceil_div(in, tile) * ceil_div(out, tile);
+  const int64_t tiles = tile == 128 ? t128 : t64;
   const int64_t steps = rows > 0 ? (rows + kp - 1) / kp : 1;
   int64_t sk = blocks / tiles;
   if (sk > (steps + 7) / 8) sk = (steps + 7) / 8;  // at least 8 steps each
@@ -701,7 +731,7 @@ int simhand_linear_dgrad(const void* dz, const void* w, void* dx, int64_t rows, 
   const int ve = dtype == SH_F32 ? 4 : 8;
   LinearArgs direct = {dz, w, dx, nullptr, nullptr, nullptr, rows, in_dim, out_dim, in_dim, SH_ACT_NONE, 0};
   LinearArgs wide = {dz, workspace, dx, nullptr, nullptr, nullptr, rows, in_dim, out_dim, (out_dim + 7) / 8 * 8, SH_ACT_NONE, 0};
-  if (in_dim % ve == 0 && out_dim % ve == 0 && !(((size_t)dz | (size_t)w) & 15) && !linear256_takes(wide, dtype))
+  if (in_dim % ve == 0 && out_dim % ve == 0 && !(((size_t)dz | (size_t)w) & 15) && !linear256_takes(wide, dtype) && !linear_rows_takes(wide, dtype))
     return dma_launch<true>(direct, dtype, s, "linear_dgrad");
   const int ldt = (out_dim + 7) / 8 * 8;
   const dim3 tg(ceil_div(in_dim, 32), ceil_div(ldt, 32));
@@ -744,15 +774,16 @@ int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, 
   int tile = 256;
   if (wide) linear_wgrad256_plan(rows, in_dim, out_dim, &splits, &per);
   else tile = linear_wgrad_plan(rows, in_dim, out_dim, dtype, &splits, &per);
-  WgradArgsL p = {dz, x, x_codes, x_exps, splits > 1 ? (float*)workspace : dw, rows, per, out_dim, in_dim, (unsigned)ceil_div(out_dim, tile),
-                  (unsigned)ceil_div(in_dim, tile)};
+  WgradArgsL p = {dz, x, x_codes, x_exps, splits > 1 ? (float*)workspace : dw, rows, per, out_dim, in_dim, (unsigned)ceil_div(out_dim, tile & ~1),
+                  (unsigned)ceil_div(in_dim, tile & ~1)};
   if (wide) {
     if (linear_wgrad256_launch(p, splits, s)) return 1;
   } else {
     const unsigned grid = p.n_tiles * p.k_tiles * (unsigned)splits;
-#define SH_WGRAD(T, A8)                                                             \
-  if (tile == 128) linear_wgrad_kernel<T, A8, 128><<<grid, 256, 0, s>>>(p);         \
-  else linear_wgrad_kernel<T, A8, 64><<<grid, 256, 0, s>>>(p)
+#define SH_WGRAD(T, A8)                                                               \
+  if (tile == 128) linear_wgrad_kernel<T, A8, 128, 1><<<grid, 256, 0, s>>>(p);        \
+  else if (tile == 65) linear_wgrad_kernel<T, A8, 64, 2><<<grid, 512, 0, s>>>(p);     \
+  else linear_wgrad_kernel<T, A8, 64, 1><<<grid, 256, 0, s>>>(p)
     if (dtype == SH_F32) {
       if (a8) { SH_WGRAD(float, true); }
       else { SH_WGRAD(float, false); }

@@ -191,7 +191,8 @@ def test_linear_forward(dtype, m, k, n, act, bias, residual, pre):
 
 # the kernel for many rows (16 bits, rows of 16-byte chunks, at least 192 tiles of 256 x 256): whole tiles, ragged rows / columns / K, one to five k-steps, the smallest N, several
 # tiles per block
-SHAPES_MANY = [(49152, 64, 256), (49100, 72, 136), (24600, 128, 520), (6200, 320, 2048), (30011, 8, 384), (131072 + 40, 200, 128), (16640, 136, 1032)]
+SHAPES_MANY = [(49152, 64, 256), (49100, 72, 136), (24600, 128, 520), (6200, 320, 2048), (30011, 8, 384), (131072 + 40, 200, 128), (16640, 136, 1032),
+               (16384, 512, 1024), (16389, 384, 1024), (33000, 256, 576), (70001, 120, 320), (66000, 72, 256), (9000, 504, 2048), (524288 + 3, 64, 64)]
 
 
 @pytest.mark.parametrize("m,k,n", SHAPES_MANY)
@@ -236,7 +237,7 @@ def test_linear_act_backward(dtype, rows, cols, act):
     close(db, want.sum(dim=0), (rows + 4) * U * want.abs().sum(dim=0) + fp.sum(dim=0) + 1e-30, "db")
 
 
-@pytest.mark.parametrize("m,k,n", SHAPES_LIN + [(5000, 64, 64), (4097, 40, 72), (1000, 256, 512), (2048, 520, 264), (70, 264, 1032), (5, 128, 136), (8200, 72, 200)])
+@pytest.mark.parametrize("m,k,n", SHAPES_LIN + [(5000, 64, 64), (4097, 40, 72), (1000, 256, 512), (2048, 520, 264), (70, 264, 1032), (5, 128, 136), (8200, 72, 200), (300, 1024, 776), (259, 820, 1024)])
 @pytest.mark.parametrize("act8", [False, True])
 def test_linear_backward(dtype, m, k, n, act8):
     from simhand_amd import ops
