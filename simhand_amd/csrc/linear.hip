@@ -413,10 +413,10 @@ __device__ __forceinline__ uint4 frag_tr16(const char* tile, int stride, int cb,
   return r;
 }
 
-// TILE = 128 or 64 columns of either operand; waves as 2 x 2.  GR = 2: two such groups of waves in a block take the steps in turn and add their sums in LDS at the end -- for
-// about as many tiles as CUs, where splits over blocks would write, re-read and add several copies of dw to keep two waves on every SIMD.
-template <typename T, bool A8, int TILE, int GR>
-__global__ __launch_bounds__(256 * GR, TILE == 128 ? 2 : 4 / GR) void linear_wgrad_kernel(WgradArgsL p) {
+// TILE = 128 or 64 columns of either operand; waves as 2 x 2.  (Measured and not kept: two such groups of waves in one block that add their sums in LDS, instead of splits: 55 us for
+// 2048 x 2048 -> 512 in fp32, the splits and their reduction 48 + 8.)
+template <typename T, bool A8, int TILE>
+__global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_wgrad_kernel(WgradArgsL p) {
   constexpr int VE = Vec16<T>::N, Q = TILE / 32;
   constexpr int KP = sizeof(T) == 2 ? 32 : TILE == 128 ? 16 : 32;  // rows per step
   constexpr int CH = TILE / VE;                     // 16-byte chunks of a tile row
@@ -424,9 +424,8 @@ __global__ __launch_bounds__(256 * GR, TILE == 128 ? 2 : 4 / GR) void linear_wgr
   constexpr int NCH = KP * CH / 256;                // chunks per thread and operand
   static_assert(NCH >= 1, "a chunk for every thread");
   // two stages: a step's operands are written while the other stage is still being read, one barrier per step
-  constexpr int GROUP = 4 * KP * STRIDE;
-  __shared__ __attribute__((aligned(16))) char smem[GR * GROUP];
-  const int tid = threadIdx.x & 255, grp = GR == 1 ? 0 : threadIdx.x >> 8, wave = tid >> 6, lane = tid & 63;
+  __shared__ __attribute__((aligned(16))) char smem[4 * KP * STRIDE];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int li = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
   unsigned logical = xcd_order(blockIdx.x, gridDim.x);
   const int k0 = (int)(logical % p.k_tiles) * TILE; logical /= p.k_tiles;
@@ -466,10 +465,10 @@ __global__ __launch_bounds__(256 * GR, TILE == 128 ? 2 : 4 / GR) void linear_wgr
   for (int mi = 0; mi < Q; ++mi)
 #pragma unroll
     for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  load(r0 + grp * KP);
+  load(r0);
   int stage = 0;
-  for (long long r = r0; r < r1; r += KP * GR) {  // (rows past r1 are zeros: the groups take as many turns)
-    char* td = smem + grp * GROUP + stage * (2 * KP * STRIDE);
+  for (long long r = r0; r < r1; r += KP) {
+    char* td = smem + stage * (2 * KP * STRIDE);
     char* tx = td + KP * STRIDE;
     stage ^= 1;
 #pragma unroll
@@ -480,7 +479,7 @@ __global__ __launch_bounds__(256 * GR, TILE == 128 ? 2 : 4 / GR) void linear_wgr
       *reinterpret_cast<uint4*>(tx + at) = rx[i];
     }
     __syncthreads();
-    if (r + KP * GR < r1) load(r + KP * GR + grp * KP);
+    if (r + KP < r1) load(r + KP);
     if constexpr (sizeof(T) == 2) {
       uint4 fd[Q], fx[Q];
 #pragma unroll
@@ -506,27 +505,6 @@ __global__ __launch_bounds__(256 * GR, TILE == 128 ? 2 : 4 / GR) void linear_wgr
           for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x4f32(fd[mi], fx[ni], acc[mi][ni], 0, 0, 0);
       }
     }
-  }
-  if constexpr (GR == 2) {
-    static_assert(GR * GROUP >= TILE * TILE * 4, "the second group's sums fit");
-    float* sums = reinterpret_cast<float*>(smem);
-    __syncthreads();
-    if (grp == 1) {
-#pragma unroll
-      for (int mi = 0; mi < Q; ++mi)
-#pragma unroll
-        for (int ni = 0; ni < Q; ++ni)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sums[((mi * Q + ni) * 4 + r) * 256 + tid] = acc[mi][ni][r];
-    }
-    __syncthreads();
-    if (grp == 1) return;
-#pragma unroll
-    for (int mi = 0; mi < Q; ++mi)
-#pragma unroll
-      for (int ni = 0; ni < Q; ++ni)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[mi][ni][r] += sums[((mi * Q + ni) * 4 + r) * 256 + tid];
   }
   // lane: rows n = n0 + wm 64 + 16 mi + 4 g + r, column k = k0 + wn 64 + 16 ni + li
   float* out = p.part + (long long)split * p.N * p.K;
@@ -566,9 +544,17 @@ static int linear_bad(const char* what, int64_t rows, int in, int out, int dtype
   return 0;
 }
 
+// The tile whose rounds over the 256 CUs cost least.  A k-step (128 bytes) of a bm x bn tile brings bm + bn rows into LDS, at about 15 bytes per clock and CU, and multiplies at 4096
+// (fp32: 256) flops per clock, whichever takes longer, and pays its barrier: 5001 x 1000 -> 333 in 16 bits is all operand traffic (64 x 64: 2 rounds of 128 rows, 15 us; 128 x 64:
+// one of 192), 2048 x 512 -> 2048 in fp32 all arithmetic.
 template <bool BT> static int dma_launch(LinearArgs p, int dtype, hipStream_t s, const char* what) {
-  auto count = [&](int bm, int bn) { return (int64_t)ceil_div(p.M, bm) * ceil_div(p.N, bn); };
-  const int bm = count(128, 64) >= 512 ? 128 : 64, bn = count(128, 128) >= 512 && p.N > 64 ? 128 : 64;
+  auto cost = [&](int64_t bm, int64_t bn) {
+    const int64_t rounds = ((int64_t)ceil_div(p.M, (int)bm) * ceil_div(p.N, (int)bn) + 255) / 256;
+    const int64_t fetch = (bm + bn) * 128 / 15, mul = bm * bn * (dtype == SH_F32 ? 64 : 128) / (dtype == SH_F32 ? 256 : 4096);
+    return rounds * ((fetch > mul ? fetch : mul) + 300);
+  };
+  const int64_t c64 = cost(64, 64), c96 = cost(128, 64), c128 = cost(128, 128);
+  const int bm = c96 < c64 || c128 < c64 ? 128 : 64, bn = bm == 128 && c128 <= c96 ? 128 : 64;
   p.n_tiles = (unsigned)ceil_div(p.N, bn);
   const unsigned grid = (unsigned)ceil_div(p.M, bm) * p.n_tiles;
 #define SH_DMA(T)                                                                  \
@@ -634,15 +620,10 @@ static void act_bwd_plan(int64_t rows, int cols, int dtype, int* gx, int* gy, in
   if (*gy < 1) *gy = 1;
 }
 
-// Tile and splits over the rows: two groups of waves per 64-wide tile where there are about as many tiles as CUs (no splits: tile code 65); else 128-wide tiles while they are
-// enough for two blocks per CU with at most 8 splits (every split writes and re-reads its own dw), else 64-wide ones (four blocks per CU).
+// Tile and splits over the rows: 128-wide tiles while they are enough for two blocks per CU with at most 8 splits (every split writes and re-reads its own dw), else 64-wide
+// ones (four blocks per CU).
 static int linear_wgrad_plan(int64_t rows, int in, int out, int dtype, int* splits, int64_t* per) {
   const int64_t t128 = (int64_t)ceil_div(in, 128) * ceil_div(out, 128), t64 = (int64_t)ceil_div(in, 64) * ceil_div(out, 64);
-  if (t64 >= 192 && t64 <= 256 && rows >= 256 && rows <= 16384) {
-    *splits = 1;
-    *per = rows;
-    return 65;
-  }
   const int tile = t128 * 8 >= 512 || rows > 65536 ? 128 : 64, blocks = tile == 128 ? 512 : 1024;
   const int kp = dtype == SH_F32 && tile == 128 ? 16 : 32;
   const int64_t tiles = tile == 128 ? t128 : t64;
@@ -774,16 +755,15 @@ int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, 
   int tile = 256;
   if (wide) linear_wgrad256_plan(rows, in_dim, out_dim, &splits, &per);
   else tile = linear_wgrad_plan(rows, in_dim, out_dim, dtype, &splits, &per);
-  WgradArgsL p = {dz, x, x_codes, x_exps, splits > 1 ? (float*)workspace : dw, rows, per, out_dim, in_dim, (unsigned)ceil_div(out_dim, tile & ~1),
-                  (unsigned)ceil_div(in_dim, tile & ~1)};
+  WgradArgsL p = {dz, x, x_codes, x_exps, splits > 1 ? (float*)workspace : dw, rows, per, out_dim, in_dim, (unsigned)ceil_div(out_dim, tile),
+                  (unsigned)ceil_div(in_dim, tile)};
   if (wide) {
     if (linear_wgrad256_launch(p, splits, s)) return 1;
   } else {
     const unsigned grid = p.n_tiles * p.k_tiles * (unsigned)splits;
-#define SH_WGRAD(T, A8)                                                               \
-  if (tile == 128) linear_wgrad_kernel<T, A8, 128, 1><<<grid, 256, 0, s>>>(p);        \
-  else if (tile == 65) linear_wgrad_kernel<T, A8, 64, 2><<<grid, 512, 0, s>>>(p);     \
-  else linear_wgrad_kernel<T, A8, 64, 1><<<grid, 256, 0, s>>>(p)
+#define SH_WGRAD(T, A8)                                                          \
+  if (tile == 128) linear_wgrad_kernel<T, A8, 128><<<grid, 256, 0, s>>>(p);      \
+  else linear_wgrad_kernel<T, A8, 64><<<grid, 256, 0, s>>>(p)
     if (dtype == SH_F32) {
       if (a8) { SH_WGRAD(float, true); }
       else { SH_WGRAD(float, false); }
