@@ -600,7 +600,7 @@ int simhand_augment_batch_ex(const uint8_t* images, const float* joints, const f
  * activation checkpoints, forward and backward.  All tensors are dense rows ([rows][cols], cols contiguous) in `dtype` = SH_F32 or SH_BF16 (the
  * build's 16-bit type) unless a parameter says fp32; rows >= 0 and cols >= 1 are arbitrary (no multiple, element alignment suffices); sums,
  * statistics and products accumulate in fp32, column sums over rows are folded in a fixed order (bit-reproducible).  Nothing is written beside the
- * outputs and the workspace.  The reference has no such operators (its head is Linear -> BatchNorm1d -> ReLU -> Linear,
+ * outputs and the workspace (a 16-byte address; a query of 0: NULL will do).  The reference has no such operators (its head is Linear -> BatchNorm1d -> ReLU -> Linear,
  * src/models/unsupervised/simclr_model.py:22-39): parity is held against the formulas in 64 bits.
  * =========================================================================== */
 enum sh_act { SH_ACT_NONE = 0, SH_ACT_RELU = 1, SH_ACT_GELU = 2 /* z Phi(z), by the error function */, SH_ACT_SILU = 3 /* z sigma(z) */ };
@@ -618,8 +618,9 @@ int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes
 
 /* z = x w^T + bias, y = act(z) + residual; x [rows][in_dim], w [out_dim][in_dim], bias fp32 [out_dim] or NULL, residual [rows][out_dim] or NULL,
  * pre [rows][out_dim] or NULL receives z (what simhand_linear_act_bwd takes).  residual may be y's own buffer. */
+size_t simhand_linear_fwd_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype);
 int simhand_linear_fwd(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, void* pre, int64_t rows, int in_dim,
-                       int out_dim, int dtype, sh_stream_t stream);
+                       int out_dim, int dtype, void* workspace, size_t workspace_bytes, sh_stream_t stream);
 /* dz = dy act'(pre), db [cols] fp32 = sum_rows dz (before dz is rounded).  SH_ACT_NONE: pre and dz may be NULL (dz = dy; only db is computed).  dz may be dy's buffer. */
 size_t simhand_linear_act_bwd_workspace_bytes(int64_t rows, int cols, int dtype);
 int simhand_linear_act_bwd(const void* dy, const void* pre, int act, void* dz, float* db, int64_t rows, int cols, int dtype, void* workspace,
@@ -628,8 +629,7 @@ int simhand_linear_act_bwd(const void* dy, const void* pre, int act, void* dz, f
 size_t simhand_linear_dgrad_workspace_bytes(int in_dim, int out_dim, int dtype);
 int simhand_linear_dgrad(const void* dz, const void* w, void* dx, int64_t rows, int in_dim, int out_dim, int dtype, void* workspace,
                          size_t workspace_bytes, sh_stream_t stream);
-/* dw [out_dim][in_dim] fp32 = dz^T x; x as it is, or (x = NULL) as its 8-bit checkpoint, whose values enter the product rounded to dtype.
- * A workspace query of 0: NULL will do. */
+/* dw [out_dim][in_dim] fp32 = dz^T x; x as it is, or (x = NULL) as its 8-bit checkpoint, whose values enter the product rounded to dtype */
 size_t simhand_linear_wgrad_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype);
 int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, float* dw, int64_t rows, int in_dim,
                          int out_dim, int dtype, void* workspace, size_t workspace_bytes, sh_stream_t stream);

@@ -78,9 +78,10 @@ struct WgradArgsL {
 // 256 x 256 tiles, 16-bit operands (linear256.hip, linear_wgrad256.hip)
 bool linear256_takes(const LinearArgs& p, int dtype);
 int linear256_launch(const LinearArgs& p, hipStream_t s, const char* what);
-// rows in registers, K <= 512 (linear_rows.hip)
+// rows in registers, K <= 1024 (linear_rows.hip)
 bool linear_rows_takes(const LinearArgs& p, int dtype);
-int linear_rows_launch(const LinearArgs& p, hipStream_t s, const char* what);
+size_t linear_rows_workspace_bytes(const LinearArgs& p);
+int linear_rows_launch(const LinearArgs& p, bool b_padded, void* workspace, hipStream_t s, const char* what);
 bool linear_wgrad256_takes(const void* dz, const void* x, const uint8_t* codes, const uint8_t* exps, int64_t rows, int in_dim, int out_dim, int dtype);
 void linear_wgrad256_plan(int64_t rows, int in_dim, int out_dim, int* splits, int64_t* per);
 int linear_wgrad256_launch(const WgradArgsL& p, int splits, hipStream_t s);

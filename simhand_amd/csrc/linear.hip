@@ -39,10 +39,19 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_gemm_kernel(L
   uint4 ra[Q], rb[Q];
   auto load = [&](int k0) {
     const int k = k0 + sc * VE;
+    if (p.K >= VE) {
+      const int at = kchunk_at<T>(k, p.K);
 #pragma unroll
-    for (int i = 0; i < Q; ++i) {
-      ra[i] = ld_kchunk<T>(pa[i], k, p.K);
-      rb[i] = ld_kchunk<T>(pb[i], k, p.K);
+      for (int i = 0; i < Q; ++i) {
+        ra[i] = ld16_any(pa[i] + at);
+        rb[i] = ld16_any(pb[i] + at);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        ra[i] = ld_kchunk<T>(pa[i], k, p.K);
+        rb[i] = ld_kchunk<T>(pb[i], k, p.K);
+      }
     }
   };
   auto key_b = [](int row) { return ((row >> 1) & 1) | (((row >> 3) & 3) << 1); };
@@ -54,6 +63,14 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_gemm_kernel(L
   load(0);
   for (int k0 = 0; k0 < p.K; k0 += KE) {
     __syncthreads();
+    if (k0 + KE > p.K && p.K >= VE) {
+      const int gone = kchunk_gone<T>(k0 + sc * VE, p.K);
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        ra[i] = drop_first<T>(ra[i], gone);
+        rb[i] = drop_first<T>(rb[i], gone);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
       const int row = sr + 32 * i;
@@ -398,35 +415,25 @@ __global__ __launch_bounds__(256) void linear_act_bwd_kernel(const T* __restrict
 }
 
 // ---- dw = dz^T x ---------------------------------------------------------------------------------------------------------------
-// 16-bit operand of 32 rows x 16 columns read transposed: lane gets rows {4g..4g+3, 16+4g..16+4g+3} of column cb + (lane & 15)
-__device__ __forceinline__ uint4 frag_tr16(const char* tile, int stride, int cb, int lane) {
-  typedef s16x4_t __attribute__((address_space(3))) * lds_ptr;
-  const int p = lane & 15, g = lane >> 4;
-  const char* a0 = tile + (4 * g + (p >> 2)) * stride + (cb + (p & 3) * 4) * 2;
-  const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(a0));
-  const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(a0 + 16 * stride));
-  uint4 r;
-  r.x = (unsigned)(unsigned short)lo[0] | ((unsigned)(unsigned short)lo[1] << 16);
-  r.y = (unsigned)(unsigned short)lo[2] | ((unsigned)(unsigned short)lo[3] << 16);
-  r.z = (unsigned)(unsigned short)hi[0] | ((unsigned)(unsigned short)hi[1] << 16);
-  r.w = (unsigned)(unsigned short)hi[2] | ((unsigned)(unsigned short)hi[3] << 16);
-  return r;
-}
+// A tile of TILE columns of either operand by KP rows a step, staged global -> registers -> LDS, so any alignment will do: 16-byte loads at element addresses, PF steps ahead (the ragged
+// columns behind a row are the next row's -- read, multiplied and never stored; only the tensor's very last chunk goes element by element).  256: 8 waves as 2 x 4 of 128 x 64, for wide
+// layers whose rows are no whole chunks (the LDS-DMA kernel takes the others); 128, 64: 4 waves as 2 x 2.
+template <int TILE> struct WgradWaves { static constexpr int M = 2, N = TILE == 256 ? 4 : 2, THREADS = 64 * M * N; };
 
-// TILE = 128 or 64 columns of either operand; waves as 2 x 2.  (Measured and not kept: two such groups of waves in one block that add their sums in LDS, instead of splits: 55 us for
-// 2048 x 2048 -> 512 in fp32, the splits and their reduction 48 + 8.)
 template <typename T, bool A8, int TILE>
-__global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_wgrad_kernel(WgradArgsL p) {
-  constexpr int VE = Vec16<T>::N, Q = TILE / 32;
-  constexpr int KP = sizeof(T) == 2 ? 32 : TILE == 128 ? 16 : 32;  // rows per step
-  constexpr int CH = TILE / VE;                     // 16-byte chunks of a tile row
-  constexpr int STRIDE = TILE * sizeof(T) + (sizeof(T) == 2 ? 32 : 64);  // padded: the rows a transpose read / a group of lanes touches fall on different banks
-  constexpr int NCH = KP * CH / 256;                // chunks per thread and operand
-  static_assert(NCH >= 1, "a chunk for every thread");
-  // two stages: a step's operands are written while the other stage is still being read, one barrier per step
-  __shared__ __attribute__((aligned(16))) char smem[4 * KP * STRIDE];
+__global__ __launch_bounds__(WgradWaves<TILE>::THREADS, TILE == 256 ? 1 : TILE == 128 ? 2 : 4) void linear_wgrad_kernel(WgradArgsL p) {
+  constexpr bool H = sizeof(T) == 2;
+  constexpr int VE = Vec16<T>::N, NT = WgradWaves<TILE>::THREADS;
+  constexpr int QM = TILE / 16 / WgradWaves<TILE>::M, QN = TILE / 16 / WgradWaves<TILE>::N;  // MFMA tiles of a wave
+  constexpr int KP = H ? 32 : TILE == 64 ? 32 : 16;     // rows per step
+  constexpr int CH = TILE / VE, NCH = KP * CH / NT;     // 16-byte chunks of a tile row; per thread and operand
+  constexpr int PF = TILE == 256 || (TILE == 64 && sizeof(T) == 4) ? 2 : 3;  // (3 would not fit the registers of those two)
+  static_assert(KP * CH % NT == 0, "a whole number of chunks for every thread");
+  // 16 bits: sub-tiles of [KP rows][64 columns] whose 32-byte column groups are rotated by row / 2 (as the LDS-DMA kernel's); fp32: rows padded by 64 bytes
+  constexpr int STRIDE = H ? TILE * 2 : TILE * 4 + 64, OPERAND = KP * STRIDE;
+  __shared__ __attribute__((aligned(16))) char smem[4 * OPERAND];  // two stages, one barrier per step
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int li = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
+  const int li = lane & 15, g = lane >> 4, wm = wave / WgradWaves<TILE>::N, wn = wave % WgradWaves<TILE>::N;
   unsigned logical = xcd_order(blockIdx.x, gridDim.x);
   const int k0 = (int)(logical % p.k_tiles) * TILE; logical /= p.k_tiles;
   const int n0 = (int)(logical % p.n_tiles) * TILE;
@@ -434,101 +441,189 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_wgrad_kernel(
   const long long r0 = (long long)split * p.per_split;
   const long long r1 = r0 + p.per_split < p.M ? r0 + p.per_split : p.M;
   const int eb = (p.K + kAct8Block - 1) / kAct8Block;
-  uint4 rd[NCH], rx[NCH];
-  auto load = [&](long long r) {
+  const long long end_z = p.M * p.N, end_x = p.M * p.K;
+  uint4 rd[PF][NCH], rx[A8 ? 1 : PF][NCH];
+  unsigned rc[A8 ? PF : 1][NCH][VE / 4], re[A8 ? PF : 1][NCH];
+  auto load = [&](long long r, auto set) __attribute__((always_inline)) {
+    constexpr int S = decltype(set)::value;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int q = tid + 256 * i;
+      const int q = tid + NT * i, col = (q % CH) * VE;
       const long long row = r + q / CH;
-      const int col = (q % CH) * VE;
       const int ln = p.N - (n0 + col), lk = p.K - (k0 + col);
-      rd[i] = (row < r1 && ln > 0) ? ld_chunk<T>((const T*)p.dz + row * p.N + n0 + col, ln) : make_uint4(0u, 0u, 0u, 0u);
+      rd[S][i] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < r1 && ln > 0) {
+        const long long at = row * p.N + n0 + col;
+        rd[S][i] = at + VE <= end_z ? ld16_any((const T*)p.dz + at) : ld_chunk<T>((const T*)p.dz + at, ln);
+      }
       if constexpr (A8) {
-        float v[VE];
 #pragma unroll
-        for (int e = 0; e < VE; ++e) v[e] = 0.f;
+        for (int j = 0; j < VE / 4; ++j) rc[S][i][j] = 0u;
+        re[S][i] = 0u;
         if (row < r1 && lk > 0) {
-          unsigned w[VE / 4];
-          act8_ld_codes<VE>(p.codes + row * p.K + k0 + col, lk, w);
-          const float sc = act8_scale(p.exps[row * eb + (k0 + col) / kAct8Block]);
-#pragma unroll
-          for (int j = 0; j < VE / 4; ++j) act8_decode4(w[j], sc, v + 4 * j);
+          const long long at = row * p.K + k0 + col;
+          act8_ld_codes<VE>(p.codes + at, at + VE <= end_x ? VE : lk, rc[S][i]);
+          re[S][i] = p.exps[row * eb + (k0 + col) / kAct8Block];
         }
-        rx[i] = pack16<T>(v);
       } else {
-        rx[i] = (row < r1 && lk > 0) ? ld_chunk<T>((const T*)p.x + row * p.K + k0 + col, lk) : make_uint4(0u, 0u, 0u, 0u);
+        rx[S][i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < r1 && lk > 0) {
+          const long long at = row * p.K + k0 + col;
+          rx[S][i] = at + VE <= end_x ? ld16_any((const T*)p.x + at) : ld_chunk<T>((const T*)p.x + at, lk);
+        }
       }
     }
   };
-  f32x4 acc[Q][Q];
-#pragma unroll
-  for (int mi = 0; mi < Q; ++mi)
-#pragma unroll
-    for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  load(r0);
-  int stage = 0;
-  for (long long r = r0; r < r1; r += KP) {
-    char* td = smem + stage * (2 * KP * STRIDE);
-    char* tx = td + KP * STRIDE;
-    stage ^= 1;
+  auto place = [](int q) __attribute__((always_inline)) -> int {  // LDS offset of chunk q of an operand's tile
+    const int row = q / CH, c = q % CH;
+    if constexpr (H) return (c >> 3) * (KP * 128) + row * 128 + ((((c >> 1) & 3) + (row >> 1)) & 3) * 32 + (c & 1) * 16;
+    else return row * STRIDE + c * 16;
+  };
+  auto put = [&](char* stage, auto set) __attribute__((always_inline)) {
+    constexpr int S = decltype(set)::value;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int q = tid + 256 * i;
-      const int at = (q / CH) * STRIDE + (q % CH) * 16;
-      *reinterpret_cast<uint4*>(td + at) = rd[i];
-      *reinterpret_cast<uint4*>(tx + at) = rx[i];
+      const int at = place(tid + NT * i);
+      *reinterpret_cast<uint4*>(stage + at) = rd[S][i];
+      uint4 v;
+      if constexpr (A8 && H) {
+        v = act8_decode8_h16(rc[S][i][0], rc[S][i][1], act8_scale(re[S][i]));
+      } else if constexpr (A8) {
+        float f[4];
+        act8_decode4(rc[S][i][0], act8_scale(re[S][i]), f);
+        v = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+      } else {
+        v = rx[S][i];
+      }
+      *reinterpret_cast<uint4*>(stage + OPERAND + at) = v;
     }
-    __syncthreads();
-    if (r + KP < r1) load(r + KP);
-    if constexpr (sizeof(T) == 2) {
-      uint4 fd[Q], fx[Q];
+  };
+  f32x4 acc[QM][QN];
 #pragma unroll
-      for (int mi = 0; mi < Q; ++mi) fd[mi] = frag_tr16(td, STRIDE, wm * 16 * Q + mi * 16, lane);
+  for (int mi = 0; mi < QM; ++mi)
 #pragma unroll
-      for (int ni = 0; ni < Q; ++ni) fx[ni] = frag_tr16(tx, STRIDE, wn * 16 * Q + ni * 16, lane);
+    for (int ni = 0; ni < QN; ++ni) acc[mi][ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  // 16 bits: a transposed read hands lane li rows {4g .. 4g+3, 16+4g ..} of column 16 c16 + li
+  const int frow = 4 * g + (li >> 2), fbase = frow * 128 + (li & 3) * 8, frot = frow >> 1;
+  auto frag = [&](const char* operand, int c16) __attribute__((always_inline)) -> uint4 {
+    typedef s16x4_t __attribute__((address_space(3))) * lds_ptr;
+    const char* at = operand + (c16 >> 2) * (KP * 128) + fbase + (((c16 & 3) + frot) & 3) * 32;
+    const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at)));
+    const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 16 * 128)));
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+  };
+  auto multiply = [&](const char* td, const char* tx) __attribute__((always_inline)) {
+    if constexpr (H) {
+      uint4 fx[QN];
 #pragma unroll
-      for (int mi = 0; mi < Q; ++mi)
+      for (int ni = 0; ni < QN; ++ni) fx[ni] = frag(tx, wn * QN + ni);
 #pragma unroll
-        for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = mma16<T>(fd[mi], fx[ni], acc[mi][ni]);
+      for (int mi = 0; mi < QM; ++mi) {
+        const uint4 fd = frag(td, wm * QM + mi);
+#pragma unroll
+        for (int ni = 0; ni < QN; ++ni) acc[mi][ni] = mma16<T>(fd, fx[ni], acc[mi][ni]);
+      }
     } else {
 #pragma unroll
       for (int s4 = 0; s4 < KP / 4; ++s4) {
-        float fd[Q], fx[Q];
+        float fd[QM], fx[QN];
 #pragma unroll
-        for (int mi = 0; mi < Q; ++mi) {
-          fd[mi] = *reinterpret_cast<const float*>(td + (s4 * 4 + g) * STRIDE + (wm * 16 * Q + mi * 16 + li) * 4);
-          fx[mi] = *reinterpret_cast<const float*>(tx + (s4 * 4 + g) * STRIDE + (wn * 16 * Q + mi * 16 + li) * 4);
-        }
+        for (int mi = 0; mi < QM; ++mi) fd[mi] = *reinterpret_cast<const float*>(td + (s4 * 4 + g) * STRIDE + ((wm * QM + mi) * 16 + li) * 4);
 #pragma unroll
-        for (int mi = 0; mi < Q; ++mi)
+        for (int ni = 0; ni < QN; ++ni) fx[ni] = *reinterpret_cast<const float*>(tx + (s4 * 4 + g) * STRIDE + ((wn * QN + ni) * 16 + li) * 4);
 #pragma unroll
-          for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x4f32(fd[mi], fx[ni], acc[mi][ni], 0, 0, 0);
+        for (int mi = 0; mi < QM; ++mi)
+#pragma unroll
+          for (int ni = 0; ni < QN; ++ni) acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x4f32(fd[mi], fx[ni], acc[mi][ni], 0, 0, 0);
       }
     }
+  };
+  int stage = 0;
+  auto step = [&](long long r, auto set) __attribute__((always_inline)) {
+    char* at = smem + stage * (2 * OPERAND);
+    stage ^= 1;
+    put(at, set);
+    __syncthreads();
+    load(r + PF * KP, set);
+    multiply(at, at + OPERAND);
+  };
+  load(r0, std::integral_constant<int, 0>());
+  load(r0 + KP, std::integral_constant<int, 1>());
+  if constexpr (PF == 3) load(r0 + 2 * KP, std::integral_constant<int, PF - 1>());
+  for (long long r = r0; r < r1; r += PF * KP) {
+    step(r, std::integral_constant<int, 0>());
+    if (r + KP < r1) step(r + KP, std::integral_constant<int, 1>());
+    if constexpr (PF == 3) {
+      if (r + 2 * KP < r1) step(r + 2 * KP, std::integral_constant<int, PF - 1>());
+    }
   }
-  // lane: rows n = n0 + wm 64 + 16 mi + 4 g + r, column k = k0 + wn 64 + 16 ni + li
+  // lane: rows n = n0 + 16 (wm QM + mi) + 4 g + r, column k = k0 + 16 (wn QN + ni) + li
   float* out = p.part + (long long)split * p.N * p.K;
 #pragma unroll
-  for (int mi = 0; mi < Q; ++mi)
+  for (int mi = 0; mi < QM; ++mi)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int n = n0 + wm * 16 * Q + mi * 16 + 4 * g + r;
+      const int n = n0 + (wm * QM + mi) * 16 + 4 * g + r;
       if (n >= p.N) continue;
 #pragma unroll
-      for (int ni = 0; ni < Q; ++ni) {
-        const int k = k0 + wn * 16 * Q + ni * 16 + li;
+      for (int ni = 0; ni < QN; ++ni) {
+        const int k = k0 + (wn * QN + ni) * 16 + li;
         if (k < p.K) out[(long long)n * p.K + k] = acc[mi][ni][r];
       }
     }
 }
 
-// the splits' partial sums in a fixed order
-__global__ __launch_bounds__(256) void linear_wgrad_reduce_kernel(const float* __restrict__ part, long long count, int splits, float* __restrict__ dw) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= count) return;
-  float a = 0.f;
-  for (int s = 0; s < splits; ++s) a += part[(long long)s * count + i];
-  dw[i] = a;
+// dw from the splits' partial sums, in a fixed order: GROUPS groups of 64 16-byte columns a block take the splits in turn, 4 loads in flight a thread, and are joined in LDS.  One group
+// for few splits, 16 for many (one thread a value walking 512 splits of 64 x 64 took 100 us; 16 groups for the 4 splits of 2048 x 2048 left twelve of them idle: 38 us, not 16).
+template <int GROUPS>
+__global__ __launch_bounds__(64 * GROUPS) void linear_wgrad_reduce_kernel(const float* __restrict__ part, long long count, int splits, float* __restrict__ dw) {
+  __shared__ float4 red[GROUPS][64];
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const long long i = ((long long)blockIdx.x * 64 + tx) * 4;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  const bool whole = i + 4 <= count && (count & 3) == 0;
+  if (whole) {
+    int s = ty;
+    for (; s + 3 * GROUPS < splits; s += 4 * GROUPS) {
+      float4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const float4*>(part + (long long)(s + GROUPS * u) * count + i);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) { a.x += v[u].x; a.y += v[u].y; a.z += v[u].z; a.w += v[u].w; }
+    }
+    for (; s < splits; s += GROUPS) {
+      const float4 v = *reinterpret_cast<const float4*>(part + (long long)s * count + i);
+      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+    }
+  } else if (i < count) {  // dw of an odd number of values: its rows of partial sums start at any element
+    const int left = count - i < 4 ? (int)(count - i) : 4;
+    for (int s = ty; s < splits; s += GROUPS) {
+      float v[4];
+      ld_f32<4>(part + (long long)s * count + i, left, v);
+      a.x += v[0]; a.y += v[1]; a.z += v[2]; a.w += v[3];
+    }
+  }
+  if constexpr (GROUPS > 1) {
+    red[ty][tx] = a;
+    __syncthreads();
+    for (int o = GROUPS / 2; o > 0; o >>= 1) {
+      if (ty < o) {
+        const float4 v = red[ty + o][tx];
+        float4 w = red[ty][tx];
+        w.x += v.x; w.y += v.y; w.z += v.z; w.w += v.w;
+        red[ty][tx] = w;
+      }
+      __syncthreads();
+    }
+    if (ty > 0) return;
+    a = red[0][tx];
+  }
+  if (whole) {
+    *reinterpret_cast<float4*>(dw + i) = a;
+  } else {
+    const float w[4] = {a.x, a.y, a.z, a.w};
+    for (int e = 0; e < 4 && i + e < count; ++e) dw[i + e] = w[e];
+  }
 }
 
 __global__ __launch_bounds__(256) void rows_zero_kernel(float* p, long long n) {
@@ -569,7 +664,7 @@ template <bool BT> static int dma_launch(LinearArgs p, int dtype, hipStream_t s,
 
 // Which kernel: few rows -> the skinny one (rows <= 64 and so little work that tiles would leave most CUs idle); 64-wide tiles while 128-wide ones would not put two
 // blocks on each of the 256 CUs; else 128-wide ones.
-static int gemm_launch(const LinearArgs& base, int dtype, hipStream_t s, const char* what) {
+static int gemm_launch(const LinearArgs& base, bool b_padded, void* workspace, int dtype, hipStream_t s, const char* what) {
   LinearArgs p = base;
   if (p.M <= 64 && ceil_div(p.N, 64) < 256) {
     const int mt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
@@ -587,7 +682,7 @@ static int gemm_launch(const LinearArgs& base, int dtype, hipStream_t s, const c
 #undef SH_SKINNY
     return check_launch(what);
   }
-  if (linear_rows_takes(p, dtype)) return linear_rows_launch(p, s, what);
+  if (linear_rows_takes(p, dtype)) return linear_rows_launch(p, b_padded, workspace, s, what);
   if (linear256_takes(p, dtype)) return linear256_launch(p, s, what);
   const int ve = dtype == SH_F32 ? 4 : 8;
   if (p.K % ve == 0 && p.ldb % ve == 0 && !(((size_t)p.a | (size_t)p.b) & 15)) return dma_launch<false>(p, dtype, s, what);
@@ -620,13 +715,14 @@ static void act_bwd_plan(int64_t rows, int cols, int dtype, int* gx, int* gy, in
   if (*gy < 1) *gy = 1;
 }
 
-// Tile and splits over the rows: 128-wide tiles while they are enough for two blocks per CU with at most 8 splits (every split writes and re-reads its own dw), else 64-wide
-// ones (four blocks per CU).
+// Tile and splits over the rows (every split writes and re-reads its own dw).  16 bits, both sides wide, many rows: 256-wide tiles, one block per CU; else 128-wide ones while they are
+// enough for two blocks per CU with at most 8 splits, or where the rows are many and a side is wider than 64; else 64-wide ones, four blocks per CU.
 static int linear_wgrad_plan(int64_t rows, int in, int out, int dtype, int* splits, int64_t* per) {
-  const int64_t t128 = (int64_t)ceil_div(in, 128) * ceil_div(out, 128), t64 = (int64_t)ceil_div(in, 64) * ceil_div(out, 64);
-  const int tile = t128 * 8 >= 512 || rows > 65536 ? 128 : 64, blocks = tile == 128 ? 512 : 1024;
+  const int64_t t128 = (int64_t)ceil_div(in, 128) * ceil_div(out, 128);
+  const int tile = dtype != SH_F32 && in > 128 && out > 128 && rows >= 4096 ? 256 : t128 * 8 >= 512 || (rows > 16384 && (in > 64 || out > 64)) ? 128 : 64;
+  const int blocks = tile == 256 ? 256 : tile == 128 ? 512 : 1024;
   const int kp = dtype == SH_F32 && tile == 128 ? 16 : 32;
-  const int64_t tiles = tile == 128 ? t128 : t64;
+  const int64_t tiles = (int64_t)ceil_div(in, tile) * ceil_div(out, tile);
   const int64_t steps = rows > 0 ? (rows + kp - 1) / kp : 1;
   int64_t sk = blocks / tiles;
   if (sk > (steps + 7) / 8) sk = (steps + 7) / 8;  // at least 8 steps each
@@ -643,17 +739,26 @@ using namespace sh;
 
 extern "C" {
 
+size_t simhand_linear_fwd_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype) {
+  if (rows < 1 || in_dim < 1 || out_dim < 1 || dtype != SH_BF16) return 0;
+  // the padded copy of w, if the call turns out to need it (rows that are no whole 16-byte chunks, by length or by address)
+  LinearArgs p = {(const void*)2, nullptr, nullptr, nullptr, nullptr, nullptr, rows, out_dim, in_dim, in_dim, SH_ACT_NONE, 0};
+  return linear_rows_takes(p, dtype) ? linear_rows_workspace_bytes(p) : 0;
+}
+
 int simhand_linear_fwd(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, void* pre, int64_t rows, int in_dim,
-                       int out_dim, int dtype, sh_stream_t stream) {
+                       int out_dim, int dtype, void* workspace, size_t workspace_bytes, sh_stream_t stream) {
   if (linear_bad("linear_fwd", rows, in_dim, out_dim, dtype)) return 1;
   SH_REQUIRE(act >= SH_ACT_NONE && act <= SH_ACT_SILU, "linear_fwd: act %d", act);
   if (rows == 0) return 0;
   SH_REQUIRE(x && w && y, "linear_fwd: NULL argument");
+  const size_t need = simhand_linear_fwd_workspace_bytes(rows, in_dim, out_dim, dtype);
+  SH_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && !((size_t)workspace & 15)), "linear_fwd: workspace too small or not at a 16-byte address");
   hipStream_t s = (hipStream_t)stream;
   const double eb = dtype == SH_F32 ? 4 : 2;
   ProfScope ps(SH_PROF_MISC, s, 2.0 * rows * in_dim * out_dim, eb * ((double)rows * in_dim + (double)in_dim * out_dim + (double)rows * out_dim));
   LinearArgs p = {x, w, y, pre, bias, residual, rows, out_dim, in_dim, in_dim, act, 0};
-  return gemm_launch(p, dtype, s, "linear_fwd");
+  return gemm_launch(p, false, workspace, dtype, s, "linear_fwd");
 }
 
 size_t simhand_linear_act_bwd_workspace_bytes(int64_t rows, int cols, int dtype) {
@@ -705,6 +810,7 @@ int simhand_linear_dgrad(const void* dz, const void* w, void* dx, int64_t rows, 
   if (rows == 0) return 0;
   SH_REQUIRE(dz && w && dx, "linear_dgrad: NULL argument");
   SH_REQUIRE(workspace && workspace_bytes >= simhand_linear_dgrad_workspace_bytes(in_dim, out_dim, dtype), "linear_dgrad: workspace too small");
+  SH_REQUIRE(!((size_t)workspace & 15), "linear_dgrad: workspace at a 16-byte address");
   hipStream_t s = (hipStream_t)stream;
   const double eb = dtype == SH_F32 ? 4 : 2;
   ProfScope ps(SH_PROF_MISC, s, 2.0 * rows * in_dim * out_dim, eb * ((double)rows * in_dim + (double)in_dim * out_dim + (double)rows * out_dim));
@@ -719,7 +825,7 @@ int simhand_linear_dgrad(const void* dz, const void* w, void* dx, int64_t rows, 
   if (dtype == SH_F32) linear_transpose_kernel<float><<<tg, 256, 0, s>>>((const float*)w, (float*)workspace, out_dim, in_dim, ldt);
   else linear_transpose_kernel<bf16_t><<<tg, 256, 0, s>>>((const bf16_t*)w, (bf16_t*)workspace, out_dim, in_dim, ldt);
   if (check_launch("linear_dgrad")) return 1;
-  return gemm_launch(wide, dtype, s, "linear_dgrad");
+  return gemm_launch(wide, true, nullptr, dtype, s, "linear_dgrad");
 }
 
 size_t simhand_linear_wgrad_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype) {
@@ -740,7 +846,7 @@ int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, 
   SH_REQUIRE(!a8 || (x_exps && !x), "linear_wgrad: pass either x or its codes and exponents");
   SH_REQUIRE(dw && (rows == 0 || (dz && (x || a8))), "linear_wgrad: NULL argument");
   const size_t need = simhand_linear_wgrad_workspace_bytes(rows, in_dim, out_dim, dtype);
-  SH_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "linear_wgrad: workspace too small");
+  SH_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && !((size_t)workspace & 15)), "linear_wgrad: workspace too small or not at a 16-byte address");
   hipStream_t s = (hipStream_t)stream;
   const double eb = dtype == SH_F32 ? 4 : 2;
   ProfScope ps(SH_PROF_MISC, s, 2.0 * rows * in_dim * out_dim, eb * (double)rows * out_dim + (a8 ? 1.03125 : eb) * rows * in_dim + 4.0 * in_dim * out_dim);
@@ -752,7 +858,7 @@ int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, 
   int splits;
   int64_t per;
   const bool wide = linear_wgrad256_takes(dz, x, x_codes, x_exps, rows, in_dim, out_dim, dtype);
-  int tile = 256;
+  int tile = 256;  // (the wide kernel's own)
   if (wide) linear_wgrad256_plan(rows, in_dim, out_dim, &splits, &per);
   else tile = linear_wgrad_plan(rows, in_dim, out_dim, dtype, &splits, &per);
   WgradArgsL p = {dz, x, x_codes, x_exps, splits > 1 ? (float*)workspace : dw, rows, per, out_dim, in_dim, (unsigned)ceil_div(out_dim, tile),
@@ -761,9 +867,13 @@ int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, 
     if (linear_wgrad256_launch(p, splits, s)) return 1;
   } else {
     const unsigned grid = p.n_tiles * p.k_tiles * (unsigned)splits;
-#define SH_WGRAD(T, A8)                                                          \
-  if (tile == 128) linear_wgrad_kernel<T, A8, 128><<<grid, 256, 0, s>>>(p);      \
+#define SH_WGRAD(T, A8)                                                               \
+  if (tile == 128) linear_wgrad_kernel<T, A8, 128><<<grid, 256, 0, s>>>(p);           \
   else linear_wgrad_kernel<T, A8, 64><<<grid, 256, 0, s>>>(p)
+    if (tile == 256) {
+      if (a8) linear_wgrad_kernel<bf16_t, true, 256><<<grid, 512, 0, s>>>(p);
+      else linear_wgrad_kernel<bf16_t, false, 256><<<grid, 512, 0, s>>>(p);
+    } else
     if (dtype == SH_F32) {
       if (a8) { SH_WGRAD(float, true); }
       else { SH_WGRAD(float, false); }
@@ -775,7 +885,9 @@ int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, 
     if (check_launch("linear_wgrad")) return 1;
   }
   if (splits > 1) {
-    linear_wgrad_reduce_kernel<<<(unsigned)((count + 255) / 256), 256, 0, s>>>((const float*)workspace, count, splits, dw);
+    const unsigned blocks = (unsigned)((count + 255) / 256);
+    if (splits <= 16) linear_wgrad_reduce_kernel<1><<<blocks, 64, 0, s>>>((const float*)workspace, count, splits, dw);
+    else linear_wgrad_reduce_kernel<16><<<blocks, 1024, 0, s>>>((const float*)workspace, count, splits, dw);
     return check_launch("linear_wgrad_reduce");
   }
   return 0;

@@ -1,10 +1,12 @@
-// out [M][N] = a [M][K] b[N][K]^T of 16-bit operands for many rows and a short K (at most 512): the rows stay in registers.
+// out [M][N] = a [M][K] b[N][ldb]^T of 16-bit operands for many rows and a short K (at most 1024): the rows stay in registers.
 //
 // What bounds the 256 x 256 kernel at these sizes is the path from L2 into the CUs (8 TB/s over the chip, about 15 bytes per clock and CU): every tile fetches both its operands, 1.6 GB
 // for 100352 x 512 -> 2048, on top of what the epilogue moves.  Here a wave holds 32 rows of a for the WHOLE of K as MFMA operands (128 registers at K = 512), eight waves 256 rows,
 // and only b streams through LDS -- half the traffic.  The work is a list of units (256 rows x 64 columns), dealt out evenly over the CUs in contiguous ranges; b's steps (64 columns x
 // 128 of K, 16 KB, four stages, fetched three steps ahead by LDS-DMA) form one sequence across the units, and the residual's tile of the next unit arrives by LDS-DMA as well, so
 // nothing in the loop waits for memory but the counted waits below; the stores drain behind them.
+// Above K = 512 a wave holds 16 rows (RM = 1), a block 128.  RAG: rows of a (any K) and of out (any N) at element alignment -- a goes straight to registers, so only b, which is
+// copied into padded rows first, needs whole chunks; the residual is then read in the epilogue, and the waits are not counted past stores that may be missing.
 #include "linear.h"
 
 namespace sh {
@@ -13,11 +15,12 @@ __device__ uint4 g_lrows_zero[8];  // read-only zeros
 
 constexpr int kRowsMaxN = 4096;  // the bias waits in LDS
 
-template <int KS2, bool RES, bool PRE>
+template <int KS2, int RM, bool RES, bool PRE, bool RAG>
 __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsigned units, unsigned per_cu) {
   typedef bf16_t T;
-  constexpr int S = 4, D = 3, W_BYTES = 16384, R_BYTES = 32768, R0 = S * W_BYTES, BIAS0 = R0 + (RES ? 2 * R_BYTES : 0);
-  constexpr int E_R = RES ? 4 : 0, E_ST = PRE ? 8 : 4;  // vector-memory operations of a unit: residual DMAs, stores of whole rows
+  constexpr int S = 4, D = 3, W_BYTES = 16384, R_BYTES = 16384 * RM, R0 = S * W_BYTES, BIAS0 = R0 + (RES && !RAG ? 2 * R_BYTES : 0);
+  constexpr int ROWS = 128 * RM;  // of a block
+  constexpr int E_R = RES && !RAG ? 2 * RM : 0, E_ST = (PRE ? 4 : 2) * RM;  // vector-memory operations of a unit: residual DMAs, stores of whole rows
   __shared__ __attribute__((aligned(16))) char smem[BIAS0 + kRowsMaxN * 4];
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
   auto dma16 = [](const void* src, unsigned lds_addr) __attribute__((always_inline)) {
@@ -28,9 +31,9 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
   const unsigned cu = xcd_order(blockIdx.x, gridDim.x);
   const unsigned u0 = cu * per_cu, u1 = u0 + per_cu < units ? u0 + per_cu : units;
   if (u0 >= u1) return;
-  const unsigned nt = p.n_tiles;  // units per row tile (N / 64)
+  const unsigned nt = p.n_tiles;  // units per row tile
   float* bias = reinterpret_cast<float*>(smem + BIAS0);
-  for (int n = tid; n < p.N; n += 512) bias[n] = p.bias != nullptr ? p.bias[n] : 0.f;
+  for (int n = tid; n < (int)nt * 64; n += 512) bias[n] = p.bias != nullptr && n < p.N ? p.bias[n] : 0.f;
   __syncthreads();
 
   // b: a wave's two DMA instructions of a step fill rows 8 wave .. + 7 (columns of out) of the step's two 64-k halves; slot s of a row holds chunk s ^ key(row)
@@ -39,36 +42,40 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
   const char* zero = reinterpret_cast<const char*>(g_lrows_zero) + slot * 16;
   unsigned wu = u0, wn_ = u0 % nt, w_stage = 0;  // walker over b's steps: unit, its column tile, stage, k
   int wk = 0;
-  const char* wrow = reinterpret_cast<const char*>((const T*)p.b + (long long)(wn_ * 64 + brow) * p.ldb + bk);
+  auto b_row = [&](unsigned tile) __attribute__((always_inline)) {
+    const int n = (int)tile * 64 + brow;
+    return reinterpret_cast<const char*>((const T*)p.b + (long long)(!RAG || n < p.N ? n : p.N - 1) * p.ldb + bk);
+  };
+  const char* wrow = b_row(wn_);
   auto dma_w = [&]() __attribute__((always_inline)) {
     const unsigned dst = lds0 + w_stage * W_BYTES + wave * 1024;
-    dma16(wu < u1 && wk + bk < p.K ? wrow + wk * 2 : zero, dst);
-    dma16(wu < u1 && wk + 64 + bk < p.K ? wrow + wk * 2 + 128 : zero, dst + 8192);
+    dma16(wu < u1 && wk + bk < p.ldb ? wrow + wk * 2 : zero, dst);
+    dma16(wu < u1 && wk + 64 + bk < p.ldb ? wrow + wk * 2 + 128 : zero, dst + 8192);
     w_stage = (w_stage + 1) & (S - 1);
     wk += 128;
     if (wk >= KS2 * 128) {
       wk = 0;
       ++wu;
       wn_ = wn_ + 1 == nt ? 0 : wn_ + 1;
-      wrow = reinterpret_cast<const char*>((const T*)p.b + (long long)(wn_ * 64 + brow) * p.ldb + bk);
+      wrow = b_row(wn_);
     }
   };
   // the residual's tile of unit u: each wave fetches its own 32 rows (8 an instruction); slot s of a row holds chunk s ^ (row & 7)
   auto dma_r = [&](unsigned u) __attribute__((always_inline)) {
     const unsigned uu = u < u1 ? u : u1 - 1;
-    const long long m0 = (long long)(uu / nt) * 256 + wave * 32 + (lane >> 3);
+    const long long m0 = (long long)(uu / nt) * ROWS + wave * (16 * RM) + (lane >> 3);
     const long long col = (long long)(uu % nt) * 64 + (slot ^ (lane >> 3)) * 8;
-    const unsigned dst = lds0 + R0 + (u & 1) * R_BYTES + wave * 4096;
+    const unsigned dst = lds0 + R0 + (u & 1) * R_BYTES + wave * (2048 * RM);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2 * RM; ++i) {
       const long long m = m0 + 8 * i < p.M ? m0 + 8 * i : p.M - 1;
       // read once: past the caches where K is long (100352 x 512 -> 2048: 263 -> 251 us; 383 -> 389 at K = 256)
-      if constexpr (KS2 >= 3) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(dst + i * 1024), "v"((const T*)p.residual + m * p.N + col));
+      if constexpr (KS2 >= 3 && RM == 2) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(dst + i * 1024), "v"((const T*)p.residual + m * p.N + col));
       else dma16((const T*)p.residual + m * p.N + col, dst + i * 1024);
     }
   };
 
-  if constexpr (RES) dma_r(u0);
+  if constexpr (RES && !RAG) dma_r(u0);
 #pragma unroll
   for (int i = 0; i < D; ++i) dma_w();
   const int rowb = lin_col(0, li);
@@ -83,14 +90,14 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * (D - 1)) : "memory");
   read_b(0, 0, fb[0]);
   unsigned stage = 0, m_have = 0xffffffffu;
-  uint4 a[2][KS2 * 2][2];
+  uint4 a[RM][KS2 * 2][2];
   for (unsigned u = u0; u < u1; ++u) {
     const unsigned mt = u / nt;
-    const long long mrow = (long long)mt * 256 + wave * 32 + li;
+    const long long mrow = (long long)mt * ROWS + wave * (16 * RM) + li;
     if (mt != m_have) {  // (its loads' wait drains the DMA queue: once per 256 rows)
       m_have = mt;
 #pragma unroll
-      for (int mi = 0; mi < 2; ++mi) {
+      for (int mi = 0; mi < RM; ++mi) {
         const long long m = mrow + 16 * mi < p.M ? mrow + 16 * mi : p.M - 1;
         const T* row = (const T*)p.a + m * p.K;
 #pragma unroll
@@ -98,15 +105,27 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) {
             const int k = ks * 64 + kk * 32 + g * 8;
-            a[mi][ks][kk] = k < p.K ? ld16_any(row + k) : make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (!RAG) {
+              a[mi][ks][kk] = k < p.K ? ld16_any(row + k) : make_uint4(0u, 0u, 0u, 0u);
+            } else {  // the ragged last chunk: the row's last 8 elements, moved into place below -- no branch between the loads
+              a[mi][ks][kk] = ld16_any(row + (k + 8 <= p.K ? k : p.K - 8));
+            }
           }
       }
-    }
-    const bool full = (long long)mt * 256 + wave * 32 + 32 <= p.M;
-    const bool steady = full && u >= u0 + 2;  // the two units before this one made all their stores
-    f32x4 acc[2][4];
+      if constexpr (RAG) {
 #pragma unroll
-    for (int mi = 0; mi < 2; ++mi)
+        for (int mi = 0; mi < RM; ++mi)
+#pragma unroll
+          for (int ks = KS2 * 2 - 2; ks < KS2 * 2; ++ks)
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) a[mi][ks][kk] = move_down<T>(a[mi][ks][kk], ks * 64 + kk * 32 + g * 8 + 8 - p.K);
+      }
+    }
+    const bool full = !RAG && (long long)mt * ROWS + (wave + 1) * (16 * RM) <= p.M;
+    const bool steady = full && u >= u0 + 2;  // the two units before this one made all their stores
+    f32x4 acc[RM][4];
+#pragma unroll
+    for (int mi = 0; mi < RM; ++mi)
 #pragma unroll
       for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -129,20 +148,22 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
             else asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
           }
           dma_w();
-          if (RES && j == 0) dma_r(u + 1);
+          if constexpr (RES && !RAG) {
+            if (j == 0) dma_r(u + 1);
+          }
         }
         if (ph < 3) read_b(stage, ph + 1, fb[(ph + 1) & 1]);
         else read_b((stage + 1) & (S - 1), 0, fb[0]);
 #pragma unroll
-        for (int mi = 0; mi < 2; ++mi)
+        for (int mi = 0; mi < RM; ++mi)
 #pragma unroll
           for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = sh_mfma16(fb[ph & 1][ni], a[mi][2 * j + (ph >> 1)][ph & 1], acc[mi][ni]);
       }
       stage = (stage + 1) & (S - 1);
     }
-    // ---- the unit's 32 x 64 values of this wave: lane = row mrow + 16 mi, columns n + 32 h (8 each)
+    // ---- the unit's 16 RM x 64 values of this wave: lane = row mrow + 16 mi, columns n + 32 h (8 each)
     asm volatile("" ::: "memory");
-    if constexpr (RES) {
+    if constexpr (RES && !RAG) {
       // behind this unit's residual (fetched at the start of the unit before): 2 KS2 - 1 steps of b, the next residual, the last unit's stores
       if (steady) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (2 * KS2 - 1) + E_R + E_ST) : "memory");
       else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * KS2 - 2) : "memory");
@@ -154,10 +175,12 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
     auto finish = [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        const int left = RAG ? p.N - (n + 32 * h) : 8;
+        if (RAG && left <= 0) continue;
         float b8[8];
-        ld_f32<8>(bias + n + 32 * h, 8, b8);
+        ld_f32<8>(bias + n + 32 * h, 8, b8);  // (the bias's place in LDS is padded with zeros)
 #pragma unroll
-        for (int mi = 0; mi < 2; ++mi) {
+        for (int mi = 0; mi < RM; ++mi) {
           float z[8];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -166,20 +189,29 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
           }
           const bool in = mrow + 16 * mi < p.M;
           const long long at = at0 + 16 * mi * row_bytes + 64 * h;
-          if (PRE && in) st16_any((char*)p.pre + at, pack16<T>(z));
+          if (PRE && in) {
+            if constexpr (RAG) st_chunk<T>((T*)((char*)p.pre + at), left, pack16<T>(z));
+            else st16_any((char*)p.pre + at, pack16<T>(z));
+          }
 #pragma unroll
           for (int e = 0; e < 8; ++e) z[e] = act_value(z[e], decltype(act)::value);
           if constexpr (RES) {
             float r8[8];
-            const uint4 q = *reinterpret_cast<const uint4*>(smem + R0 + (u & 1) * R_BYTES + wave * 4096 + (16 * mi + li) * 128 + (((h * 4 + g) ^ (li & 7)) * 16));
+            uint4 q = make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (!RAG) q = *reinterpret_cast<const uint4*>(smem + R0 + (u & 1) * R_BYTES + wave * (2048 * RM) + (16 * mi + li) * 128 + (((h * 4 + g) ^ (li & 7)) * 16));
+            else if (in) q = ld_chunk<T>((const T*)((const char*)p.residual + at), left);
             unpack16<T>(q, r8);
 #pragma unroll
             for (int e = 0; e < 8; ++e) z[e] += r8[e];
           }
           if (!in) continue;
           // without a residual the stores go past the caches (401408 x 256 -> 1024: 285 -> 272 us); with one that costs a fifth (383 -> 469)
-          if (RES || !aligned) st16_any((char*)p.out + at, pack16<T>(z));
-          else st16<true>((char*)p.out + at, pack16<T>(z));
+          if constexpr (RAG) {
+            st_chunk<T>((T*)((char*)p.out + at), left, pack16<T>(z));
+          } else {
+            if (RES || !aligned) st16_any((char*)p.out + at, pack16<T>(z));
+            else st16<true>((char*)p.out + at, pack16<T>(z));
+          }
         }
       }
     };
@@ -192,25 +224,60 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the DMAs past the end have landed before the LDS is given back
 }
 
-// Whole 64-column units, K in registers, 16-byte chunks at 16-byte addresses, at least four units a CU; and where it pays: with a residual (100352 x 512 -> 2048: 263 us, the
-// 256 x 256 kernel 325; 1605632 x 128 -> 512: 732 and 826), without one from K = 256 on (401408 x 256 -> 1024: 286 and 319; but 1605632 x 128 -> 512: 452 and 435).
-bool linear_rows_takes(const LinearArgs& p, int dtype) {
-  if (dtype != SH_BF16 || p.K % 8 || p.K > 512 || p.N % 64 || p.N > kRowsMaxN || p.ldb % 8) return false;
-  if (p.residual == nullptr && p.K < 256) return false;
-  if (((size_t)p.a | (size_t)p.b | (size_t)p.residual) & 15) return false;
-  return (int64_t)ceil_div(p.M, 256) * (p.N / 64) >= 1024;
+// K in registers, at least four units a CU; and where it pays.  Whole chunks and 64-column units: with a residual (100352 x 512 -> 2048: 260 us, the 256 x 256 kernel 325; 1605632 x 128
+// -> 512: 732 and 826), without one for K of 256 to 512 (401408 x 256 -> 1024: 272 and 319; but 1605632 x 128 -> 512: 452 and 435).  Anything else: the other kernels stage its ragged
+// rows through registers for every tile.
+static bool rows_whole(const LinearArgs& p) {
+  return p.K % 8 == 0 && p.N % 64 == 0 && p.ldb % 8 == 0 && !(((size_t)p.a | (size_t)p.b | (size_t)p.residual) & 15);
 }
-int linear_rows_launch(const LinearArgs& base, hipStream_t s, const char* what) {
+static int rows_block(const LinearArgs& p) { return p.K <= 512 ? 256 : 128; }
+bool linear_rows_takes(const LinearArgs& p, int dtype) {
+  if (dtype != SH_BF16 || p.K > 1024 || p.N > kRowsMaxN || p.K < 32 || (int64_t)ceil_div(p.M, rows_block(p)) * ceil_div(p.N, 64) < 1024) return false;
+  if (rows_whole(p)) return p.K <= 512 && (p.residual != nullptr || p.K >= 256);
+  return p.K % 8 != 0 || (((size_t)p.a) & 15) != 0;  // (ragged columns alone: the LDS-DMA tiles take them)
+}
+size_t linear_rows_workspace_bytes(const LinearArgs& p) { return rows_whole(p) ? 0 : (size_t)p.N * ((p.K + 7) / 8 * 8) * 2; }
+
+// b [N][ldb] -> rows of kp elements, zeros behind K
+__global__ __launch_bounds__(256) void linear_pad_kernel(const bf16_t* __restrict__ b, bf16_t* __restrict__ out, int n, int k, int ldb, int kp) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int row = (int)(i / (kp / 8)), c = (int)(i % (kp / 8)) * 8;
+  if (row < n) *reinterpret_cast<uint4*>(out + (long long)row * kp + c) = ld_chunk<bf16_t>(b + (long long)row * ldb + c, k - c);
+}
+
+// workspace: linear_rows_workspace_bytes() (unless b's rows are already padded with zeros to a multiple of 8 at 16-byte addresses: b_padded)
+int linear_rows_launch(const LinearArgs& base, bool b_padded, void* workspace, hipStream_t s, const char* what) {
   LinearArgs p = base;
-  p.n_tiles = (unsigned)(p.N / 64);
-  const unsigned units = (unsigned)ceil_div(p.M, 256) * p.n_tiles, per_cu = (units + 255) / 256;
-#define SH_ROWS(KS2, RES, PRE) linear_rows_kernel<KS2, RES, PRE><<<256, 512, 0, s>>>(p, units, per_cu)
+  const bool rag = !rows_whole(base);
+  if (rag && !b_padded) {
+    const int kp = (p.K + 7) / 8 * 8;
+    linear_pad_kernel<<<(unsigned)(((int64_t)p.N * (kp / 8) + 255) / 256), 256, 0, s>>>((const bf16_t*)p.b, (bf16_t*)workspace, p.N, p.K, p.ldb, kp);
+    if (check_launch(what)) return 1;
+    p.b = workspace;
+    p.ldb = kp;
+  }
+  p.n_tiles = (unsigned)ceil_div(p.N, 64);
+  const unsigned units = (unsigned)ceil_div(p.M, rows_block(p)) * p.n_tiles, per_cu = (units + 255) / 256;
+#define SH_ROWS(KS2, RM, RES, PRE, RAG) linear_rows_kernel<KS2, RM, RES, PRE, RAG><<<256, 512, 0, s>>>(p, units, per_cu)
 #define SH_ROWS_K(RES, PRE)                                                                      \
-  switch ((p.K + 127) / 128) {                                                                   \
-    case 1: SH_ROWS(1, RES, PRE); break;                                                         \
-    case 2: SH_ROWS(2, RES, PRE); break;                                                         \
-    case 3: SH_ROWS(3, RES, PRE); break;                                                         \
-    default: SH_ROWS(4, RES, PRE); break;                                                        \
+  if (rag) {                                                                                     \
+    switch ((p.K + 127) / 128) {                                                                 \
+      case 1: SH_ROWS(1, 2, RES, PRE, true); break;                                              \
+      case 2: SH_ROWS(2, 2, RES, PRE, true); break;                                              \
+      case 3: SH_ROWS(3, 2, RES, PRE, true); break;                                              \
+      case 4: SH_ROWS(4, 2, RES, PRE, true); break;                                              \
+      case 5: SH_ROWS(5, 1, RES, PRE, true); break;                                              \
+      case 6: SH_ROWS(6, 1, RES, PRE, true); break;                                              \
+      case 7: SH_ROWS(7, 1, RES, PRE, true); break;                                              \
+      default: SH_ROWS(8, 1, RES, PRE, true); break;                                             \
+    }                                                                                            \
+  } else {                                                                                       \
+    switch ((p.K + 127) / 128) {                                                                 \
+      case 1: SH_ROWS(1, 2, RES, PRE, false); break;                                             \
+      case 2: SH_ROWS(2, 2, RES, PRE, false); break;                                             \
+      case 3: SH_ROWS(3, 2, RES, PRE, false); break;                                             \
+      default: SH_ROWS(4, 2, RES, PRE, false); break;                                            \
+    }                                                                                            \
   }
   if (p.residual != nullptr) {
     if (p.pre != nullptr) { SH_ROWS_K(true, true) }

@@ -72,9 +72,26 @@ template <typename T> __device__ __forceinline__ uint4 drop_first(const uint4& v
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+// v's elements moved down by `gone` places, zeros behind them (16-bit elements; gone <= 0: v, gone >= 8: zeros)
+template <typename T> __device__ __forceinline__ uint4 move_down(const uint4& v, int gone) {
+  unsigned w[4] = {v.x, v.y, v.z, v.w};
+  if (gone >= 8) return make_uint4(0u, 0u, 0u, 0u);
+  if (gone > 0) {
+    if (gone & 4) { w[0] = w[2]; w[1] = w[3]; w[2] = 0u; w[3] = 0u; }
+    if (gone & 2) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = 0u; }
+    if (gone & 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = w[i] >> 16 | (i < 3 ? w[i + 1] << 16 : 0u);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 // One chunk of a reduction row (the product's K): `k` its first element, `len` the row's length.  The ragged last chunk of a row is read as the row's last N elements with
 // those that the chunk before it holds zeroed -- both operands of a product are read like this, so element e of either is the same k, and no element is
 // loaded by itself.  Rows shorter than a chunk go element by element.
+// In two steps, so that a loop can have the next step's loads in flight: kchunk_at is where to read (no branch), kchunk_gone how much of it to drop.
+template <typename T> __device__ __forceinline__ int kchunk_at(int k, int len) { return k + Vec16<T>::N <= len ? k : len - Vec16<T>::N; }
+template <typename T> __device__ __forceinline__ int kchunk_gone(int k, int len) { return k + Vec16<T>::N <= len ? 0 : k - (len - Vec16<T>::N); }
 template <typename T> __device__ __forceinline__ uint4 ld_kchunk(const T* row, int k, int len) {
   constexpr int N = Vec16<T>::N;
   if (k + N <= len) return ld16_any(row + k);

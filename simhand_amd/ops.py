@@ -318,7 +318,11 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     pr = _like(residual, x, shape, x.dtype, "linear_fwd (residual)")
     y = torch.empty(shape, dtype=x.dtype, device=x.device)
     pre = torch.empty_like(y) if want_pre else None
-    check(lib.simhand_linear_fwd(px, pw, pb, a, pr, y.data_ptr(), pre.data_ptr() if want_pre else 0, rows, cin, cout, dt(x.dtype), _row_stream(x)), "linear_fwd")
+    d = dt(x.dtype)
+    nb = lib.simhand_linear_fwd_workspace_bytes(rows, cin, cout, d)
+    ws = _scratch(nb, x) if nb else None
+    check(lib.simhand_linear_fwd(px, pw, pb, a, pr, y.data_ptr(), pre.data_ptr() if want_pre else 0, rows, cin, cout, d, ws.data_ptr() if nb else 0, nb, _row_stream(x)),
+          "linear_fwd")
     return (y, pre) if want_pre else y
 
 

@@ -192,7 +192,8 @@ def test_linear_forward(dtype, m, k, n, act, bias, residual, pre):
 # the kernel for many rows (16 bits, rows of 16-byte chunks, at least 192 tiles of 256 x 256): whole tiles, ragged rows / columns / K, one to five k-steps, the smallest N, several
 # tiles per block
 SHAPES_MANY = [(49152, 64, 256), (49100, 72, 136), (24600, 128, 520), (6200, 320, 2048), (30011, 8, 384), (131072 + 40, 200, 128), (16640, 136, 1032),
-               (16384, 512, 1024), (16389, 384, 1024), (33000, 256, 576), (70001, 120, 320), (66000, 72, 256), (9000, 504, 2048), (524288 + 3, 64, 64)]
+               (16384, 512, 1024), (16389, 384, 1024), (33000, 256, 576), (70001, 120, 320), (66000, 72, 256), (9000, 504, 2048), (524288 + 3, 64, 64),
+               (40001, 77, 333), (33333, 333, 520), (20003, 777, 333), (66001, 130, 128), (16400, 1001, 500), (131073, 45, 130), (30000, 513, 300)]
 
 
 @pytest.mark.parametrize("m,k,n", SHAPES_MANY)
@@ -254,7 +255,8 @@ def test_linear_backward(dtype, m, k, n, act8):
 
 # the kernels for many rows (weight gradient: at least 4096 rows and 192 columns on both sides; input gradient: 192 tiles): whole and ragged tiles, rows that end inside a step,
 # one and several tiles, ranges of rows that leave some blocks with less
-@pytest.mark.parametrize("m,k,n", [(4096, 256, 256), (49152, 256, 256), (49157, 200, 328), (8195, 512, 200), (6001, 384, 1024), (20000, 1024, 264), (33333, 640, 192)])
+@pytest.mark.parametrize("m,k,n", [(4096, 256, 256), (49152, 256, 256), (49157, 200, 328), (8195, 512, 200), (6001, 384, 1024), (20000, 1024, 264), (33333, 640, 192),
+                                   (20001, 333, 257), (5003, 777, 131), (30000, 64, 64), (40001, 50, 61), (17000, 100, 30), (100001, 129, 7), (4097, 260, 2047)])
 @pytest.mark.parametrize("act8", [False, True])
 def test_linear_backward_many_rows(dtype, m, k, n, act8):
     from simhand_amd import ops
@@ -287,6 +289,24 @@ def test_linear_gradient_against_differences():
             num = (f(x + h * e[0], w + h * e[1], b + h * e[2]) - f(x - h * e[0], w - h * e[1], b - h * e[2])) / (2 * h)
             parts = [(g.double().cpu() * t) for g, t in zip((dx, dw, db), e)]
             assert abs(float(num - sum(p.sum() for p in parts))) < 1e-4 * float(sum(p.abs().sum() for p in parts))
+
+
+def test_linear_many_rows_at_odd_addresses(dtype):
+    """Whole rows whose first element is not at a 16-byte address, and one operand of each kind."""
+    from simhand_amd import ops
+
+    m, k, n = 40000, 128, 192
+    xb, wb = randn(m * k + 5, dtype=dtype).cuda(), randn(n * k + 3, seed=1, dtype=dtype).cuda()
+    for ox, ow in ((5, 0), (0, 3), (1, 1), (0, 0)):
+        x, w = xb[ox:ox + m * k].view(m, k), wb[ow:ow + n * k].view(n, k)
+        y = ops.linear_fwd(x, w)
+        want, mag = x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t()
+        assert bool(((y.double() - want).abs() <= half_step(dtype) * want.abs() + 2.02 * (k + 2) * U * mag + tiny(dtype)).all()), (ox, ow)
+        dz = y[:, :].contiguous()
+        dx, dw = ops.linear_bwd(dz, x, w)
+        zd = dz.double()
+        assert bool(((dx.double() - zd @ w.double()).abs() <= half_step(dtype) * (zd @ w.double()).abs() + 2.02 * (n + 2) * U * (zd.abs() @ w.double().abs()) + tiny(dtype)).all())
+        assert bool(((dw.double() - zd.t() @ x.double()).abs() <= 2 * (m + 40) * U * (zd.abs().t() @ x.double().abs())).all())
 
 
 def test_linear_unaligned_and_inplace_residual(dtype):
@@ -524,7 +544,7 @@ def test_nothing_is_written_beside_the_outputs(dtype):
 
     bufs = []
     y, yv = guarded(m * n, dtype); pre, prev = guarded(m * n, dtype)
-    assert lib.simhand_linear_fwd(p(x), p(w), None, 2, None, p(yv), p(prev), m, k, n, d, st) == 0
+    assert lib.simhand_linear_fwd(p(x), p(w), None, 2, None, p(yv), p(prev), m, k, n, d, None, 0, st) == 0
     dx, dxv = guarded(m * k, dtype)
     ws = torch.empty(lib.simhand_linear_dgrad_workspace_bytes(k, n, d), dtype=torch.uint8, device="cuda")
     assert lib.simhand_linear_dgrad(p(dz), p(w), p(dxv), m, k, n, d, p(ws), ws.numel(), st) == 0

@@ -26,11 +26,12 @@ def test_c_entry_points_refuse_bad_arguments():
     assert refused(lib.simhand_layer_norm_bwd(P, P, N, N, P, P, P, P, 0, P, P, 4, 8, 0, P, 4, N))  # workspace
     assert refused(lib.simhand_layer_norm_bwd(P, P, P, P, P, P, P, P, 0, P, P, 4, 8, 0, P, 1 << 20, N))  # x and codes
     assert refused(lib.simhand_layer_norm_bwd(P, N, P, N, P, P, P, P, 0, P, P, 4, 8, 0, P, 1 << 20, N))  # codes without exponents
-    assert refused(lib.simhand_linear_fwd(P, P, N, 4, N, P, N, 4, 8, 8, 0, N))                     # act
-    assert refused(lib.simhand_linear_fwd(P, P, N, 0, N, P, N, 4, 0, 8, 0, N))                     # in_dim
-    assert refused(lib.simhand_linear_fwd(P, P, N, 0, N, P, N, 4, 8, 0, 0, N))                     # out_dim
-    assert refused(lib.simhand_linear_fwd(P, P, N, 0, N, P, N, 1 << 31, 8, 8, 0, N))               # rows
-    assert refused(lib.simhand_linear_fwd(P, P, N, 0, N, N, N, 4, 8, 8, 0, N))                     # y
+    assert refused(lib.simhand_linear_fwd(P, P, N, 4, N, P, N, 4, 8, 8, 0, P, 1 << 30, N))                     # act
+    assert refused(lib.simhand_linear_fwd(P, P, N, 0, N, P, N, 4, 0, 8, 0, P, 1 << 30, N))                     # in_dim
+    assert refused(lib.simhand_linear_fwd(P, P, N, 0, N, P, N, 4, 8, 0, 0, P, 1 << 30, N))                     # out_dim
+    assert refused(lib.simhand_linear_fwd(P, P, N, 0, N, P, N, 1 << 31, 8, 8, 0, P, 1 << 30, N))               # rows
+    assert refused(lib.simhand_linear_fwd(P, P, N, 0, N, N, N, 4, 8, 8, 0, P, 1 << 30, N))                     # y
+    assert refused(lib.simhand_linear_fwd(P, P, N, 0, N, P, N, 200000, 77, 130, 1, N, 0, N))       # workspace
     assert refused(lib.simhand_linear_act_bwd(P, N, 2, P, P, 4, 8, 0, P, 1 << 20, N))              # gelu without pre
     assert refused(lib.simhand_linear_act_bwd(P, P, 2, P, P, 4, 8, 0, N, 0, N))                    # workspace
     assert refused(lib.simhand_linear_dgrad(P, P, P, 4, 8, 8, 0, P, 8, N))                         # workspace
@@ -45,7 +46,7 @@ def test_c_entry_points_refuse_bad_arguments():
 def test_no_rows_is_no_launch():
     lib = _lib.load()
     assert lib.simhand_layer_norm_fwd(None, P, P, 1e-5, 0, None, None, None, 0, 8, 0, None) == 0
-    assert lib.simhand_linear_fwd(None, P, None, 0, None, None, None, 0, 8, 8, 1, None) == 0
+    assert lib.simhand_linear_fwd(None, P, None, 0, None, None, None, 0, 8, 8, 1, None, 0, None) == 0
     assert lib.simhand_act8_pack(None, None, None, 0, 8, 0, None) == 0
     assert lib.simhand_act8_unpack(None, None, None, 0, 8, 1, None) == 0
 
