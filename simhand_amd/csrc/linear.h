@@ -30,37 +30,57 @@ struct LinearArgs {
 // tile column that row m of MFMA tile ni holds: lane group g of the tiles 2 j, 2 j + 1 ends with columns 32 j + 8 g .. + 7
 __device__ __forceinline__ int lin_col(int ni, int m) { return (ni >> 1) * 32 + (m >> 2) * 8 + (ni & 1) * 4 + (m & 3); }
 
-// the 8 finished sums of one row: z = acc + bias, pre <- z, out <- act(z) + residual
-template <typename T>
-__device__ __forceinline__ void linear_store8(const LinearArgs& p, long long row, int n, const float (&acc)[8]) {
-  constexpr int VE = Vec16<T>::N;
-  const int left = p.N - n;
-  if (left <= 0) return;
-  float z[8];
-  float b[8];
-  if (p.bias != nullptr) ld_f32<8>(p.bias + n, left, b);
+// A wave's finished sums, rows row0 + 16 mi, columns n0 + 32 j .. + 7 of a lane: z = acc + bias, pre <- z, out <- act(z) + residual.  The residual is read for the whole tile before
+// the first value is used (chunk after chunk, each waited for: 300000 x 77 -> 256 fp32 with gelu 333 us, like this 293).
+template <typename T, int QM, int QN>
+__device__ __forceinline__ void linear_store_tile(const LinearArgs& p, long long row0, int n0, const f32x4 (&acc)[QM][QN]) {
+  constexpr int VE = Vec16<T>::N, H = 8 / VE;
+  uint4 res[QM][QN / 2][H];
+  if (p.residual != nullptr) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) z[e] = p.bias != nullptr ? acc[e] + b[e] : acc[e];
-  const long long at = row * p.N + n;
+    for (int mi = 0; mi < QM; ++mi) {
+      const long long row = row0 + 16 * mi < p.M ? row0 + 16 * mi : p.M - 1;
 #pragma unroll
-  for (int h = 0; h < 8 / VE; ++h) {
-    const int l = left - h * VE;
-    if (l <= 0) break;
-    float o[VE];
+      for (int j = 0; j < QN / 2; ++j)
 #pragma unroll
-    for (int e = 0; e < VE; ++e) o[e] = z[h * VE + e];
-    if (p.pre != nullptr) st_chunk<T>((T*)p.pre + at + h * VE, l, pack16<T>(o));
-    if (p.act != SH_ACT_NONE) {
-#pragma unroll
-      for (int e = 0; e < VE; ++e) o[e] = act_value(o[e], p.act);
+        for (int h = 0; h < H; ++h) res[mi][j][h] = ld_tail<T>((const T*)p.residual + row * p.N, n0 + 32 * j + h * VE, p.N);
     }
-    if (p.residual != nullptr) {
-      float r[VE];
-      unpack16<T>(ld_chunk<T>((const T*)p.residual + at + h * VE, l), r);
+  }
 #pragma unroll
-      for (int e = 0; e < VE; ++e) o[e] += r[e];
+  for (int j = 0; j < QN / 2; ++j) {
+    const int n = n0 + 32 * j, left = p.N - n;
+    if (left <= 0) break;
+    float b[8];
+    if (p.bias != nullptr) ld_f32<8>(p.bias + n, left, b);
+#pragma unroll
+    for (int mi = 0; mi < QM; ++mi) {
+      const long long row = row0 + 16 * mi;
+      if (row >= p.M) break;
+      const long long at = row * p.N + n;
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const int l = left - h * VE;
+        if (l <= 0) break;
+        float o[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float z = acc[mi][2 * j + (h * VE + e) / 4][(h * VE + e) & 3];
+          o[e] = p.bias != nullptr ? z + b[h * VE + e] : z;
+        }
+        if (p.pre != nullptr) st_chunk<T>((T*)p.pre + at + h * VE, l, pack16<T>(o));
+        if (p.act != SH_ACT_NONE) {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) o[e] = act_value(o[e], p.act);
+        }
+        if (p.residual != nullptr) {
+          float r[VE];
+          unpack16<T>(tail_of<T>(res[mi][j][h], n + h * VE, p.N), r);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) o[e] += r[e];
+        }
+        st_chunk<T>((T*)p.out + at + h * VE, l, pack16<T>(o));
+      }
     }
-    st_chunk<T>((T*)p.out + at + h * VE, l, pack16<T>(o));
   }
 }
 
@@ -78,7 +98,7 @@ struct WgradArgsL {
 // 256 x 256 tiles, 16-bit operands (linear256.hip, linear_wgrad256.hip)
 bool linear256_takes(const LinearArgs& p, int dtype);
 int linear256_launch(const LinearArgs& p, hipStream_t s, const char* what);
-// rows in registers, K <= 1024 (linear_rows.hip)
+// rows in registers, K <= 512 (linear_rows.hip)
 bool linear_rows_takes(const LinearArgs& p, int dtype);
 size_t linear_rows_workspace_bytes(const LinearArgs& p);
 int linear_rows_launch(const LinearArgs& p, bool b_padded, void* workspace, hipStream_t s, const char* what);

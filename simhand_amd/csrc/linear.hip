@@ -98,21 +98,7 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_gemm_kernel(L
         for (int ni = 0; ni < Q; ++ni) acc[mi][ni] = mma16<T>(fb[ni], fa[mi], acc[mi][ni]);
     }
   }
-#pragma unroll
-  for (int mi = 0; mi < Q; ++mi) {
-    const long long row = m0 + wm * HALF + mi * 16 + li;
-    if (row >= p.M) continue;
-#pragma unroll
-    for (int j = 0; j < Q / 2; ++j) {
-      float v[8];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        v[r] = acc[mi][2 * j][r];
-        v[4 + r] = acc[mi][2 * j + 1][r];
-      }
-      linear_store8<T>(p, row, n0 + wn * HALF + j * 32 + g * 8, v);
-    }
-  }
+  linear_store_tile<T, Q, Q>(p, m0 + wm * HALF + li, n0 + wn * HALF + g * 8, acc);
 }
 
 // The same product with both operands by LDS-DMA, for rows of whole 16-byte chunks: several k-steps ahead, one barrier per step and nothing staged in registers.  Waves as 2 x 2, each
@@ -271,21 +257,7 @@ __global__ __launch_bounds__(256, 2) void linear_dma_kernel(LinearArgs p) {
     }
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the DMAs past the end have landed before the LDS is given back
-#pragma unroll
-  for (int mi = 0; mi < QM; ++mi) {
-    const long long row = m0 + wm * 16 * QM + mi * 16 + li;
-    if (row >= p.M) continue;
-#pragma unroll
-    for (int j = 0; j < QN / 2; ++j) {
-      float v[8];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        v[r] = acc[mi][2 * j][r];
-        v[4 + r] = acc[mi][2 * j + 1][r];
-      }
-      linear_store8<T>(p, row, n0 + wn * 16 * QN + j * 32 + g * 8, v);
-    }
-  }
+  linear_store_tile<T, QM, QN>(p, m0 + wm * 16 * QM + li, n0 + wn * 16 * QN + g * 8, acc);
 }
 
 // Few rows: a block of 8 waves makes 16 columns of up to 16 MT rows; every wave takes each eighth 64-byte piece of K, both operands go from memory straight into MFMA
@@ -742,7 +714,7 @@ extern "C" {
 size_t simhand_linear_fwd_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype) {
   if (rows < 1 || in_dim < 1 || out_dim < 1 || dtype != SH_BF16) return 0;
   // the padded copy of w, if the call turns out to need it (rows that are no whole 16-byte chunks, by length or by address)
-  LinearArgs p = {(const void*)2, nullptr, nullptr, nullptr, nullptr, nullptr, rows, out_dim, in_dim, in_dim, SH_ACT_NONE, 0};
+  LinearArgs p = {(const void*)2, nullptr, nullptr, nullptr, nullptr, (const void*)2, rows, out_dim, in_dim, in_dim, SH_ACT_NONE, 0};
   return linear_rows_takes(p, dtype) ? linear_rows_workspace_bytes(p) : 0;
 }
 

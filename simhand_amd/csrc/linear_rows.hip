@@ -1,11 +1,11 @@
-// out [M][N] = a [M][K] b[N][ldb]^T of 16-bit operands for many rows and a short K (at most 1024): the rows stay in registers.
+// out [M][N] = a [M][K] b[N][ldb]^T of 16-bit operands for many rows and a short K (at most 512): the rows stay in registers.
 //
 // What bounds the 256 x 256 kernel at these sizes is the path from L2 into the CUs (8 TB/s over the chip, about 15 bytes per clock and CU): every tile fetches both its operands, 1.6 GB
 // for 100352 x 512 -> 2048, on top of what the epilogue moves.  Here a wave holds 32 rows of a for the WHOLE of K as MFMA operands (128 registers at K = 512), eight waves 256 rows,
 // and only b streams through LDS -- half the traffic.  The work is a list of units (256 rows x 64 columns), dealt out evenly over the CUs in contiguous ranges; b's steps (64 columns x
 // 128 of K, 16 KB, four stages, fetched three steps ahead by LDS-DMA) form one sequence across the units, and the residual's tile of the next unit arrives by LDS-DMA as well, so
 // nothing in the loop waits for memory but the counted waits below; the stores drain behind them.
-// Above K = 512 a wave holds 16 rows (RM = 1), a block 128.  RAG: rows of a (any K) and of out (any N) at element alignment -- a goes straight to registers, so only b, which is
+// RAG: rows of a (any K) and of out (any N) at element alignment -- a goes straight to registers, so only b, which is
 // copied into padded rows first, needs whole chunks; the residual is then read in the epilogue, and the waits are not counted past stores that may be missing.
 #include "linear.h"
 
@@ -15,11 +15,10 @@ __device__ uint4 g_lrows_zero[8];  // read-only zeros
 
 constexpr int kRowsMaxN = 4096;  // the bias waits in LDS
 
-template <int KS2, int RM, bool RES, bool PRE, bool RAG>
+template <int KS2, bool RES, bool PRE, bool RAG>
 __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsigned units, unsigned per_cu) {
   typedef bf16_t T;
-  constexpr int S = 4, D = 3, W_BYTES = 16384, R_BYTES = 16384 * RM, R0 = S * W_BYTES, BIAS0 = R0 + (RES && !RAG ? 2 * R_BYTES : 0);
-  constexpr int ROWS = 128 * RM;  // of a block
+  constexpr int S = 4, D = 3, W_BYTES = 16384, RM = 2, ROWS = 128 * RM, R_BYTES = 16384 * RM, R0 = S * W_BYTES, BIAS0 = R0 + (RES && !RAG ? 2 * R_BYTES : 0);
   constexpr int E_R = RES && !RAG ? 2 * RM : 0, E_ST = (PRE ? 4 : 2) * RM;  // vector-memory operations of a unit: residual DMAs, stores of whole rows
   __shared__ __attribute__((aligned(16))) char smem[BIAS0 + kRowsMaxN * 4];
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
@@ -70,7 +69,7 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
     for (int i = 0; i < 2 * RM; ++i) {
       const long long m = m0 + 8 * i < p.M ? m0 + 8 * i : p.M - 1;
       // read once: past the caches where K is long (100352 x 512 -> 2048: 263 -> 251 us; 383 -> 389 at K = 256)
-      if constexpr (KS2 >= 3 && RM == 2) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(dst + i * 1024), "v"((const T*)p.residual + m * p.N + col));
+      if constexpr (KS2 >= 3) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(dst + i * 1024), "v"((const T*)p.residual + m * p.N + col));
       else dma16((const T*)p.residual + m * p.N + col, dst + i * 1024);
     }
   };
@@ -225,16 +224,16 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
 }
 
 // K in registers, at least four units a CU; and where it pays.  Whole chunks and 64-column units: with a residual (100352 x 512 -> 2048: 260 us, the 256 x 256 kernel 325; 1605632 x 128
-// -> 512: 732 and 826), without one for K of 256 to 512 (401408 x 256 -> 1024: 272 and 319; but 1605632 x 128 -> 512: 452 and 435).  Anything else: the other kernels stage its ragged
-// rows through registers for every tile.
+// -> 512: 732 and 826), without one for K of 256 to 512 (401408 x 256 -> 1024: 272 and 319; but 1605632 x 128 -> 512: 452 and 435).  Rows that are no whole chunks, which the other
+// kernel stages through registers once per column tile: with a residual (with gelu, 100000 x 333 -> 777: 218 and 280, 200000 x 129 -> 130: 104 and 117), without one from three units
+// a row tile (300000 x 77 -> 192: 59 and 84, 100000 x 333 -> 777: 124 and 170; but 200000 x 129 -> 130: 85 and 65).
 static bool rows_whole(const LinearArgs& p) {
   return p.K % 8 == 0 && p.N % 64 == 0 && p.ldb % 8 == 0 && !(((size_t)p.a | (size_t)p.b | (size_t)p.residual) & 15);
 }
-static int rows_block(const LinearArgs& p) { return p.K <= 512 ? 256 : 128; }
 bool linear_rows_takes(const LinearArgs& p, int dtype) {
-  if (dtype != SH_BF16 || p.K > 1024 || p.N > kRowsMaxN || p.K < 32 || (int64_t)ceil_div(p.M, rows_block(p)) * ceil_div(p.N, 64) < 1024) return false;
-  if (rows_whole(p)) return p.K <= 512 && (p.residual != nullptr || p.K >= 256);
-  return p.K % 8 != 0 || (((size_t)p.a) & 15) != 0;  // (ragged columns alone: the LDS-DMA tiles take them)
+  if (dtype != SH_BF16 || p.K > 512 || p.N > kRowsMaxN || p.K < 32 || (int64_t)ceil_div(p.M, 256) * ceil_div(p.N, 64) < 1024) return false;
+  if (rows_whole(p)) return p.residual != nullptr || p.K >= 256;
+  return (p.K % 8 != 0 || (((size_t)p.a) & 15) != 0) && (p.residual != nullptr || p.N >= 192);  // (ragged columns alone: the LDS-DMA tiles take them)
 }
 size_t linear_rows_workspace_bytes(const LinearArgs& p) { return rows_whole(p) ? 0 : (size_t)p.N * ((p.K + 7) / 8 * 8) * 2; }
 
@@ -257,26 +256,22 @@ int linear_rows_launch(const LinearArgs& base, bool b_padded, void* workspace, h
     p.ldb = kp;
   }
   p.n_tiles = (unsigned)ceil_div(p.N, 64);
-  const unsigned units = (unsigned)ceil_div(p.M, rows_block(p)) * p.n_tiles, per_cu = (units + 255) / 256;
-#define SH_ROWS(KS2, RM, RES, PRE, RAG) linear_rows_kernel<KS2, RM, RES, PRE, RAG><<<256, 512, 0, s>>>(p, units, per_cu)
+  const unsigned units = (unsigned)ceil_div(p.M, 256) * p.n_tiles, per_cu = (units + 255) / 256;
+#define SH_ROWS(KS2, RES, PRE, RAG) linear_rows_kernel<KS2, RES, PRE, RAG><<<256, 512, 0, s>>>(p, units, per_cu)
 #define SH_ROWS_K(RES, PRE)                                                                      \
   if (rag) {                                                                                     \
     switch ((p.K + 127) / 128) {                                                                 \
-      case 1: SH_ROWS(1, 2, RES, PRE, true); break;                                              \
-      case 2: SH_ROWS(2, 2, RES, PRE, true); break;                                              \
-      case 3: SH_ROWS(3, 2, RES, PRE, true); break;                                              \
-      case 4: SH_ROWS(4, 2, RES, PRE, true); break;                                              \
-      case 5: SH_ROWS(5, 1, RES, PRE, true); break;                                              \
-      case 6: SH_ROWS(6, 1, RES, PRE, true); break;                                              \
-      case 7: SH_ROWS(7, 1, RES, PRE, true); break;                                              \
-      default: SH_ROWS(8, 1, RES, PRE, true); break;                                             \
+      case 1: SH_ROWS(1, RES, PRE, true); break;                                              \
+      case 2: SH_ROWS(2, RES, PRE, true); break;                                              \
+      case 3: SH_ROWS(3, RES, PRE, true); break;                                              \
+      default: SH_ROWS(4, RES, PRE, true); break;                                             \
     }                                                                                            \
   } else {                                                                                       \
     switch ((p.K + 127) / 128) {                                                                 \
-      case 1: SH_ROWS(1, 2, RES, PRE, false); break;                                             \
-      case 2: SH_ROWS(2, 2, RES, PRE, false); break;                                             \
-      case 3: SH_ROWS(3, 2, RES, PRE, false); break;                                             \
-      default: SH_ROWS(4, 2, RES, PRE, false); break;                                            \
+      case 1: SH_ROWS(1, RES, PRE, false); break;                                             \
+      case 2: SH_ROWS(2, RES, PRE, false); break;                                             \
+      case 3: SH_ROWS(3, RES, PRE, false); break;                                             \
+      default: SH_ROWS(4, RES, PRE, false); break;                                            \
     }                                                                                            \
   }
   if (p.residual != nullptr) {

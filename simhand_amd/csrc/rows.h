@@ -72,19 +72,30 @@ template <typename T> __device__ __forceinline__ uint4 drop_first(const uint4& v
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// v's elements moved down by `gone` places, zeros behind them (16-bit elements; gone <= 0: v, gone >= 8: zeros)
+// v's elements moved down by `gone` places, zeros behind them (gone <= 0: v, all of them or more: zeros)
 template <typename T> __device__ __forceinline__ uint4 move_down(const uint4& v, int gone) {
+  constexpr int N = Vec16<T>::N, D = N / 4;  // elements per dword
   unsigned w[4] = {v.x, v.y, v.z, v.w};
-  if (gone >= 8) return make_uint4(0u, 0u, 0u, 0u);
+  if (gone >= N) return make_uint4(0u, 0u, 0u, 0u);
   if (gone > 0) {
-    if (gone & 4) { w[0] = w[2]; w[1] = w[3]; w[2] = 0u; w[3] = 0u; }
-    if (gone & 2) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = 0u; }
-    if (gone & 1) {
+    if (gone & (2 * D)) { w[0] = w[2]; w[1] = w[3]; w[2] = 0u; w[3] = 0u; }
+    if (gone & D) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = 0u; }
+    if (D == 2 && (gone & 1)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = w[i] >> 16 | (i < 3 ? w[i + 1] << 16 : 0u);
     }
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Elements at .. of a row of len, in two steps: the load (without a branch if the row holds a whole chunk: a ragged last one is read as the row's last N elements), and
+// where the values are used tail_of()
+template <typename T> __device__ __forceinline__ uint4 ld_tail(const T* row, int at, int len) {
+  constexpr int N = Vec16<T>::N;
+  if (len < N) return at < len ? ld_chunk<T>(row + at, len - at) : make_uint4(0u, 0u, 0u, 0u);
+  return ld16_any(row + (at + N <= len ? at : len - N));
+}
+template <typename T> __device__ __forceinline__ uint4 tail_of(const uint4& v, int at, int len) {
+  return len < Vec16<T>::N ? v : move_down<T>(v, at + Vec16<T>::N - len);
 }
 // One chunk of a reduction row (the product's K): `k` its first element, `len` the row's length.  The ragged last chunk of a row is read as the row's last N elements with
 // those that the chunk before it holds zeroed -- both operands of a product are read like this, so element e of either is the same k, and no element is
