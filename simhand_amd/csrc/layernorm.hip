@@ -388,12 +388,13 @@ int simhand_layer_norm_fwd(const void* x, const float* gamma, const float* beta,
   SH_REQUIRE(eps >= 0.f, "layer_norm_fwd: eps < 0");
   if (rows == 0) return 0;
   const int nvec = ln_nvec(cols, dtype);
-  const int64_t grid = (rows + ln_rows_per_block(nvec) - 1) / ln_rows_per_block(nvec);
-  SH_REQUIRE(grid < (1ll << 31), "layer_norm_fwd: too many rows");
+  const int rpb = ln_rows_per_block(nvec);
+  const int64_t most = (1ll << 23) * rpb;  // rows of a launch: its threads are counted in 32 bits
   hipStream_t s = (hipStream_t)stream;
   ProfScope ps(SH_PROF_BN, s, 0, 2.0 * rows * cols * (dtype == SH_F32 ? 4 : 2));
   const bool rag = cols % (dtype == SH_F32 ? 4 : 8) != 0;
-#define SH_ONE(T, G, NV, RAG) layer_norm_fwd_kernel<T, G, NV, RAG><<<(unsigned)grid, 256, 0, s>>>((const T*)x, gamma, beta, eps, relu, (T*)y, mean, rstd, rows, cols)
+#define SH_ONE(T, G, NV, RAG) \
+  layer_norm_fwd_kernel<T, G, NV, RAG><<<grid, 256, 0, s>>>((const T*)x + r * cols, gamma, beta, eps, relu, (T*)y + r * cols, mean + r, rstd + r, n, cols)
 #define SH_CALL(G, NV)                       \
   if (dtype == SH_F32) {                     \
     if (rag) SH_ONE(float, G, NV, true);     \
@@ -402,7 +403,11 @@ int simhand_layer_norm_fwd(const void* x, const float* gamma, const float* beta,
     if (rag) SH_ONE(bf16_t, G, NV, true);    \
     else SH_ONE(bf16_t, G, NV, false);       \
   }
-  SH_LN_DISPATCH(SH_CALL)
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = rows - r < most ? rows - r : most;
+    const unsigned grid = (unsigned)((n + rpb - 1) / rpb);
+    SH_LN_DISPATCH(SH_CALL)
+  }
 #undef SH_CALL
 #undef SH_ONE
   return check_launch("layer_norm_fwd");

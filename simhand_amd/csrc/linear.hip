@@ -634,6 +634,21 @@ template <bool BT> static int dma_launch(LinearArgs p, int dtype, hipStream_t s,
   return check_launch(what);
 }
 
+// A launch's threads are counted in 32 bits: more than 2^23 tiles (of 64 x 64) go in several launches, each over a range of whole tiles' rows.
+template <typename F> static int by_row_ranges(const LinearArgs& p, int dtype, F&& launch) {
+  const int64_t tiles = (p.N + 63) / 64, most = ((1ll << 23) / tiles) * 64, eb = dtype == SH_F32 ? 4 : 2;
+  for (int64_t r = 0; r < p.M; r += most) {
+    LinearArgs q = p;
+    q.M = p.M - r < most ? p.M - r : most;
+    q.a = (const char*)p.a + r * p.K * eb;
+    q.out = (char*)p.out + r * p.N * eb;
+    if (p.pre != nullptr) q.pre = (char*)p.pre + r * p.N * eb;
+    if (p.residual != nullptr) q.residual = (const char*)p.residual + r * p.N * eb;
+    if (launch(q)) return 1;
+  }
+  return 0;
+}
+
 // Which kernel: few rows -> the skinny one (rows <= 64 and so little work that tiles would leave most CUs idle); 64-wide tiles while 128-wide ones would not put two
 // blocks on each of the 256 CUs; else 128-wide ones.
 static int gemm_launch(const LinearArgs& base, bool b_padded, void* workspace, int dtype, hipStream_t s, const char* what) {
@@ -730,7 +745,7 @@ int simhand_linear_fwd(const void* x, const void* w, const float* bias, int act,
   const double eb = dtype == SH_F32 ? 4 : 2;
   ProfScope ps(SH_PROF_MISC, s, 2.0 * rows * in_dim * out_dim, eb * ((double)rows * in_dim + (double)in_dim * out_dim + (double)rows * out_dim));
   LinearArgs p = {x, w, y, pre, bias, residual, rows, out_dim, in_dim, in_dim, act, 0};
-  return gemm_launch(p, false, workspace, dtype, s, "linear_fwd");
+  return by_row_ranges(p, dtype, [&](const LinearArgs& q) { return gemm_launch(q, false, workspace, dtype, s, "linear_fwd"); });
 }
 
 size_t simhand_linear_act_bwd_workspace_bytes(int64_t rows, int cols, int dtype) {
@@ -791,13 +806,13 @@ int simhand_linear_dgrad(const void* dz, const void* w, void* dx, int64_t rows, 
   LinearArgs direct = {dz, w, dx, nullptr, nullptr, nullptr, rows, in_dim, out_dim, in_dim, SH_ACT_NONE, 0};
   LinearArgs wide = {dz, workspace, dx, nullptr, nullptr, nullptr, rows, in_dim, out_dim, (out_dim + 7) / 8 * 8, SH_ACT_NONE, 0};
   if (in_dim % ve == 0 && out_dim % ve == 0 && !(((size_t)dz | (size_t)w) & 15) && !linear256_takes(wide, dtype) && !linear_rows_takes(wide, dtype))
-    return dma_launch<true>(direct, dtype, s, "linear_dgrad");
+    return by_row_ranges(direct, dtype, [&](const LinearArgs& q) { return dma_launch<true>(q, dtype, s, "linear_dgrad"); });
   const int ldt = (out_dim + 7) / 8 * 8;
   const dim3 tg(ceil_div(in_dim, 32), ceil_div(ldt, 32));
   if (dtype == SH_F32) linear_transpose_kernel<float><<<tg, 256, 0, s>>>((const float*)w, (float*)workspace, out_dim, in_dim, ldt);
   else linear_transpose_kernel<bf16_t><<<tg, 256, 0, s>>>((const bf16_t*)w, (bf16_t*)workspace, out_dim, in_dim, ldt);
   if (check_launch("linear_dgrad")) return 1;
-  return gemm_launch(wide, true, nullptr, dtype, s, "linear_dgrad");
+  return by_row_ranges(wide, dtype, [&](const LinearArgs& q) { return gemm_launch(q, true, nullptr, dtype, s, "linear_dgrad"); });
 }
 
 size_t simhand_linear_wgrad_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype) {

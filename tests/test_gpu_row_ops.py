@@ -589,3 +589,156 @@ def test_refusals_on_the_device():
         with pytest.raises(E):
             f()
             pytest.fail(f"case {i} was not refused")
+
+
+# ------------------------------------------------------------------ sizes that 32 bits do not count
+def whole_numbers(*shape, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(-2, 3, shape, generator=g, device="cuda", dtype=torch.int8).to(dtype)  # their products sum exactly in fp32
+
+
+def spots(rows, cols):
+    """first, last, and where the element and the byte offset pass 2^31 and 2^32"""
+    return [slice(0, 70)] + [slice(max(0, b // cols - 40), min(rows, b // cols + 40)) for b in (1 << 30, 1 << 31) if b // cols < rows] + [slice(rows - 70, rows)]
+
+
+@pytest.fixture
+def huge():
+    torch.cuda.empty_cache()
+    yield 4300003, 512  # 2.2e9 values
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("cols", [512, 509])
+def test_offsets_past_32_bits_rowwise(dtype, huge, cols):
+    from simhand_amd import ops
+
+    rows = huge[0] * huge[1] // cols if dtype != torch.float32 else (1 << 30) // cols + 9999  # (fp32: past 2^32 bytes)
+    x = torch.empty(rows, cols, dtype=dtype, device="cuda").normal_()
+    dy = torch.empty_like(x).normal_()
+    dy[:-300] = 0  # the column sums are the last rows'
+    gamma, beta = randn(cols, seed=1).cuda(), randn(cols, seed=2).cuda()
+    y, mean, rstd = ops.layer_norm_fwd(x, gamma, beta)
+    dx, dg, db = ops.layer_norm_bwd(dy, x, gamma, beta, mean, rstd)
+    c = ops.act8_pack(x)
+    back = ops.act8_unpack(c)
+    dz, dbias = ops.linear_act_bwd(dy, x, "gelu")
+    for s in spots(rows, cols):
+        ys, ms, rs = ops.layer_norm_fwd(x[s], gamma, beta)
+        assert torch.equal(y[s], ys) and torch.equal(mean[s], ms) and torch.equal(rstd[s], rs), s
+        assert torch.equal(dx[s], ops.layer_norm_bwd(dy[s].contiguous(), x[s].contiguous(), gamma, beta, ms, rs)[0]), s
+        cs = ops.act8_pack(x[s])
+        assert torch.equal(c.codes[s], cs.codes) and torch.equal(c.exps[s], cs.exps) and torch.equal(back[s], ops.act8_unpack(cs)), s
+        assert torch.equal(dz[s], ops.linear_act_bwd(dy[s], x[s], "gelu")[0]), s
+    t = slice(rows - 300, rows)
+    h = (x[t].double() - mean[t, None].double()) * rstd[t, None].double()
+    d = dy[t].double()
+    for got, want, mag in ((dg, (d * h).sum(0), (d * h).abs().sum(0)), (db, d.sum(0), d.abs().sum(0))):
+        assert bool(((got.double() - want).abs() <= 320 * U * mag + U * want.abs()).all())  # (terms off by 4 U each, 300 of them added)
+
+
+@pytest.mark.parametrize("k,n", [(512, 64), (64, 512), (509, 200), (61, 520), (64, 76)])
+def test_offsets_past_32_bits_linear(dtype, huge, k, n):
+    from simhand_amd import ops
+
+    rows = huge[0] * huge[1] // max(k, n) if dtype != torch.float32 else (1 << 30) // max(k, n) + 9999
+    x, w = whole_numbers(rows, k, dtype=dtype), whole_numbers(n, k, dtype=dtype, seed=1)
+    res = whole_numbers(rows, n, dtype=dtype, seed=2)
+    y, yr = ops.linear_fwd(x, w), ops.linear_fwd(x, w, act="relu", residual=res)
+    dx = ops.linear_bwd(res, x[:, :k], w)[0]
+    tail = torch.zeros_like(res)
+    tail[-300:] = res[-300:]
+    dw = ops.linear_wgrad(tail, x)
+    assert torch.equal(dw, tail[-300:].float().t().contiguous() @ x[-300:].float())
+    for s in spots(rows, max(k, n)):
+        z = x[s].float() @ w.float().t().contiguous()
+        assert torch.equal(y[s], z.to(dtype)), s
+        assert torch.equal(yr[s], (z.clamp(min=0) + res[s].float()).to(dtype)), s
+        assert torch.equal(dx[s], (res[s].float() @ w.float()).to(dtype)), s
+
+
+def test_more_threads_than_32_bits_count():
+    """A launch holds fewer than 2^32 threads: calls over more rows go in several."""
+    from simhand_amd import ops
+
+    torch.cuda.empty_cache()
+    b = torch.bfloat16
+    rows, edge = (1 << 26) + 70, 1 << 25
+    x = torch.empty(rows, 129, dtype=b, device="cuda").normal_()
+    gamma, beta = randn(129, seed=1).cuda(), randn(129, seed=2).cuda()
+    y, mean, rstd = ops.layer_norm_fwd(x, gamma, beta)
+    for s in (slice(0, 70), slice(edge - 70, edge + 70), slice(2 * edge - 70, rows)):
+        ys, ms, rs = ops.layer_norm_fwd(x[s], gamma, beta)
+        assert torch.equal(y[s], ys) and torch.equal(mean[s], ms) and torch.equal(rstd[s], rs), s
+    del x, y, mean, rstd
+    torch.cuda.empty_cache()
+    edge = 1 << 29
+    rows = edge + 70
+    for k, n in ((2, 1), (3, 2), (8, 8)):  # the ragged tiles, and the LDS-DMA ones (both directions)
+        x, w = whole_numbers(rows, k, dtype=b), whole_numbers(n, k, dtype=b, seed=1)
+        y = ops.linear_fwd(x, w)
+        dx = ops.linear_bwd(y, x, w)[0] if n > 1 else None
+        for s in (slice(0, 70), slice(edge - 70, rows)):
+            assert torch.equal(y[s], (x[s].float() @ w.float().t().contiguous()).to(b)), (k, n, s)
+            if dx is not None:
+                assert torch.equal(dx[s], (y[s].float() @ w.float()).to(b)), (k, n, s)
+        del x, y, dx
+        torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("m,k,n", [(40000, 333, 777), (70000, 512, 256), (50000, 256, 512)])
+def test_captured_many_rows(dtype, m, k, n):
+    """The kernels for many rows in a graph, replayed with new inputs between eager work on the same operands."""
+    from simhand_amd import ops
+
+    x, w, r = (randn(*s, seed=i, dtype=dtype).cuda() for i, s in enumerate(((m, k), (n, k), (m, n))))
+
+    def calls():
+        y, pre = ops.linear_fwd(x, w, act="gelu", residual=r, want_pre=True)
+        dz, db = ops.linear_act_bwd(y, pre, "gelu")
+        dx, dw = ops.linear_bwd(dz, ops.act8_pack(x), w)
+        return y, pre, dz, db, dx, dw
+
+    calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = calls()
+    for s in range(3):
+        x.copy_(randn(m, k, seed=60 + s, dtype=dtype))
+        eager = calls()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager)), s
+
+
+@pytest.mark.parametrize("m,k,n", [(5, 136, 128), (70, 33, 40), (300, 77, 130), (5001, 1000, 333), (33333, 640, 192), (40001, 333, 777), (66001, 130, 128), (49152, 256, 256),
+                                   (20000, 505, 300), (70000, 512, 256)])
+def test_linear_bad_values_stay_where_they_belong(dtype, m, k, n):
+    """Inf and NaN of one row (column) reach that row (column) of the result and nothing beside it: ragged ends and rows past the end are kept out, not multiplied by zero."""
+    from simhand_amd import ops
+
+    x, w, r = (randn(*s, seed=i, scale=0.1, dtype=dtype).cuda() for i, s in enumerate(((m, k), (n, k), (m, n))))
+    bad = sorted({1, m // 2, m - 1})
+    xb = x.clone()
+    xb[bad, k - 1] = torch.tensor([math.inf, math.nan, -math.inf], device="cuda")[:len(bad)].to(dtype)
+    xb[bad[0], 0] = math.nan
+    for res in (None, r):
+        y, yb = ops.linear_fwd(x, w, residual=res), ops.linear_fwd(xb, w, residual=res)
+        ok = torch.ones(m, dtype=torch.bool, device="cuda")
+        ok[bad] = False
+        assert torch.equal(y[ok], yb[ok]) and not bool(torch.isfinite(yb[~ok]).any())
+    rb = r.clone()
+    rb[bad, n - 1] = math.nan
+    dx, dxb = ops.linear_bwd(r, x, w)[0], ops.linear_bwd(rb, x, w)[0]
+    assert torch.equal(dx[ok], dxb[ok]) and not bool(torch.isfinite(dxb[~ok]).any())
+    for pack in (False, True):
+        keep = ops.act8_pack if pack else (lambda t: t)
+        dw, dwx, dwz = ops.linear_wgrad(r, keep(x)), ops.linear_wgrad(r, keep(xb)), ops.linear_wgrad(rb, keep(x))
+        cols = torch.ones(k, dtype=torch.bool, device="cuda")
+        cols[k - 1] = cols[0] = False
+        if pack:  # (a block's scale is that of its finite values: the neighbours keep their codes unless the bad value was the largest)
+            cols[(k - 1) // 32 * 32:] = False
+            cols[:32] = False
+        assert torch.equal(dw[:, cols], dwx[:, cols]) and not bool(torch.isfinite(dwx[:, k - 1]).any())
+        assert torch.equal(dw[:n - 1], dwz[:n - 1]) and not bool(torch.isfinite(dwz[n - 1]).any())
