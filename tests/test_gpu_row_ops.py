@@ -742,3 +742,33 @@ def test_linear_bad_values_stay_where_they_belong(dtype, m, k, n):
             cols[:32] = False
         assert torch.equal(dw[:, cols], dwx[:, cols]) and not bool(torch.isfinite(dwx[:, k - 1]).any())
         assert torch.equal(dw[:n - 1], dwz[:n - 1]) and not bool(torch.isfinite(dwz[n - 1]).any())
+
+
+@pytest.mark.parametrize("m,k,n", [(40001, 333, 777), (66001, 130, 128), (33333, 640, 192), (20001, 505, 300), (9001, 777, 333), (49157, 200, 328), (70001, 512, 256), (7, 33, 5)])
+def test_nothing_is_written_beside_outputs_and_workspaces(dtype, m, k, n):
+    """As above for the kernels for many rows, with workspaces of exactly the bytes that were asked for."""
+    from simhand_amd import _lib, ops
+
+    lib, d, pad = _lib.load(), ops.dt(dtype), 256
+    st = torch.cuda.current_stream().cuda_stream
+    x, w, dz = randn(m, k, dtype=dtype).cuda(), randn(n, k, seed=1, dtype=dtype).cuda(), randn(m, n, seed=2, dtype=dtype).cuda()
+    c = ops.act8_pack(x)
+    bufs = []
+
+    def guarded(count, t):
+        buf = torch.full((count + 2 * pad,), 7, dtype=t, device="cuda")
+        bufs.append(buf)
+        return buf[pad:pad + count]
+
+    nf = lib.simhand_linear_fwd_workspace_bytes(m, k, n, d)
+    nd, nw = lib.simhand_linear_dgrad_workspace_bytes(k, n, d), lib.simhand_linear_wgrad_workspace_bytes(m, k, n, d)
+    for res in (0, dz.data_ptr()):
+        y, pre, ws = guarded(m * n, dtype), guarded(m * n, dtype), guarded(nf, torch.uint8)
+        assert lib.simhand_linear_fwd(x.data_ptr(), w.data_ptr(), 0, 2, res, y.data_ptr(), pre.data_ptr(), m, k, n, d, ws.data_ptr(), nf, st) == 0
+    dx, ws = guarded(m * k, dtype), guarded(nd, torch.uint8)
+    assert lib.simhand_linear_dgrad(dz.data_ptr(), w.data_ptr(), dx.data_ptr(), m, k, n, d, ws.data_ptr(), nd, st) == 0
+    for px, pc, pe in ((x.data_ptr(), 0, 0), (0, c.codes.data_ptr(), c.exps.data_ptr())):
+        dw, ws = guarded(n * k, torch.float32), guarded(nw, torch.uint8)
+        assert lib.simhand_linear_wgrad(dz.data_ptr(), px, pc, pe, dw.data_ptr(), m, k, n, d, ws.data_ptr(), nw, st) == 0
+    torch.cuda.synchronize()
+    assert all(bool((b[:pad] == 7).all()) and bool((b[-pad:] == 7).all()) for b in bufs)
