@@ -7,6 +7,8 @@
 // One pass over the data each way: a group of G lanes holds a whole row in registers (NV 16-byte vectors per lane), so the variance is summed about
 // the finished mean (no E[x^2] - m^2 cancellation) and nothing is read twice.  Statistics and sums are fp32, the column sums over row blocks are
 // folded in 64 bits in a fixed order (bit-reproducible).  Bound by HBM: 2 (3) elements of traffic per element forward (backward).
+// Measured: forward 100352 x 2048 bf16 154 us (5.3 TB/s; a large copy reaches 4.9), 256 x 512 fp32 3.1 (11 with the call around it); backward 33001 x 777 fp16 from codes 38 + 4 for the
+// fold (2.7 TB/s: a ragged row costs more arithmetic than its bytes take), 2048 x 512 fp32 with ReLU 5.8 + 3.4.
 #include "rows.h"
 
 namespace sh {

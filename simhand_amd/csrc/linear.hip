@@ -4,11 +4,13 @@
 //   (fp32 operands on v_mfma_f32_16x16x4_f32: exact products, no reduced-precision mode), every output is rounded once.
 //   act backward: dz = dy act'(pre), db = sum_rows dz (of the unrounded dz);   dx = dz w;   dw = dz^T x, x possibly as its 8-bit checkpoint.
 //
-// linear_gemm_kernel (forward, and dx with w transposed first): out [M][N] = a [M][K] b[N][K]^T, tiles of 128 x 128, 128 bytes of K a step, both operands
-// global -> registers -> LDS with the next step's loads in flight under the MFMAs.  The operands are swapped (b is the MFMA's first one), and b's rows are permuted inside
+// linear_gemm_kernel (forward, and dx with w transposed first; rows at any element address): out [M][N] = a [M][K] b[N][K]^T, tiles of 128 x 128 or 64 x 64, 128 bytes of K a step, both
+// operands global -> registers -> LDS with the next step's loads in flight under the MFMAs (a second step in flight and a second buffer: no faster).
+// 100000 x 777 -> 333: bf16 138 us, fp32 548 (336 at the fp32 rate of a large matrix product).  The operands are swapped (b is the MFMA's first one), and b's rows are permuted inside
 // the tile, so that a lane ends with 8 consecutive columns of one row: bias, residual, pre-activation and output move as 16-byte vectors.
-// linear_wgrad_kernel: dw [N][K] = dz^T x, the reduction runs over rows: tiles of 128 x 128 over a range of rows (split), 16-bit operands are read transposed from LDS
-// (ds_read_b64_tr_b16); the splits' fp32 partial sums are added in a fixed order by a second launch.
+// linear_wgrad_kernel: dw [N][K] = dz^T x, the reduction runs over rows: tiles of 64, 128 or 256 squared over a range of rows (split), 16-bit operands are read transposed from LDS
+// (ds_read_b64_tr_b16); the splits' fp32 partial sums are added in a fixed order by a second launch.  100000 x 777 -> 333: bf16 149 us, fp32 617; 400000 x 64 -> 64 bf16 29;
+// 2048 x 2048 -> 512 fp32 48 + 8 (28 at that rate).
 #include "linear.h"
 
 namespace sh {
@@ -103,7 +105,8 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_gemm_kernel(L
 
 // The same product with both operands by LDS-DMA, for rows of whole 16-byte chunks: several k-steps ahead, one barrier per step and nothing staged in registers.  Waves as 2 x 2, each
 // QM x QN MFMA tiles: 128 x 128 (80 KB of LDS: activations two steps ahead, weights one), 128 x 64 (72 KB, two steps), 64 x 64 (80 KB, four steps: so small a tile is all
-// latency) -- the largest that still puts two blocks on every CU.  One block's epilogue runs under the other's k-loop.
+// latency).  One block's epilogue runs under the other's k-loop.  5001 x 1000 -> 333 fp16 11 us, 16 with gelu and the pre-activation; 2048 x 512 -> 2048 fp32 40 (28 at the fp32 rate
+// of a large matrix product).  Twice the stages for grids of one block a CU: slower (13.9 us for 11.2); barrier in mid-step with the next fragments read ahead: 12.3.
 // BT: b is stored [K][N] (dx = dz w reads w as it is, without a transposed copy): its tile is sub-tiles of 64 columns by K rows, 16-bit operands are read transposed
 // (ds_read_b64_tr_b16; the activations' chunks are then read in the halves that match its row order), fp32 ones element by element.
 __device__ uint4 g_lin_zero[8];  // read-only zeros
@@ -262,7 +265,7 @@ __global__ __launch_bounds__(256, 2) void linear_dma_kernel(LinearArgs p) {
 
 // Few rows: a block of 8 waves makes 16 columns of up to 16 MT rows; every wave takes each eighth 64-byte piece of K, both operands go from memory straight into MFMA
 // operands (no LDS: nothing is used twice), and the waves' sums meet in LDS.  What counts here is latency and the number of CUs that read w: 16 columns a block
-// put 32 blocks on 512 columns.
+// put 32 blocks on 512 columns: 8 x 2048 -> 512 fp32 8.3 us, of which the 4 MB of w are one.
 template <typename T, int MT>
 __global__ __launch_bounds__(512) void linear_skinny_kernel(LinearArgs p) {
   constexpr int VE = Vec16<T>::N, KE = 4 * VE, W = 8;  // elements of a lane group's four chunks
@@ -343,6 +346,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_transpose_ke
 }
 
 // ---- dz = dy act'(pre), db ----------------------------------------------------------------------------------------------------
+// One pass, bound by HBM: 100352 x 2048 bf16 with gelu 254 us (4.9 TB/s) and 5 for the fold of the blocks' sums.
 // A block covers TX 16-byte vectors of columns (TX = 8 .. 64, the power of two at or above a narrow row's vectors) and 256 / TX rows at a time over its range of rows;
 // part [row blocks][cols] = its column sums.
 template <typename T, int TX>
@@ -611,7 +615,7 @@ static int linear_bad(const char* what, int64_t rows, int in, int out, int dtype
   return 0;
 }
 
-// The tile whose rounds over the 256 CUs cost least.  A k-step (128 bytes) of a bm x bn tile brings bm + bn rows into LDS, at about 15 bytes per clock and CU, and multiplies at 4096
+// The tile whose rounds over the 256 CUs cost least.  A k-step (128 bytes) of a bm x bn tile brings bm + bn rows into LDS, at the 15 bytes per clock and CU that these kernels reach, and multiplies at 4096
 // (fp32: 256) flops per clock, whichever takes longer, and pays its barrier: 5001 x 1000 -> 333 in 16 bits is all operand traffic (64 x 64: 2 rounds of 128 rows, 15 us; 128 x 64:
 // one of 192), 2048 x 512 -> 2048 in fp32 all arithmetic.
 template <bool BT> static int dma_launch(LinearArgs p, int dtype, hipStream_t s, const char* what) {

@@ -1,12 +1,12 @@
 // out [M][N] = a [M][K] b[N][ldb]^T of 16-bit operands for many rows and a short K (at most 512): the rows stay in registers.
 //
-// What bounds the 256 x 256 kernel at these sizes is the path from L2 into the CUs (8 TB/s over the chip, about 15 bytes per clock and CU): every tile fetches both its operands, 1.6 GB
-// for 100352 x 512 -> 2048, on top of what the epilogue moves.  Here a wave holds 32 rows of a for the WHOLE of K as MFMA operands (128 registers at K = 512), eight waves 256 rows,
+// What bounds the 256 x 256 kernel at these sizes is operand traffic: every tile fetches both its operands, 1.6 GB for 100352 x 512 -> 2048, on top of what the epilogue moves -- and the
+// epilogue's streams drive the operands out of the 4 MB L2s, behind which 8 TB/s are to be had (30 from the L2s themselves).  Here a wave holds 32 rows of a for the WHOLE of K as MFMA operands (128 registers at K = 512), eight waves 256 rows,
 // and only b streams through LDS -- half the traffic.  The work is a list of units (256 rows x 64 columns), dealt out evenly over the CUs in contiguous ranges; b's steps (64 columns x
 // 128 of K, 16 KB, four stages, fetched three steps ahead by LDS-DMA) form one sequence across the units, and the residual's tile of the next unit arrives by LDS-DMA as well, so
 // nothing in the loop waits for memory but the counted waits below; the stores drain behind them.
-// RAG: rows of a (any K) and of out (any N) at element alignment -- a goes straight to registers, so only b, which is
-// copied into padded rows first, needs whole chunks; the residual is then read in the epilogue, and the waits are not counted past stores that may be missing.
+// Measured, bf16: 100352 x 512 -> 2048 with a residual 256 us (0.93 GB: 3.6 TB/s; multiplying, storing and fetching rows do not overlap inside a block), 401408 x 256 -> 1024 283.
+// RAG: rows of a (any K) and of out (any N) at element alignment -- a goes straight to registers, so only b, which is copied into padded rows first, needs whole chunks; the residual is then read in the epilogue, and the waits are not counted past stores that may be missing.
 #include "linear.h"
 
 namespace sh {
