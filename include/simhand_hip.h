@@ -617,16 +617,17 @@ int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes
                            void* workspace, size_t workspace_bytes, sh_stream_t stream);
 
 /* z = x w^T + bias, y = act(z) + residual; x [rows][in_dim], w [out_dim][in_dim], bias fp32 [out_dim] or NULL, residual [rows][out_dim] or NULL,
- * pre [rows][out_dim] or NULL receives z (what simhand_linear_act_bwd takes).  residual may be y's own buffer. */
-size_t simhand_linear_fwd_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype);
+ * pre [rows][out_dim] or NULL receives z (what simhand_linear_act_bwd takes).  residual may be y's own buffer.  Workspace query, here and below: aligned = every operand (x, w,
+ * residual; dz, w) lies at a 16-byte address. */
+size_t simhand_linear_fwd_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int aligned);
 int simhand_linear_fwd(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, void* pre, int64_t rows, int in_dim,
                        int out_dim, int dtype, void* workspace, size_t workspace_bytes, sh_stream_t stream);
 /* dz = dy act'(pre), db [cols] fp32 = sum_rows dz (before dz is rounded).  SH_ACT_NONE: pre and dz may be NULL (dz = dy; only db is computed).  dz may be dy's buffer. */
 size_t simhand_linear_act_bwd_workspace_bytes(int64_t rows, int cols, int dtype);
 int simhand_linear_act_bwd(const void* dy, const void* pre, int act, void* dz, float* db, int64_t rows, int cols, int dtype, void* workspace,
                            size_t workspace_bytes, sh_stream_t stream);
-/* dx [rows][in_dim] = dz w (w [out_dim][in_dim] as in the forward call; its transposed copy lives in the workspace) */
-size_t simhand_linear_dgrad_workspace_bytes(int in_dim, int out_dim, int dtype);
+/* dx [rows][in_dim] = dz w (w [out_dim][in_dim] as in the forward call; where a transposed copy of it pays, that lives in the workspace) */
+size_t simhand_linear_dgrad_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int aligned);
 int simhand_linear_dgrad(const void* dz, const void* w, void* dx, int64_t rows, int in_dim, int out_dim, int dtype, void* workspace,
                          size_t workspace_bytes, sh_stream_t stream);
 /* dw [out_dim][in_dim] fp32 = dz^T x; x as it is, or (x = NULL) as its 8-bit checkpoint, whose values enter the product rounded to dtype */

@@ -361,6 +361,7 @@ static int ln_nv(int nvec) { return nvec <= 64 ? 1 : nvec <= 128 ? 2 : nvec <= 2
 // pass over 33001 x 777), and no more partial sums than that
 static int ln_bwd_blocks(int64_t rows, int cols, int dtype) {
   const int nvec = ln_nvec(cols, dtype);
+  if (rows <= 8 * ln_rows_per_block(nvec)) return 1;  // few rows: one block writes the column sums itself, a launch (of the fold) and a workspace less
   const int64_t need = (rows + ln_rows_per_block(nvec) - 1) / ln_rows_per_block(nvec);
   const int64_t most = 256 * ln_bwd_occupancy(ln_nv(nvec), dtype == SH_F32, cols % (dtype == SH_F32 ? 4 : 8) != 0);
   return (int)(need < 1 ? 1 : need > most ? most : need);
@@ -417,7 +418,8 @@ int simhand_layer_norm_fwd(const void* x, const float* gamma, const float* beta,
 
 size_t simhand_layer_norm_bwd_workspace_bytes(int64_t rows, int cols, int dtype) {
   if (rows < 0 || cols < 1) return 0;
-  return (size_t)ln_bwd_blocks(rows, cols, dtype) * 2 * cols * sizeof(float);
+  const int blocks = ln_bwd_blocks(rows, cols, dtype);
+  return blocks > 1 ? (size_t)blocks * 2 * cols * sizeof(float) : 0;
 }
 
 int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, const float* gamma, const float* beta,
@@ -431,11 +433,11 @@ int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes
   SH_REQUIRE(gamma && beta && dgamma_dbeta && (rows == 0 || (dy && (x || a8) && mean && rstd && dx)), "layer_norm_bwd: NULL argument");
   const int nvec = ln_nvec(cols, dtype);
   const int grid = ln_bwd_blocks(rows, cols, dtype);
-  SH_REQUIRE(workspace && workspace_bytes >= simhand_layer_norm_bwd_workspace_bytes(rows, cols, dtype), "layer_norm_bwd: workspace too small");
+  SH_REQUIRE(grid == 1 || (workspace && workspace_bytes >= simhand_layer_norm_bwd_workspace_bytes(rows, cols, dtype)), "layer_norm_bwd: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   const double eb = dtype == SH_F32 ? 4 : 2;
   ProfScope ps(SH_PROF_BN, s, 0, (double)rows * cols * (2 * eb + (a8 ? 1.03125 : eb)));
-  float* part = (float*)workspace;
+  float* part = grid == 1 ? dgamma_dbeta : (float*)workspace;
   const bool rag = cols % (dtype == SH_F32 ? 4 : 8) != 0;
 #define SH_LAUNCH(T, G, NV, A8, RAG, GATE)                                                                                                           \
   layer_norm_bwd_kernel<T, G, NV, A8, RAG, GATE><<<grid, 256, 0, s>>>((const T*)dy, (const T*)x, x_codes, x_exps, gamma, beta, mean, rstd, (T*)dx, part, \
@@ -463,6 +465,7 @@ int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes
 #undef SH_ONE
 #undef SH_LAUNCH
   if (check_launch("layer_norm_bwd")) return 1;
+  if (grid == 1) return 0;
   return fold_columns(part, grid, 2 * cols, dgamma_dbeta, s);
 }
 

@@ -698,6 +698,7 @@ static void act_bwd_plan(int64_t rows, int cols, int dtype, int* gx, int* gy, in
   const int tx = act_bwd_tx(cols, dtype), ty = 256 / tx, ve = dtype == SH_F32 ? 4 : 8;
   *gx = ceil_div(cols, tx * ve);
   int64_t want = (2048 + *gx - 1) / *gx, most = (rows + ty - 1) / ty;
+  if (most <= 8) want = 1;  // few rows: one block a strip of columns, whose sums need no fold (a launch and a workspace less)
   if (want > most) want = most;
   if (want < 1) want = 1;
   *per = ((rows + want - 1) / want + ty - 1) / ty * ty;
@@ -730,10 +731,11 @@ using namespace sh;
 
 extern "C" {
 
-size_t simhand_linear_fwd_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype) {
+size_t simhand_linear_fwd_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int aligned) {
   if (rows < 1 || in_dim < 1 || out_dim < 1 || dtype != SH_BF16) return 0;
-  // the padded copy of w, if the call turns out to need it (rows that are no whole 16-byte chunks, by length or by address)
-  LinearArgs p = {(const void*)2, nullptr, nullptr, nullptr, nullptr, (const void*)2, rows, out_dim, in_dim, in_dim, SH_ACT_NONE, 0};
+  // the padded copy of w, where the rows-in-registers kernel takes rows that are no whole 16-byte chunks, by length or by address (with a residual it takes more cases)
+  const void* at = (const void*)(size_t)(aligned ? 16 : 2);
+  LinearArgs p = {at, at, nullptr, nullptr, nullptr, at, rows, out_dim, in_dim, in_dim, SH_ACT_NONE, 0};
   return linear_rows_takes(p, dtype) ? linear_rows_workspace_bytes(p) : 0;
 }
 
@@ -743,7 +745,7 @@ int simhand_linear_fwd(const void* x, const void* w, const float* bias, int act,
   SH_REQUIRE(act >= SH_ACT_NONE && act <= SH_ACT_SILU, "linear_fwd: act %d", act);
   if (rows == 0) return 0;
   SH_REQUIRE(x && w && y, "linear_fwd: NULL argument");
-  const size_t need = simhand_linear_fwd_workspace_bytes(rows, in_dim, out_dim, dtype);
+  const size_t need = simhand_linear_fwd_workspace_bytes(rows, in_dim, out_dim, dtype, !(((size_t)x | (size_t)w | (size_t)residual) & 15));
   SH_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && !((size_t)workspace & 15)), "linear_fwd: workspace too small or not at a 16-byte address");
   hipStream_t s = (hipStream_t)stream;
   const double eb = dtype == SH_F32 ? 4 : 2;
@@ -757,7 +759,7 @@ size_t simhand_linear_act_bwd_workspace_bytes(int64_t rows, int cols, int dtype)
   int gx, gy;
   int64_t per;
   act_bwd_plan(rows, cols, dtype, &gx, &gy, &per);
-  return (size_t)gy * cols * sizeof(float);
+  return gy > 1 ? (size_t)gy * cols * sizeof(float) : 0;
 }
 
 int simhand_linear_act_bwd(const void* dy, const void* pre, int act, void* dz, float* db, int64_t rows, int cols, int dtype, void* workspace,
@@ -766,13 +768,14 @@ int simhand_linear_act_bwd(const void* dy, const void* pre, int act, void* dz, f
   SH_REQUIRE(act >= SH_ACT_NONE && act <= SH_ACT_SILU, "linear_act_bwd: act %d", act);
   SH_REQUIRE(db && (rows == 0 || dy), "linear_act_bwd: NULL argument");
   SH_REQUIRE(rows == 0 || act == SH_ACT_NONE || (pre && dz), "linear_act_bwd: an activation needs pre and dz");
-  SH_REQUIRE(workspace && workspace_bytes >= simhand_linear_act_bwd_workspace_bytes(rows, cols, dtype), "linear_act_bwd: workspace too small");
+  const size_t need = simhand_linear_act_bwd_workspace_bytes(rows, cols, dtype);
+  SH_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "linear_act_bwd: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   ProfScope ps(SH_PROF_MISC, s, 0, (dtype == SH_F32 ? 4.0 : 2.0) * rows * cols * (act == SH_ACT_NONE ? 1 : 3));
   int gx, gy;
   int64_t per;
   act_bwd_plan(rows, cols, dtype, &gx, &gy, &per);
-  float* part = (float*)workspace;
+  float* part = gy == 1 ? db : (float*)workspace;
   const dim3 grid(gx, gy);
 #define SH_ACT(T, TX) linear_act_bwd_kernel<T, TX><<<grid, 256, 0, s>>>((const T*)dy, (const T*)pre, act, (T*)dz, part, rows, cols, per)
 #define SH_ACT_TX(T)                       \
@@ -787,31 +790,39 @@ int simhand_linear_act_bwd(const void* dy, const void* pre, int act, void* dz, f
 #undef SH_ACT_TX
 #undef SH_ACT
   if (check_launch("linear_act_bwd")) return 1;
+  if (gy == 1) return 0;
   return fold_columns(part, gy, cols, db, s);
 }
 
-size_t simhand_linear_dgrad_workspace_bytes(int in_dim, int out_dim, int dtype) {
-  if (in_dim < 1 || out_dim < 1) return 0;
+// dx = dz w with w as it is, unless the product is large enough for the kernels for many rows (whose transposed copy of w is then small change) or w's rows are no whole chunks
+static bool dgrad_direct(int64_t rows, int in_dim, int out_dim, int dtype, bool aligned) {
+  const int ve = dtype == SH_F32 ? 4 : 8;
+  if (in_dim % ve || out_dim % ve || !aligned) return false;
+  const void* at = (const void*)(size_t)16;
+  LinearArgs wide = {at, at, nullptr, nullptr, nullptr, nullptr, rows, in_dim, out_dim, (out_dim + 7) / 8 * 8, SH_ACT_NONE, 0};
+  return !linear256_takes(wide, dtype) && !linear_rows_takes(wide, dtype);
+}
+size_t simhand_linear_dgrad_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int aligned) {
+  if (rows < 1 || in_dim < 1 || out_dim < 1 || dgrad_direct(rows, in_dim, out_dim, dtype, aligned != 0)) return 0;
   return (size_t)in_dim * ((out_dim + 7) / 8 * 8) * (dtype == SH_F32 ? 4 : 2);
 }
-
 int simhand_linear_dgrad(const void* dz, const void* w, void* dx, int64_t rows, int in_dim, int out_dim, int dtype, void* workspace,
                          size_t workspace_bytes, sh_stream_t stream) {
   if (linear_bad("linear_dgrad", rows, in_dim, out_dim, dtype)) return 1;
   if (rows == 0) return 0;
   SH_REQUIRE(dz && w && dx, "linear_dgrad: NULL argument");
-  SH_REQUIRE(workspace && workspace_bytes >= simhand_linear_dgrad_workspace_bytes(in_dim, out_dim, dtype), "linear_dgrad: workspace too small");
-  SH_REQUIRE(!((size_t)workspace & 15), "linear_dgrad: workspace at a 16-byte address");
+  const bool direct = dgrad_direct(rows, in_dim, out_dim, dtype, !(((size_t)dz | (size_t)w) & 15));
+  SH_REQUIRE(direct || (workspace && workspace_bytes >= simhand_linear_dgrad_workspace_bytes(rows, in_dim, out_dim, dtype, 0) && !((size_t)workspace & 15)),
+             "linear_dgrad: workspace too small or not at a 16-byte address");
   hipStream_t s = (hipStream_t)stream;
   const double eb = dtype == SH_F32 ? 4 : 2;
   ProfScope ps(SH_PROF_MISC, s, 2.0 * rows * in_dim * out_dim, eb * ((double)rows * in_dim + (double)in_dim * out_dim + (double)rows * out_dim));
-  // dx = dz w with w as it is, unless the product is large enough for the 256-wide tiles (whose transposed copy of w is then small change) or w's rows are no whole chunks
-  const int ve = dtype == SH_F32 ? 4 : 8;
-  LinearArgs direct = {dz, w, dx, nullptr, nullptr, nullptr, rows, in_dim, out_dim, in_dim, SH_ACT_NONE, 0};
-  LinearArgs wide = {dz, workspace, dx, nullptr, nullptr, nullptr, rows, in_dim, out_dim, (out_dim + 7) / 8 * 8, SH_ACT_NONE, 0};
-  if (in_dim % ve == 0 && out_dim % ve == 0 && !(((size_t)dz | (size_t)w) & 15) && !linear256_takes(wide, dtype) && !linear_rows_takes(wide, dtype))
-    return by_row_ranges(direct, dtype, [&](const LinearArgs& q) { return dma_launch<true>(q, dtype, s, "linear_dgrad"); });
+  if (direct) {
+    LinearArgs p = {dz, w, dx, nullptr, nullptr, nullptr, rows, in_dim, out_dim, in_dim, SH_ACT_NONE, 0};
+    return by_row_ranges(p, dtype, [&](const LinearArgs& q) { return dma_launch<true>(q, dtype, s, "linear_dgrad"); });
+  }
   const int ldt = (out_dim + 7) / 8 * 8;
+  LinearArgs wide = {dz, workspace, dx, nullptr, nullptr, nullptr, rows, in_dim, out_dim, ldt, SH_ACT_NONE, 0};
   const dim3 tg(ceil_div(in_dim, 32), ceil_div(ldt, 32));
   if (dtype == SH_F32) linear_transpose_kernel<float><<<tg, 256, 0, s>>>((const float*)w, (float*)workspace, out_dim, in_dim, ldt);
   else linear_transpose_kernel<bf16_t><<<tg, 256, 0, s>>>((const bf16_t*)w, (bf16_t*)workspace, out_dim, in_dim, ldt);

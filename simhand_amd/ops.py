@@ -213,24 +213,23 @@ class Act8:
         return self.codes.device
 
 
-def _rows_of(x, what: str) -> Tuple[int, int]:
+def _rows_of(x: torch.Tensor, what: str) -> Tuple[int, int]:
     """(rows, cols) of a row tensor [..., cols] that lives on the current device (the launch goes to that device's current stream)."""
-    dev = x.device
-    if dev.type != "cuda":
+    if not x.is_cuda:
         raise _lib.SimhandHipError(f"{what}: simhand_amd ops need device tensors (there is no CPU path)")
-    if dev.index != torch.cuda.current_device():
-        raise _lib.SimhandHipError(f"{what}: the tensor is on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+    if x.get_device() != torch._C._cuda_getDevice():
+        raise _lib.SimhandHipError(f"{what}: the tensor is on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
     shape = x.shape
     if len(shape) < 1 or shape[-1] < 1:
         raise _lib.SimhandHipError(f"{what}: rows of at least one value, got shape {tuple(shape)}")
     cols = shape[-1]
-    n = x.codes.numel() if isinstance(x, Act8) else x.numel()
-    return n // cols, cols
+    return x.numel() // cols, cols
 
 
-# Small batches are bound by the host: the row operators pass addresses and the stream as plain integers (what ctypes makes of a c_void_p anyway; 0 = NULL)
-def _row_stream(x) -> int:
-    return torch._C._cuda_getCurrentRawStream(x.device.index)
+# Small batches are bound by the host (a launch through ctypes takes 3.6 of layer_norm_fwd's 9 us): the row operators pass addresses and the stream as plain integers (what
+# ctypes makes of a c_void_p anyway; 0 = NULL) and compare device numbers, not device objects
+def _row_stream(x: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(x.get_device())
 
 
 def _at(t: torch.Tensor) -> int:
@@ -239,19 +238,21 @@ def _at(t: torch.Tensor) -> int:
     return t.data_ptr()
 
 
-def _like(t: Optional[torch.Tensor], x, shape, dtype: torch.dtype, what: str) -> int:
+def _like(t: Optional[torch.Tensor], x: torch.Tensor, shape, dtype: torch.dtype, what: str) -> int:
     """Address of an operand that has to have this shape and type, on x's device (None: NULL)."""
     if t is None:
         return 0
-    if t.shape != shape or t.dtype != dtype or t.device != x.device:
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != x.get_device():
         raise _lib.SimhandHipError(f"{what}: expected {tuple(shape)} {dtype} on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    return _at(t)
+    if not t.is_contiguous():
+        raise _lib.SimhandHipError("simhand_amd ops need contiguous tensors")
+    return t.data_ptr()
 
 
 def _saved(x, like: torch.Tensor, shape, what: str):
     """(x, codes, exps) addresses of a saved activation: a tensor, or its 8-bit checkpoint."""
     if isinstance(x, Act8):
-        if x.dtype != like.dtype:
+        if x.dtype is not like.dtype:
             raise _lib.SimhandHipError(f"{what}: checkpoint of a {x.dtype} activation next to a {like.dtype} gradient")
         return 0, _like(x.codes, like, shape, torch.uint8, what), _at(x.exps)
     return _like(x, like, shape, like.dtype, what), 0, 0
@@ -294,10 +295,10 @@ def layer_norm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, beta: torch.Tensor,
     dgb = torch.empty((2, cols), dtype=_F32, device=dy.device)
     d = dt(dy.dtype)
     nb = lib.simhand_layer_norm_bwd_workspace_bytes(rows, cols, d)
-    ws = _scratch(nb, dy)
+    ws = _scratch(nb, dy) if nb else None
     check(lib.simhand_layer_norm_bwd(pdy, px, pc, pe, _like(gamma, dy, shape, _F32, what + " (gamma)"), _like(beta, dy, shape, _F32, what + " (beta)"),
                                      _like(mean, dy, stats, _F32, what + " (mean)"), _like(rstd, dy, stats, _F32, what + " (rstd)"), 1 if relu else 0,
-                                     dx.data_ptr(), dgb.data_ptr(), rows, cols, d, ws.data_ptr(), nb, _row_stream(dy)), what)
+                                     dx.data_ptr(), dgb.data_ptr(), rows, cols, d, ws.data_ptr() if nb else 0, nb, _row_stream(dy)), what)
     dgamma, dbeta = dgb.unbind(0)
     return dx, dgamma, dbeta
 
@@ -319,7 +320,7 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     y = torch.empty(shape, dtype=x.dtype, device=x.device)
     pre = torch.empty_like(y) if want_pre else None
     d = dt(x.dtype)
-    nb = lib.simhand_linear_fwd_workspace_bytes(rows, cin, cout, d)
+    nb = lib.simhand_linear_fwd_workspace_bytes(rows, cin, cout, d, 1 if (px | pw | pr) & 15 == 0 else 0)
     ws = _scratch(nb, x) if nb else None
     check(lib.simhand_linear_fwd(px, pw, pb, a, pr, y.data_ptr(), pre.data_ptr() if want_pre else 0, rows, cin, cout, d, ws.data_ptr() if nb else 0, nb, _row_stream(x)),
           "linear_fwd")
@@ -339,8 +340,9 @@ def linear_act_bwd(dy: torch.Tensor, pre: Optional[torch.Tensor] = None, act: Op
     dz = torch.empty_like(dy) if a else dy
     db = torch.empty(cols, dtype=_F32, device=dy.device)
     nb = lib.simhand_linear_act_bwd_workspace_bytes(rows, cols, d)
-    ws = _scratch(nb, dy)
-    check(lib.simhand_linear_act_bwd(pdy, ppre, a, dz.data_ptr() if a else 0, db.data_ptr(), rows, cols, d, ws.data_ptr(), nb, _row_stream(dy)), "linear_act_bwd")
+    ws = _scratch(nb, dy) if nb else None
+    check(lib.simhand_linear_act_bwd(pdy, ppre, a, dz.data_ptr() if a else 0, db.data_ptr(), rows, cols, d, ws.data_ptr() if nb else 0, nb, _row_stream(dy)),
+          "linear_act_bwd")
     return dz, db
 
 
@@ -362,9 +364,9 @@ def linear_bwd(dz: torch.Tensor, x, w: torch.Tensor, need_dx: bool = True):
     dx = None
     if need_dx:
         dx = torch.empty(xshape, dtype=dz.dtype, device=dz.device)
-        nb = lib.simhand_linear_dgrad_workspace_bytes(cin, cout, d)
-        ws = _scratch(nb, dz)
-        check(lib.simhand_linear_dgrad(pz, pw, dx.data_ptr(), rows, cin, cout, d, ws.data_ptr(), nb, _row_stream(dz)), "linear_dgrad")
+        nb = lib.simhand_linear_dgrad_workspace_bytes(rows, cin, cout, d, 1 if (pz | pw) & 15 == 0 else 0)
+        ws = _scratch(nb, dz) if nb else None
+        check(lib.simhand_linear_dgrad(pz, pw, dx.data_ptr(), rows, cin, cout, d, ws.data_ptr() if nb else 0, nb, _row_stream(dz)), "linear_dgrad")
     return dx, _wgrad(lib, dz, pz, px, pc, pe, rows, cin, cout, d)
 
 
@@ -393,7 +395,7 @@ def act8_pack(x: torch.Tensor) -> Act8:
     rows, cols = _rows_of(x, "act8_pack")
     lib = _lib_dev()
     px, d = _at(x), dt(x.dtype)
-    codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+    codes = torch.empty_like(x, dtype=torch.uint8)
     exps = torch.empty((rows, (cols + 31) // 32), dtype=torch.uint8, device=x.device)
     check(lib.simhand_act8_pack(px, codes.data_ptr(), exps.data_ptr(), rows, cols, d, _row_stream(x)), "act8_pack")
     return Act8(codes, exps, x.dtype)
@@ -401,11 +403,12 @@ def act8_pack(x: torch.Tensor) -> Act8:
 
 def act8_unpack(a: Act8) -> torch.Tensor:
     """The values an 8-bit checkpoint stands for, in the type it was packed from."""
-    rows, cols = _rows_of(a, "act8_unpack")
+    codes = a.codes
+    rows, cols = _rows_of(codes, "act8_unpack")
     lib = _lib_dev()
-    pc, pe, d = _at(a.codes), _at(a.exps), dt(a.dtype)
-    x = torch.empty(a.shape, dtype=a.dtype, device=a.device)
-    check(lib.simhand_act8_unpack(pc, pe, x.data_ptr(), rows, cols, d, _row_stream(a)), "act8_unpack")
+    pc, pe, d = _at(codes), _at(a.exps), dt(a.dtype)
+    x = torch.empty_like(codes, dtype=a.dtype)
+    check(lib.simhand_act8_unpack(pc, pe, x.data_ptr(), rows, cols, d, _row_stream(codes)), "act8_unpack")
     return x
 
 

@@ -546,7 +546,7 @@ def test_nothing_is_written_beside_the_outputs(dtype):
     y, yv = guarded(m * n, dtype); pre, prev = guarded(m * n, dtype)
     assert lib.simhand_linear_fwd(p(x), p(w), None, 2, None, p(yv), p(prev), m, k, n, d, None, 0, st) == 0
     dx, dxv = guarded(m * k, dtype)
-    ws = torch.empty(lib.simhand_linear_dgrad_workspace_bytes(k, n, d), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(lib.simhand_linear_dgrad_workspace_bytes(m, k, n, d, 0), dtype=torch.uint8, device="cuda")
     assert lib.simhand_linear_dgrad(p(dz), p(w), p(dxv), m, k, n, d, p(ws), ws.numel(), st) == 0
     dw, dwv = guarded(n * k, torch.float32)
     ws2 = torch.empty(lib.simhand_linear_wgrad_workspace_bytes(m, k, n, d) + 16, dtype=torch.uint8, device="cuda")
@@ -760,8 +760,8 @@ def test_nothing_is_written_beside_outputs_and_workspaces(dtype, m, k, n):
         bufs.append(buf)
         return buf[pad:pad + count]
 
-    nf = lib.simhand_linear_fwd_workspace_bytes(m, k, n, d)
-    nd, nw = lib.simhand_linear_dgrad_workspace_bytes(k, n, d), lib.simhand_linear_wgrad_workspace_bytes(m, k, n, d)
+    nf = lib.simhand_linear_fwd_workspace_bytes(m, k, n, d, 1)
+    nd, nw = lib.simhand_linear_dgrad_workspace_bytes(m, k, n, d, 1), lib.simhand_linear_wgrad_workspace_bytes(m, k, n, d)
     for res in (0, dz.data_ptr()):
         y, pre, ws = guarded(m * n, dtype), guarded(m * n, dtype), guarded(nf, torch.uint8)
         assert lib.simhand_linear_fwd(x.data_ptr(), w.data_ptr(), 0, 2, res, y.data_ptr(), pre.data_ptr(), m, k, n, d, ws.data_ptr(), nf, st) == 0

@@ -23,7 +23,7 @@ def test_c_entry_points_refuse_bad_arguments():
     assert refused(lib.simhand_layer_norm_fwd(P, P, P, 1e-5, 0, P, P, P, 4, 16385, 1, N))          # too wide, 16 bits
     assert refused(lib.simhand_layer_norm_fwd(P, P, P, -1.0, 0, P, P, P, 4, 8, 0, N))              # eps
     assert refused(lib.simhand_layer_norm_fwd(N, P, P, 1e-5, 0, P, P, P, 4, 8, 0, N))              # x
-    assert refused(lib.simhand_layer_norm_bwd(P, P, N, N, P, P, P, P, 0, P, P, 4, 8, 0, P, 4, N))  # workspace
+    assert refused(lib.simhand_layer_norm_bwd(P, P, N, N, P, P, P, P, 0, P, P, 4000, 8, 0, P, 4, N))  # workspace
     assert refused(lib.simhand_layer_norm_bwd(P, P, P, P, P, P, P, P, 0, P, P, 4, 8, 0, P, 1 << 20, N))  # x and codes
     assert refused(lib.simhand_layer_norm_bwd(P, N, P, N, P, P, P, P, 0, P, P, 4, 8, 0, P, 1 << 20, N))  # codes without exponents
     assert refused(lib.simhand_linear_fwd(P, P, N, 4, N, P, N, 4, 8, 8, 0, P, 1 << 30, N))                     # act
@@ -33,7 +33,7 @@ def test_c_entry_points_refuse_bad_arguments():
     assert refused(lib.simhand_linear_fwd(P, P, N, 0, N, N, N, 4, 8, 8, 0, P, 1 << 30, N))                     # y
     assert refused(lib.simhand_linear_fwd(P, P, N, 0, N, P, N, 200000, 77, 130, 1, N, 0, N))       # workspace
     assert refused(lib.simhand_linear_act_bwd(P, N, 2, P, P, 4, 8, 0, P, 1 << 20, N))              # gelu without pre
-    assert refused(lib.simhand_linear_act_bwd(P, P, 2, P, P, 4, 8, 0, N, 0, N))                    # workspace
+    assert refused(lib.simhand_linear_act_bwd(P, P, 2, P, P, 4000, 8, 0, N, 0, N))                 # workspace
     assert refused(lib.simhand_linear_dgrad(P, P, P, 4, 8, 8, 0, P, 8, N))                         # workspace
     assert refused(lib.simhand_linear_wgrad(P, P, N, N, N, 4, 8, 8, 0, P, 1 << 20, N))             # dw
     assert refused(lib.simhand_linear_wgrad(P, P, N, N, P, 4, 8, 8, 2, P, 1 << 20, N))             # dtype
@@ -53,12 +53,13 @@ def test_no_rows_is_no_launch():
 
 def test_workspace_queries():
     lib = _lib.load()
-    assert lib.simhand_layer_norm_bwd_workspace_bytes(0, 8, 0) > 0
+    assert lib.simhand_layer_norm_bwd_workspace_bytes(0, 8, 0) == 0  # one block: its sums are the result
+    assert lib.simhand_layer_norm_bwd_workspace_bytes(4000, 8, 0) > 0
     assert lib.simhand_layer_norm_bwd_workspace_bytes(-1, 8, 0) == 0
-    assert lib.simhand_linear_dgrad_workspace_bytes(8, 0, 0) == 0
+    assert lib.simhand_linear_dgrad_workspace_bytes(4, 8, 0, 0, 0) == 0
     for rows in (0, 1, 1000, 401408, (1 << 31) - 1):
         for cols in (1, 77, 2048):
-            assert 0 < lib.simhand_linear_act_bwd_workspace_bytes(rows, cols, 1) < 1 << 28
+            assert 0 <= lib.simhand_linear_act_bwd_workspace_bytes(rows, cols, 1) < 1 << 28
             assert 0 <= lib.simhand_linear_wgrad_workspace_bytes(rows, cols, 512, 1) < 1 << 30
 
 
