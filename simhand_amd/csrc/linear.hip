@@ -8,9 +8,9 @@
 // operands global -> registers -> LDS with the next step's loads in flight under the MFMAs (a second step in flight and a second buffer: no faster).
 // 100000 x 777 -> 333: bf16 138 us, fp32 548 (336 at the fp32 rate of a large matrix product).  The operands are swapped (b is the MFMA's first one), and b's rows are permuted inside
 // the tile, so that a lane ends with 8 consecutive columns of one row: bias, residual, pre-activation and output move as 16-byte vectors.
-// linear_wgrad_kernel: dw [N][K] = dz^T x, the reduction runs over rows: tiles of 64, 128 or 256 squared over a range of rows (split), 16-bit operands are read transposed from LDS
-// (ds_read_b64_tr_b16); the splits' fp32 partial sums are added in a fixed order by a second launch.  100000 x 777 -> 333: bf16 149 us, fp32 617; 400000 x 64 -> 64 bf16 29;
-// 2048 x 2048 -> 512 fp32 48 + 8 (28 at that rate).
+// linear_wgrad_kernel: dw [N][K] = dz^T x, the reduction runs over rows: tiles of 64 or 128 squared over a range of rows (split), 16-bit operands are read transposed from LDS
+// (ds_read_b64_tr_b16); the splits' fp32 partial sums are added in a fixed order by a second launch.  100000 x 777 -> 333: bf16 113 us, fp32 608; 400000 x 64 -> 64 bf16 27;
+// 2048 x 2048 -> 512 fp32 53 (28 at that rate).
 #include "linear.h"
 
 namespace sh {
@@ -392,24 +392,24 @@ __global__ __launch_bounds__(256) void linear_act_bwd_kernel(const T* __restrict
 
 // ---- dw = dz^T x ---------------------------------------------------------------------------------------------------------------
 // A tile of TILE columns of either operand by KP rows a step, staged global -> registers -> LDS, so any alignment will do: 16-byte loads at element addresses, PF steps ahead (the ragged
-// columns behind a row are the next row's -- read, multiplied and never stored; only the tensor's very last chunk goes element by element).  256: 8 waves as 2 x 4 of 128 x 64, for wide
-// layers whose rows are no whole chunks (the LDS-DMA kernel takes the others); 128, 64: 4 waves as 2 x 2.
-template <int TILE> struct WgradWaves { static constexpr int M = 2, N = TILE == 256 ? 4 : 2, THREADS = 64 * M * N; };
+// columns behind a row are the next row's -- read, multiplied and never stored; only the tensor's very last chunk goes element by element).  4 waves as 2 x 2.  (Tiles of 256 with 8
+// waves: 100000 x 777 -> 333 in 16 bits 143 us for 113, 50000 x 1537 -> 400 122 for 135.)
+constexpr int wgrad_rows(bool h, int tile) { return h || tile == 64 ? 32 : 16; }  // of a step
 
 template <typename T, bool A8, int TILE>
-__global__ __launch_bounds__(WgradWaves<TILE>::THREADS, TILE == 256 ? 1 : TILE == 128 ? 2 : 4) void linear_wgrad_kernel(WgradArgsL p) {
+__global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_wgrad_kernel(WgradArgsL p) {
   constexpr bool H = sizeof(T) == 2;
-  constexpr int VE = Vec16<T>::N, NT = WgradWaves<TILE>::THREADS;
-  constexpr int QM = TILE / 16 / WgradWaves<TILE>::M, QN = TILE / 16 / WgradWaves<TILE>::N;  // MFMA tiles of a wave
-  constexpr int KP = H ? 32 : TILE == 64 ? 32 : 16;     // rows per step
+  constexpr int VE = Vec16<T>::N, NT = 256;
+  constexpr int QM = TILE / 32, QN = TILE / 32;         // MFMA tiles of a wave
+  constexpr int KP = wgrad_rows(H, TILE);               // rows per step
   constexpr int CH = TILE / VE, NCH = KP * CH / NT;     // 16-byte chunks of a tile row; per thread and operand
-  constexpr int PF = TILE == 256 || (TILE == 64 && sizeof(T) == 4) ? 2 : 3;  // (3 would not fit the registers of those two)
+  constexpr int PF = TILE == 64 && sizeof(T) == 4 ? 2 : 3;  // (3 would not fit its registers)
   static_assert(KP * CH % NT == 0, "a whole number of chunks for every thread");
   // 16 bits: sub-tiles of [KP rows][64 columns] whose 32-byte column groups are rotated by row / 2 (as the LDS-DMA kernel's); fp32: rows padded by 64 bytes
   constexpr int STRIDE = H ? TILE * 2 : TILE * 4 + 64, OPERAND = KP * STRIDE;
   __shared__ __attribute__((aligned(16))) char smem[4 * OPERAND];  // two stages, one barrier per step
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int li = lane & 15, g = lane >> 4, wm = wave / WgradWaves<TILE>::N, wn = wave % WgradWaves<TILE>::N;
+  const int li = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
   unsigned logical = xcd_order(blockIdx.x, gridDim.x);
   const int k0 = (int)(logical % p.k_tiles) * TILE; logical /= p.k_tiles;
   const int n0 = (int)(logical % p.n_tiles) * TILE;
@@ -707,22 +707,34 @@ static void act_bwd_plan(int64_t rows, int cols, int dtype, int* gx, int* gy, in
   if (*gy < 1) *gy = 1;
 }
 
-// Tile and splits over the rows (every split writes and re-reads its own dw).  16 bits, both sides wide, many rows: 256-wide tiles, one block per CU; else 128-wide ones while they are
-// enough for two blocks per CU with at most 8 splits, or where the rows are many and a side is wider than 64; else 64-wide ones, four blocks per CU.
+// Tile and splits of the rows: the pair whose estimate is least.  A step of a tile takes (us, measured with one / two / four blocks on a CU over 16384 x 1023 -> 1023) 0.37 / 0.39 / 0.66
+// in 16 bits and 1.0 / 1.5 / 2.5 in fp32 for 64, 0.60 / 0.69 and 1.35 / 2.24 for 128 (of 32 rows, in fp32 16); the join of the splits reads and writes their sums at 4 TB/s and is a
+// launch more.  It takes 64 without a split for 1000 x 1000 -> 1000 in 16 bits (13.7 us; in four 20.8), 64 in 8 splits for 5001 x
+// 1000 -> 333 (21; 128 in 20: 26), 128 in 24 for 100000 x 777 -> 333 (113; 64: 180), and 64 in 4 for 2048 x 2048 -> 512 in fp32 (53; 128 in 8: 56).
 static int linear_wgrad_plan(int64_t rows, int in, int out, int dtype, int* splits, int64_t* per) {
-  const int64_t t128 = (int64_t)ceil_div(in, 128) * ceil_div(out, 128);
-  const int tile = dtype != SH_F32 && in > 128 && out > 128 && rows >= 4096 ? 256 : t128 * 8 >= 512 || (rows > 16384 && (in > 64 || out > 64)) ? 128 : 64;
-  const int blocks = tile == 256 ? 256 : tile == 128 ? 512 : 1024;
-  const int kp = dtype == SH_F32 && tile == 128 ? 16 : 32;
-  const int64_t tiles = (int64_t)ceil_div(in, tile) * ceil_div(out, tile);
-  const int64_t steps = rows > 0 ? (rows + kp - 1) / kp : 1;
-  int64_t sk = blocks / tiles;
-  if (sk > (steps + 7) / 8) sk = (steps + 7) / 8;  // at least 8 steps each
-  if (sk < 1) sk = 1;
-  const int64_t each = (steps + sk - 1) / sk;
-  *per = each * kp;
-  *splits = (int)((steps + each - 1) / each);
-  return tile;
+  const bool h = dtype != SH_F32;
+  double best = 0.;
+  int best_tile = 0;
+  for (int tile = 64; tile <= 128; tile *= 2) {
+    const int kp = wgrad_rows(h, tile), most = tile == 64 ? 4 : 2;  // blocks on a CU
+    const int64_t tiles = (int64_t)ceil_div(in, tile) * ceil_div(out, tile), steps = rows > 0 ? (rows + kp - 1) / kp : 1;
+    for (int on_cu = 0; on_cu <= most; ++on_cu) {  // as many splits as put on_cu blocks on every CU, of at least 4 steps each; 0: no split
+      int64_t sk = on_cu == 0 ? 1 : 256 * on_cu / tiles;
+      if (sk > steps / 4) sk = steps / 4;
+      if (sk < 1) sk = 1;
+      const int64_t each = (steps + sk - 1) / sk, full = (sk * tiles + 255) / 256, rounds = (full + most - 1) / most;
+      const double b = (double)(full < most ? full : most);
+      const double t = tile == 64 ? (h ? (b <= 2 ? 0.36 + 0.015 * b : 0.165 * b) : 0.45 + 0.52 * b) : (h ? 0.51 + 0.09 * b : 0.46 + 0.89 * b);
+      const double cost = (double)(rounds * each) * t + (sk > 1 ? 5. + (double)sk * in * out * 2e-6 : 0.);
+      if (best_tile == 0 || cost < best) {
+        best = cost;
+        best_tile = tile;
+        *per = each * kp;
+        *splits = (int)((steps + each - 1) / each);
+      }
+    }
+  }
+  return best_tile;
 }
 
 }  // namespace sh
@@ -872,10 +884,6 @@ int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, 
 #define SH_WGRAD(T, A8)                                                               \
   if (tile == 128) linear_wgrad_kernel<T, A8, 128><<<grid, 256, 0, s>>>(p);           \
   else linear_wgrad_kernel<T, A8, 64><<<grid, 256, 0, s>>>(p)
-    if (tile == 256) {
-      if (a8) linear_wgrad_kernel<bf16_t, true, 256><<<grid, 512, 0, s>>>(p);
-      else linear_wgrad_kernel<bf16_t, false, 256><<<grid, 512, 0, s>>>(p);
-    } else
     if (dtype == SH_F32) {
       if (a8) { SH_WGRAD(float, true); }
       else { SH_WGRAD(float, false); }
