@@ -615,6 +615,14 @@ static int linear_bad(const char* what, int64_t rows, int in, int out, int dtype
   return 0;
 }
 
+// What 32 elements of the reduction of a register-staged tile take (us) with `on_cu` blocks on a CU, measured with one / two / four (16384 x 1023 -> 1023, weight gradient; the product
+// agrees): 64 x 64 0.37 / 0.39 / 0.66 in 16 bits and 1.0 / 1.5 / 2.5 in fp32, 128 x 128 0.60 / 0.69 and 2.7 / 4.5.
+static double staged_us(bool h, int tile, int on_cu) {
+  if (tile == 64) return h ? (on_cu <= 2 ? 0.36 + 0.015 * on_cu : 0.165 * on_cu) : 0.45 + 0.52 * on_cu;
+  return h ? 0.51 + 0.09 * on_cu : 0.92 + 1.78 * on_cu;
+}
+static int staged_on_cu(int tile) { return tile == 64 ? 4 : 2; }  // blocks that fit a CU
+
 // The tile whose rounds over the 256 CUs cost least.  A k-step (128 bytes) of a bm x bn tile brings bm + bn rows into LDS, at the 15 bytes per clock and CU that these kernels reach, and multiplies at 4096
 // (fp32: 256) flops per clock, whichever takes longer, and pays its barrier: 5001 x 1000 -> 333 in 16 bits is all operand traffic (64 x 64: 2 rounds of 128 rows, 15 us; 128 x 64:
 // one of 192), 2048 x 512 -> 2048 in fp32 all arithmetic.
@@ -653,8 +661,8 @@ template <typename F> static int by_row_ranges(const LinearArgs& p, int dtype, F
   return 0;
 }
 
-// Which kernel: few rows -> the skinny one (rows <= 64 and so little work that tiles would leave most CUs idle); 64-wide tiles while 128-wide ones would not put two
-// blocks on each of the 256 CUs; else 128-wide ones.
+// Which kernel: few rows -> the skinny one (rows <= 64 and so little work that tiles would leave most CUs idle); many -> rows in registers or the 256-wide tiles, as their rules say; whole
+// chunks -> the DMA tiles; anything else staged through registers.
 static int gemm_launch(const LinearArgs& base, bool b_padded, void* workspace, int dtype, hipStream_t s, const char* what) {
   LinearArgs p = base;
   if (p.M <= 64 && ceil_div(p.N, 64) < 256) {
@@ -677,7 +685,15 @@ static int gemm_launch(const LinearArgs& base, bool b_padded, void* workspace, i
   if (linear256_takes(p, dtype)) return linear256_launch(p, s, what);
   const int ve = dtype == SH_F32 ? 4 : 8;
   if (p.K % ve == 0 && p.ldb % ve == 0 && !(((size_t)p.a | (size_t)p.b) & 15)) return dma_launch<false>(p, dtype, s, what);
-  const int tile = (int64_t)ceil_div(p.M, 128) * ceil_div(p.N, 128) >= 512 ? 128 : 64;
+  // the tile whose rounds over the CUs cost least, each with its ends (1.2 and 4 us): 128 for 100000 x 777 -> 333 (16 bits 113 us, 64: 173; fp32 532 and 546), 64 for 400000 x 65 -> 63 (43 and
+  // 53; fp32 61 and 113) and, for its last round, 5001 x 2047 -> 2047 in fp32 (393 and 515)
+  auto cost = [&](int t) {
+    const int64_t blocks = (int64_t)ceil_div(p.M, t) * ceil_div(p.N, t), round = 256 * staged_on_cu(t), full = blocks / round, rest = blocks % round;
+    const bool h = dtype != SH_F32;
+    const double steps = (p.K + 31) / 32;
+    return full * staged_us(h, t, staged_on_cu(t)) * steps + (rest ? staged_us(h, t, (int)((rest + 255) / 256)) * steps : 0.) + (full + (rest > 0)) * (t == 64 ? 1.2 : 4.);
+  };
+  const int tile = cost(128) < cost(64) ? 128 : 64;
   p.n_tiles = (unsigned)ceil_div(p.N, tile);
   const unsigned grid = (unsigned)ceil_div(p.M, tile) * p.n_tiles;
   if (tile == 128) {
@@ -707,24 +723,22 @@ static void act_bwd_plan(int64_t rows, int cols, int dtype, int* gx, int* gy, in
   if (*gy < 1) *gy = 1;
 }
 
-// Tile and splits of the rows: the pair whose estimate is least.  A step of a tile takes (us, measured with one / two / four blocks on a CU over 16384 x 1023 -> 1023) 0.37 / 0.39 / 0.66
-// in 16 bits and 1.0 / 1.5 / 2.5 in fp32 for 64, 0.60 / 0.69 and 1.35 / 2.24 for 128 (of 32 rows, in fp32 16); the join of the splits reads and writes their sums at 4 TB/s and is a
-// launch more.  It takes 64 without a split for 1000 x 1000 -> 1000 in 16 bits (13.7 us; in four 20.8), 64 in 8 splits for 5001 x
-// 1000 -> 333 (21; 128 in 20: 26), 128 in 24 for 100000 x 777 -> 333 (113; 64: 180), and 64 in 4 for 2048 x 2048 -> 512 in fp32 (53; 128 in 8: 56).
+// Tile and splits of the rows: the pair whose estimate is least; the join of the splits reads and writes their sums at 4 TB/s and is a launch more.  It takes 64 without a split for 1000 x
+// 1000 -> 1000 in 16 bits (13.7 us; in four 20.8), 64 in 8 splits for 5001 x 1000 -> 333 (21; 128 in 20: 26), 128 in 24 for 100000 x 777 -> 333 (113; 64: 180), and 64 in 4 for 2048 x 2048
+// -> 512 in fp32 (53; 128 in 8: 56).
 static int linear_wgrad_plan(int64_t rows, int in, int out, int dtype, int* splits, int64_t* per) {
   const bool h = dtype != SH_F32;
   double best = 0.;
   int best_tile = 0;
   for (int tile = 64; tile <= 128; tile *= 2) {
-    const int kp = wgrad_rows(h, tile), most = tile == 64 ? 4 : 2;  // blocks on a CU
+    const int kp = wgrad_rows(h, tile), most = staged_on_cu(tile);
     const int64_t tiles = (int64_t)ceil_div(in, tile) * ceil_div(out, tile), steps = rows > 0 ? (rows + kp - 1) / kp : 1;
     for (int on_cu = 0; on_cu <= most; ++on_cu) {  // as many splits as put on_cu blocks on every CU, of at least 4 steps each; 0: no split
       int64_t sk = on_cu == 0 ? 1 : 256 * on_cu / tiles;
       if (sk > steps / 4) sk = steps / 4;
       if (sk < 1) sk = 1;
       const int64_t each = (steps + sk - 1) / sk, full = (sk * tiles + 255) / 256, rounds = (full + most - 1) / most;
-      const double b = (double)(full < most ? full : most);
-      const double t = tile == 64 ? (h ? (b <= 2 ? 0.36 + 0.015 * b : 0.165 * b) : 0.45 + 0.52 * b) : (h ? 0.51 + 0.09 * b : 0.46 + 0.89 * b);
+      const double t = staged_us(h, tile, (int)(full < most ? full : most)) * kp / 32;
       const double cost = (double)(rounds * each) * t + (sk > 1 ? 5. + (double)sk * in * out * 2e-6 : 0.);
       if (best_tile == 0 || cost < best) {
         best = cost;
