@@ -6,7 +6,7 @@
 //
 // linear_gemm_kernel (forward, and dx with w transposed first; rows at any element address): out [M][N] = a [M][K] b[N][K]^T, tiles of 128 x 128 or 64 x 64, 128 bytes of K a step, both
 // operands global -> registers -> LDS with the next step's loads in flight under the MFMAs (a second step in flight and a second buffer: no faster).
-// 100000 x 777 -> 333: bf16 138 us, fp32 548 (336 at the fp32 rate of a large matrix product).  The operands are swapped (b is the MFMA's first one), and b's rows are permuted inside
+// 100000 x 777 -> 333: bf16 125 us, fp32 535 (336 at the fp32 rate of a large matrix product).  The operands are swapped (b is the MFMA's first one), and b's rows are permuted inside
 // the tile, so that a lane ends with 8 consecutive columns of one row: bias, residual, pre-activation and output move as 16-byte vectors.
 // linear_wgrad_kernel: dw [N][K] = dz^T x, the reduction runs over rows: tiles of 64 or 128 squared over a range of rows (split), 16-bit operands are read transposed from LDS
 // (ds_read_b64_tr_b16); the splits' fp32 partial sums are added in a fixed order by a second launch.  100000 x 777 -> 333: bf16 113 us, fp32 608; 400000 x 64 -> 64 bf16 27;

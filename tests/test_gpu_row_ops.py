@@ -238,7 +238,7 @@ def test_linear_act_backward(dtype, rows, cols, act):
     close(db, want.sum(dim=0), (rows + 4) * U * want.abs().sum(dim=0) + fp.sum(dim=0) + 1e-30, "db")
 
 
-@pytest.mark.parametrize("m,k,n", SHAPES_LIN + [(5000, 64, 64), (4097, 40, 72), (1000, 256, 512), (2048, 520, 264), (70, 264, 1032), (5, 128, 136), (8200, 72, 200), (300, 1024, 776), (259, 820, 1024)])
+@pytest.mark.parametrize("m,k,n", SHAPES_LIN + [(33, 1, 1), (39, 3, 1), (65, 1, 9), (36, 2, 3), (8, 1, 1), (7, 500, 300), (6, 1, 3000), (5000, 64, 64), (4097, 40, 72), (1000, 256, 512), (2048, 520, 264), (70, 264, 1032), (5, 128, 136), (8200, 72, 200), (300, 1024, 776), (259, 820, 1024)])
 @pytest.mark.parametrize("act8", [False, True])
 def test_linear_backward(dtype, m, k, n, act8):
     from simhand_amd import ops
