@@ -190,3 +190,57 @@ def test_command_line(tmp_path):
               "--joints_type", "augmented", "--diff_type", "mpjpe", "--pos_neg", "pos_neg", "--synthetic", "--synthetic_samples", "24", "--image_size", "64", "--precision", "bf16",
               "--projection_head_norm", "layer", "--act8", "--max_steps", "3", "--out_dir", str(tmp_path)])
     assert t.global_step == 3 and all(torch.isfinite(torch.as_tensor(float(x))) for x in t.step_losses)
+
+
+def test_shared_operands_and_an_expanded_gradient():
+    """One weight in two places, x as input and residual, the gradient of a sum (stride 0): gradients add up as in 64 bits (terms of 12 x 90 U, as above)."""
+    from simhand_amd.host import model_utils as mu
+
+    x, w, b, g = randn(41, 24), randn(24, 24, seed=1, scale=0.3), randn(24, seed=2), 1 + 0.1 * randn(24, seed=3)
+    dev = [t.cuda().requires_grad_() for t in (x, w, b, g)]
+    h = mu.linear(dev[0], dev[1], dev[2], act="silu", residual=dev[0])
+    h = mu.layer_norm(h, dev[3], dev[2])
+    y = mu.linear(h, dev[1], residual=h)
+    y[:, 1:].square().sum().backward()
+    ref = [t.double().requires_grad_() for t in (x, w, b, g)]
+    z = ref[0] @ ref[1].t() + ref[2]
+    h = z * torch.sigmoid(z) + ref[0]
+    h = torch.nn.functional.layer_norm(h, (24,), ref[3], ref[2], 1e-5)
+    want = h @ ref[1].t() + h
+    want[:, 1:].square().sum().backward()
+    for a, c in zip(dev, ref):
+        assert float((a.grad.double().cpu() - c.grad).norm()) <= 12 * 90 * U * float(c.grad.norm()) * 4  # (three layers and the square carry one another's rounding)
+    dev[0].grad = None
+    mu.linear(dev[0], dev[1]).sum().backward()  # an expanded gradient
+    ones = torch.ones(41, 24, dtype=torch.float64) @ w.double()
+    assert float((dev[0].grad.double().cpu() - ones).norm()) <= 12 * 24 * U * float(ones.norm())
+
+
+def test_captured_forward_and_backward():
+    """Values and gradients of a block in one graph, replayed with new inputs between eager passes over the same leaves: bit for bit the eager ones."""
+    from simhand_amd.host import model_utils as mu
+
+    x, w, b, g, w2, dy = (t.cuda() for t in (randn(300, 40), randn(72, 40, seed=1), randn(72, seed=2), 1 + 0.1 * randn(72, seed=3), randn(40, 72, seed=4), randn(300, 40, seed=5)))
+    leaves = [t.requires_grad_() for t in (x, w, b, g, w2)]
+
+    def block():
+        h = mu.layer_norm(mu.linear(x, w, b, act="gelu", act8=True), g, b, relu=True, act8=True)
+        y = mu.linear(h, w2, residual=x)
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        block()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = block()
+    for s in range(3):
+        with torch.no_grad():
+            x.copy_(randn(300, 40, seed=20 + s))
+        eager = [t.clone() for t in block()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, eager)), s
