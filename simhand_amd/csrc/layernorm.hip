@@ -7,13 +7,13 @@
 // One pass over the data each way: a group of G lanes holds a whole row in registers (NV 16-byte vectors per lane), so the variance is summed about
 // the finished mean (no E[x^2] - m^2 cancellation) and nothing is read twice.  Statistics and sums are fp32, the column sums over row blocks are
 // folded in 64 bits in a fixed order (bit-reproducible).  Bound by HBM: 2 (3) elements of traffic per element forward (backward).
-// Measured: forward 100352 x 2048 bf16 154 us (5.3 TB/s; a large copy reaches 4.9), 256 x 512 fp32 3.1 (11 with the call around it); backward 33001 x 777 fp16 from codes 38 + 4 for the
-// fold (2.7 TB/s: a ragged row costs more arithmetic than its bytes take), 2048 x 512 fp32 with ReLU 5.8 + 3.4.
+// Measured: forward 100352 x 2048 bf16 154 us (5.3 TB/s; a large copy reaches 4.9), 256 x 512 fp32 3.1 (11 with the call around it); backward 33001 x 777 fp16 from codes 34 + 4 for the
+// fold (2.9 TB/s: a ragged row costs more arithmetic than its bytes take), 2048 x 512 fp32 with ReLU 5.8 + 3.4.
 #include "rows.h"
 
 namespace sh {
 
-// sums of two values over the G lanes that share a row (G = 16 or 64: inside a wave, on DPP and the row swaps -- no LDS round trips; G = 256: the whole block through
+// sums of two values over the G lanes that share a row (G = 16, 32 or 64: inside a wave, on DPP and the row swaps -- no LDS round trips; G = 256: the whole block through
 // LDS), the same bits in every lane
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
   return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
@@ -31,10 +31,8 @@ template <int G> __device__ __forceinline__ void group_sum2(float& a, float& b, 
   a = dpp_add<0x4E>(a); b = dpp_add<0x4E>(b);      // 2, 3, 0, 1
   a = dpp_add<0x141>(a); b = dpp_add<0x141>(b);    // mirrored in every eight
   a = dpp_add<0x140>(a); b = dpp_add<0x140>(b);    // mirrored in every sixteen
-  if constexpr (G >= 64) {
-    a = swap16_add(a); b = swap16_add(b);
-    a = swap32_add(a); b = swap32_add(b);
-  }
+  if constexpr (G >= 32) { a = swap16_add(a); b = swap16_add(b); }
+  if constexpr (G >= 64) { a = swap32_add(a); b = swap32_add(b); }
   if constexpr (G == 256) {
     __syncthreads();  // the previous use of red is over
     if ((threadIdx.x & 63) == 0) {
@@ -56,38 +54,34 @@ __device__ __forceinline__ float ln_affine(float x, float m, float r, float g, f
   return t + b;
 }
 
-// Vector i of lane t: columns at .. at + N - 1, of which lo .. hi - 1 count.  RAG (cols no multiple of the vector): the last vector of a row is moved back to end with the
-// row -- one whole load and store, the columns it shares with its neighbour are written twice with the same values and counted once (lo); rows shorter than
-// a vector go element by element (hi).
-template <int N, bool RAG> struct LnVec {
+// Vector i of lane t: columns at .. at + N - 1, of which lo .. hi - 1 count.  RAG = 1 (cols no multiple of the vector): the last vector of a row is moved back to end with the
+// row -- one whole load and store, the columns it shares with its neighbour are written twice with the same values and counted once (lo).  RAG = 2: rows shorter than
+// a vector go element by element (hi); a variant of its own: inlined into the loops of RAG = 1 its branches make them ten times as long (33001 x 777 from codes 38 us, without 34).
+template <int N, int RAG> struct LnVec {
   int at, lo, hi;
   bool on;
   __device__ __forceinline__ LnVec(int c, int cols) : at(c), lo(0), hi(N), on(c < cols) {
-    if constexpr (RAG) {
+    if constexpr (RAG == 1) {
       if (c + N > cols) {
-        if (cols >= N) {
-          at = cols - N;
-          lo = c - at;
-        } else {
-          at = 0;
-          hi = cols;
-        }
+        at = cols - N;
+        lo = c - at;
       }
     }
+    if constexpr (RAG == 2) hi = cols;
   }
-  __device__ __forceinline__ bool counts(int e) const { return !RAG || (e >= lo && e < hi); }
+  __device__ __forceinline__ bool counts(int e) const { return RAG == 0 || (RAG == 1 ? e >= lo : e < hi); }
   template <typename T> __device__ __forceinline__ uint4 load(const T* row) const {
-    if constexpr (RAG) return ld_chunk<T>(row + at, hi);
+    if constexpr (RAG == 2) return ld_chunk<T>(row + at, hi);
     return ld16_any(row + at);
   }
   template <typename T> __device__ __forceinline__ void store(T* row, const uint4& v) const {
-    if constexpr (RAG) st_chunk<T>(row + at, hi, v);
+    if constexpr (RAG == 2) st_chunk<T>(row + at, hi, v);
     else st16_any(row + at, v);
   }
-  __device__ __forceinline__ void load_f32(const float* p, float (&o)[N]) const { ld_f32<N>(p + at, RAG ? hi : N, o); }
+  __device__ __forceinline__ void load_f32(const float* p, float (&o)[N]) const { ld_f32<N>(p + at, RAG == 2 ? hi : N, o); }
 };
 
-template <typename T, int G, int NV, bool RAG>
+template <typename T, int G, int NV, int RAG>
 __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta,
                                                              float eps, int relu, T* __restrict__ y, float* __restrict__ mean,
                                                              float* __restrict__ rstd, long long rows, int cols) {
@@ -153,8 +147,8 @@ __host__ __device__ constexpr int ln_bwd_occupancy(int nv, bool fp32, bool rag) 
   return nv <= 1 ? 6 : nv <= 2 ? (rag ? 3 : 4) : nv <= 4 ? 2 : 1;
 }
 
-template <typename T, int G, int NV, bool A8, bool RAG, bool GATE>
-__global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG)) void layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
+template <typename T, int G, int NV, bool A8, int RAG, bool GATE>
+__global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG != 0)) void layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
                                                              const uint8_t* __restrict__ exps, const float* __restrict__ gamma,
                                                              const float* __restrict__ beta, const float* __restrict__ mean,
                                                              const float* __restrict__ rstd, T* __restrict__ dx,
@@ -194,10 +188,10 @@ __global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG)) voi
       if (!w.on) continue;
       qd[i] = w.template load<T>(dy + rr * cols);
       if constexpr (A8) {
-        act8_ld_codes<VE>(codes + rr * cols + w.at, RAG ? w.hi : VE, qc[i]);
+        act8_ld_codes<VE>(codes + rr * cols + w.at, RAG == 2 ? w.hi : VE, qc[i]);
         const uint8_t* ex = exps + rr * eb;
         qe[i] = ex[w.at / kAct8Block];
-        if constexpr (RAG) qe[i] |= (unsigned)ex[(w.at + w.hi - 1) / kAct8Block] << 8;
+        if constexpr (RAG == 1) qe[i] |= (unsigned)ex[(w.at + VE - 1) / kAct8Block] << 8;
       } else {
         qx[i] = w.template load<T>(x + rr * cols);
       }
@@ -209,7 +203,7 @@ __global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG)) voi
   for (long long row0 = first; row0 < rows; row0 += stride) {
     const long long row = row0 + sub;
     const bool live = row < rows;
-    const float m = qm, r = qr;
+    const float m = qm, r = qr, mr = m * r;
     float h[NV][VE], u[NV][VE];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -220,7 +214,7 @@ __global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG)) voi
         const float s0 = act8_scale(qe[i] & 0xffu);
 #pragma unroll
         for (int k = 0; k < W8; ++k) act8_decode4(qc[i][k], s0, &h[i][4 * k]);
-        if constexpr (RAG) {  // a vector that was moved back may span two blocks of 32
+        if constexpr (RAG == 1) {  // a vector that was moved back may span two blocks of 32
           const int edge = kAct8Block - w.at % kAct8Block;
           if (edge < VE) {
             const float s1 = act8_scale(qe[i] >> 8);
@@ -259,20 +253,20 @@ __global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG)) voi
         if constexpr (GATE) {
           if (!(ln_affine(h[i][e], m, r, ga[e], be[e], h[i][e]) > 0.f)) u[i][e] = 0.f;
         } else {
-          h[i][e] = (h[i][e] - m) * r;
+          h[i][e] = fmaf(h[i][e], r, -mr);  // off by U of |m r| more than (x - m) r, which the mean's own rounding costs already
         }
-        const float uc = RAG && 2 * i >= NV - 1 ? (w.counts(e) ? u[i][e] : 0.f) : u[i][e];
+        const float uc = RAG != 0 && 2 * i >= NV - 1 ? (w.counts(e) ? u[i][e] : 0.f) : u[i][e];
         const float gc = uc * ga[e];
         ag[i][e] += uc * h[i][e];
         ab[i][e] += uc;
         s1 += gc;
         s2 += gc * h[i][e];
-        u[i][e] = RAG && 2 * i >= NV - 1 ? u[i][e] * ga[e] : gc;
+        u[i][e] = RAG != 0 && 2 * i >= NV - 1 ? u[i][e] * ga[e] : gc;
       }
     }
     group_sum2<G>(s1, s2, red);
-    s1 *= inv;
-    s2 *= inv;
+    s1 *= inv * r;
+    s2 *= inv * r;
     if (!live) continue;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -280,7 +274,7 @@ __global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG)) voi
       if (!w.on) continue;
       float o[VE];
 #pragma unroll
-      for (int e = 0; e < VE; ++e) o[e] = r * (u[i][e] - s1 - h[i][e] * s2);
+      for (int e = 0; e < VE; ++e) o[e] = fmaf(r, u[i][e], -fmaf(h[i][e], s2, s1));  // r (g - mean(g) - h mean(g h))
       w.template store<T>(dx + row * cols, pack16<T>(o));
     }
   }
@@ -354,8 +348,9 @@ int fold_columns(const float* part, int nblk, int n, float* out, hipStream_t s) 
 
 // (G, NV) by the row's 16-byte vectors: the smallest group that holds the row
 static int ln_nvec(int cols, int dtype) { return (cols + (dtype == SH_F32 ? 4 : 8) - 1) / (dtype == SH_F32 ? 4 : 8); }
+static int ln_rag(int cols, int dtype) { return cols % (dtype == SH_F32 ? 4 : 8) == 0 ? 0 : cols >= (dtype == SH_F32 ? 4 : 8) ? 1 : 2; }
 constexpr int kLnMaxVec = 2048;
-static int ln_rows_per_block(int nvec) { return nvec <= 16 ? 16 : nvec <= 256 ? 4 : 1; }
+static int ln_rows_per_block(int nvec) { return nvec <= 16 ? 16 : nvec <= 32 ? 8 : nvec <= 256 ? 4 : 1; }
 static int ln_nv(int nvec) { return nvec <= 64 ? 1 : nvec <= 128 ? 2 : nvec <= 256 ? 4 : nvec <= 512 ? 2 : nvec <= 1024 ? 4 : 8; }
 // backward blocks: one round of what the CUs hold (each then walks its share of the rows with the next row in flight; a second, part-empty round cost a third of the
 // pass over 33001 x 777), and no more partial sums than that
@@ -369,6 +364,7 @@ static int ln_bwd_blocks(int64_t rows, int cols, int dtype) {
 
 #define SH_LN_DISPATCH(CALL)          \
   if (nvec <= 16) { CALL(16, 1); }    \
+  else if (nvec <= 32) { CALL(32, 1); }   \
   else if (nvec <= 64) { CALL(64, 1); }   \
   else if (nvec <= 128) { CALL(64, 2); }  \
   else if (nvec <= 256) { CALL(64, 4); }  \
@@ -395,21 +391,26 @@ int simhand_layer_norm_fwd(const void* x, const float* gamma, const float* beta,
   const int64_t most = (1ll << 23) * rpb;  // rows of a launch: its threads are counted in 32 bits
   hipStream_t s = (hipStream_t)stream;
   ProfScope ps(SH_PROF_BN, s, 0, 2.0 * rows * cols * (dtype == SH_F32 ? 4 : 2));
-  const bool rag = cols % (dtype == SH_F32 ? 4 : 8) != 0;
+  const int rag = ln_rag(cols, dtype);
 #define SH_ONE(T, G, NV, RAG) \
   layer_norm_fwd_kernel<T, G, NV, RAG><<<grid, 256, 0, s>>>((const T*)x + r * cols, gamma, beta, eps, relu, (T*)y + r * cols, mean + r, rstd + r, n, cols)
 #define SH_CALL(G, NV)                       \
   if (dtype == SH_F32) {                     \
-    if (rag) SH_ONE(float, G, NV, true);     \
-    else SH_ONE(float, G, NV, false);        \
+    if (rag) SH_ONE(float, G, NV, 1);        \
+    else SH_ONE(float, G, NV, 0);            \
   } else {                                   \
-    if (rag) SH_ONE(bf16_t, G, NV, true);    \
-    else SH_ONE(bf16_t, G, NV, false);       \
+    if (rag) SH_ONE(bf16_t, G, NV, 1);       \
+    else SH_ONE(bf16_t, G, NV, 0);           \
   }
   for (int64_t r = 0; r < rows; r += most) {
     const int64_t n = rows - r < most ? rows - r : most;
     const unsigned grid = (unsigned)((n + rpb - 1) / rpb);
-    SH_LN_DISPATCH(SH_CALL)
+    if (rag == 2) {
+      if (dtype == SH_F32) SH_ONE(float, 16, 1, 2);
+      else SH_ONE(bf16_t, 16, 1, 2);
+    } else {
+      SH_LN_DISPATCH(SH_CALL)
+    }
   }
 #undef SH_CALL
 #undef SH_ONE
@@ -438,7 +439,7 @@ int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes
   const double eb = dtype == SH_F32 ? 4 : 2;
   ProfScope ps(SH_PROF_BN, s, 0, (double)rows * cols * (2 * eb + (a8 ? 1.03125 : eb)));
   float* part = grid == 1 ? dgamma_dbeta : (float*)workspace;
-  const bool rag = cols % (dtype == SH_F32 ? 4 : 8) != 0;
+  const int rag = ln_rag(cols, dtype);
 #define SH_LAUNCH(T, G, NV, A8, RAG, GATE)                                                                                                           \
   layer_norm_bwd_kernel<T, G, NV, A8, RAG, GATE><<<grid, 256, 0, s>>>((const T*)dy, (const T*)x, x_codes, x_exps, gamma, beta, mean, rstd, (T*)dx, part, \
                                                                       rows, cols)
@@ -447,11 +448,11 @@ int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes
   else SH_LAUNCH(T, G, NV, A8, RAG, false)
 #define SH_TYPE(T, G, NV)                       \
   if (a8) {                                     \
-    if (rag) { SH_ONE(T, G, NV, true, true); }  \
-    else { SH_ONE(T, G, NV, true, false); }     \
+    if (rag) { SH_ONE(T, G, NV, true, 1); }     \
+    else { SH_ONE(T, G, NV, true, 0); }         \
   } else {                                      \
-    if (rag) { SH_ONE(T, G, NV, false, true); } \
-    else { SH_ONE(T, G, NV, false, false); }    \
+    if (rag) { SH_ONE(T, G, NV, false, 1); }    \
+    else { SH_ONE(T, G, NV, false, 0); }        \
   }
 #define SH_CALL(G, NV)                        \
   if (dtype == SH_F32) {                      \
@@ -459,7 +460,16 @@ int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes
   } else {                                    \
     SH_TYPE(bf16_t, G, NV)                    \
   }
-  SH_LN_DISPATCH(SH_CALL)
+#define SH_SHORT(T)                        \
+  if (a8) { SH_ONE(T, 16, 1, true, 2); }   \
+  else { SH_ONE(T, 16, 1, false, 2); }
+  if (rag == 2) {
+    if (dtype == SH_F32) { SH_SHORT(float) }
+    else { SH_SHORT(bf16_t) }
+  } else {
+    SH_LN_DISPATCH(SH_CALL)
+  }
+#undef SH_SHORT
 #undef SH_CALL
 #undef SH_TYPE
 #undef SH_ONE

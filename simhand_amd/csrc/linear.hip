@@ -361,24 +361,30 @@ __global__ __launch_bounds__(256) void linear_act_bwd_kernel(const T* __restrict
   float s[VE];
 #pragma unroll
   for (int e = 0; e < VE; ++e) s[e] = 0.f;
-  if (c < cols) {
-    const int left = cols - c;
+  // a row's ragged last vector is read moved back, as the row's last VE columns; what it shares with its neighbour is neither summed nor stored (dz may be dy)
+  const int left = cols - c, gone = left < VE && cols >= VE ? VE - left : 0;
+  if (left > 0) {
     for (long long r = r0 + ty; r < r1; r += TY) {
+      const long long at = r * cols + c;
       float d[VE];
-      unpack16<T>(ld_chunk<T>(dy + r * cols + c, left), d);
+      unpack16<T>(cols >= VE ? ld16_any(dy + at - gone) : ld_chunk<T>(dy + at, left), d);
       if (act != SH_ACT_NONE) {
         float z[VE];
-        unpack16<T>(ld_chunk<T>(pre + r * cols + c, left), z);
+        unpack16<T>(cols >= VE ? ld16_any(pre + at - gone) : ld_chunk<T>(pre + at, left), z);
 #pragma unroll
         for (int e = 0; e < VE; ++e) d[e] *= act_slope(z[e], act);
       }
 #pragma unroll
       for (int e = 0; e < VE; ++e) s[e] += d[e];
-      if (dz != nullptr) st_chunk<T>(dz + r * cols + c, left, pack16<T>(d));
+      if (dz != nullptr) {
+        if (gone == 0) st_chunk<T>(dz + at, left, pack16<T>(d));
+        else st_chunk<T>(dz + at, left, move_down<T>(pack16<T>(d), gone));
+      }
     }
   }
 #pragma unroll
-  for (int e = 0; e < VE; ++e) red[ty][tx * VE + e] = s[e];
+  for (int e = 0; e < VE; ++e)
+    if (e >= gone) red[ty][tx * VE + e - gone] = s[e];
   __syncthreads();
   for (int i = threadIdx.x; i < TX * VE; i += 256) {
     const int col = blockIdx.x * TX * VE + i;

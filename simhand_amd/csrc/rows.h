@@ -143,11 +143,11 @@ template <int N> __device__ __forceinline__ void ld_f32(const float* p, int left
 // ---- 8-bit activations: value = e4m3(code) * 2^(exp - 127), one exp byte (1 .. 247) for 32 consecutive columns of a row ------------------
 constexpr int kAct8Block = 32;
 __device__ __forceinline__ float act8_scale(unsigned exp) { return __uint_as_float(exp << 23); }
-// four codes of one word
+// four codes of one word, by gfx950's scaled conversion (exact: the scale is a power of two)
 __device__ __forceinline__ void act8_decode4(unsigned w, float scale, float* o) {
-  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
-  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-  o[0] = lo[0] * scale; o[1] = lo[1] * scale; o[2] = hi[0] * scale; o[3] = hi[1] * scale;
+  const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, false);
+  const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, true);
+  o[0] = lo[0]; o[1] = lo[1]; o[2] = hi[0]; o[3] = hi[1];
 }
 // eight codes (two words) -> a 16-byte chunk of the build's 16-bit type, by gfx950's scaled conversion: the scale's exponent is added to the code's, one rounding to nearest even (none
 // for bf16).  A quarter of the instructions of decode + pack.
