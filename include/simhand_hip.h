@@ -615,6 +615,15 @@ size_t simhand_layer_norm_bwd_workspace_bytes(int64_t rows, int cols, int dtype)
 int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, const float* gamma, const float* beta,
                            const float* mean, const float* rstd, int relu, void* dx, float* dgamma_dbeta, int64_t rows, int cols, int dtype,
                            void* workspace, size_t workspace_bytes, sh_stream_t stream);
+/* The same with the ReLU's gate kept by the forward call (gate = NULL: exactly the two above; a gate needs relu != 0).  gate [rows][ceil(cols / V)] bytes, V = 8 in 16 bits, 4 in fp32:
+ * bit e of a row's byte i says that column V i + e passed (h gamma + beta > 0); in the last byte of a row that V does not divide it is column cols - V + e (cols < V: column e).
+ * A backward call without it recomputes the gate from x: the forward's own from the tensor, but from an 8-bit checkpoint a gate that flips wherever the codes' rounding carries
+ * h gamma + beta across zero. */
+int simhand_layer_norm_fwd_ex(const void* x, const float* gamma, const float* beta, float eps, int relu, void* y, uint8_t* gate, float* mean, float* rstd,
+                              int64_t rows, int cols, int dtype, sh_stream_t stream);
+int simhand_layer_norm_bwd_ex(const void* dy, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, const float* gamma, const float* beta,
+                              const float* mean, const float* rstd, int relu, const uint8_t* gate, void* dx, float* dgamma_dbeta, int64_t rows, int cols,
+                              int dtype, void* workspace, size_t workspace_bytes, sh_stream_t stream);
 
 /* z = x w^T + bias, y = act(z) + residual; x [rows][in_dim], w [out_dim][in_dim], bias fp32 [out_dim] or NULL, residual [rows][out_dim] or NULL,
  * pre [rows][out_dim] or NULL receives z (what simhand_linear_act_bwd takes).  residual may be y's own buffer.  Workspace query, here and below: aligned = every operand (x, w,

@@ -245,6 +245,8 @@ SIGNATURES = {
     "simhand_layer_norm_fwd": (_I, [_P, _P, _P, _F, _I, _P, _P, _P, _L, _I, _I, _P]),
     "simhand_layer_norm_bwd_workspace_bytes": (_S, [_L, _I, _I]),
     "simhand_layer_norm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _L, _I, _I, _P, _S, _P]),
+    "simhand_layer_norm_fwd_ex": (_I, [_P, _P, _P, _F, _I, _P, _P, _P, _P, _L, _I, _I, _P]),
+    "simhand_layer_norm_bwd_ex": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _L, _I, _I, _P, _S, _P]),
     "simhand_linear_fwd_workspace_bytes": (_S, [_L, _I, _I, _I, _I]),
     "simhand_linear_fwd": (_I, [_P, _P, _P, _I, _P, _P, _P, _L, _I, _I, _I, _P, _S, _P]),
     "simhand_linear_act_bwd_workspace_bytes": (_S, [_L, _I, _I]),

@@ -70,6 +70,7 @@ template <int N, int RAG> struct LnVec {
     if constexpr (RAG == 2) hi = cols;
   }
   __device__ __forceinline__ bool counts(int e) const { return RAG == 0 || (RAG == 1 ? e >= lo : e < hi); }
+  __device__ __forceinline__ bool exists(int e) const { return RAG != 2 || e < hi; }
   template <typename T> __device__ __forceinline__ uint4 load(const T* row) const {
     if constexpr (RAG == 2) return ld_chunk<T>(row + at, hi);
     return ld16_any(row + at);
@@ -83,7 +84,7 @@ template <int N, int RAG> struct LnVec {
 
 template <typename T, int G, int NV, int RAG>
 __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta,
-                                                             float eps, int relu, T* __restrict__ y, float* __restrict__ mean,
+                                                             float eps, int relu, T* __restrict__ y, uint8_t* __restrict__ gate, float* __restrict__ mean,
                                                              float* __restrict__ rstd, long long rows, int cols) {
   constexpr int VE = Vec16<T>::N, RB = 256 / G;
   __shared__ float red[4][2];
@@ -133,13 +134,24 @@ __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(const T* __restrict
     for (int e = 0; e < VE; ++e) {
       float h;
       o[e] = ln_affine(v[i][e], m, r, ga[e], be[e], h);
-      if (relu) o[e] = o[e] <= 0.f ? 0.f : o[e];
+    }
+    if (gate != nullptr) {  // bit e of the vector's byte: what the ReLU lets through
+      unsigned bits = 0u;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) bits |= w.exists(e) && o[e] > 0.f ? 1u << e : 0u;
+      gate[row * ((cols + VE - 1) / VE) + i * G + t] = (uint8_t)bits;
+    }
+    if (relu) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) o[e] = o[e] <= 0.f ? 0.f : o[e];
     }
     w.template store<T>(dst, pack16<T>(o));
   }
 }
 
-// A8: x comes as its 8-bit checkpoint (codes + exponents).  part [gridDim.x][2][cols]: sums of u h and u over the block's rows.
+// A8: x comes as its 8-bit checkpoint (codes + exponents).  GATE: 0 no ReLU, 1 its gate recomputed from x, 2 the gate that the forward pass kept (one byte a vector, laid out as
+// there): from codes the recomputed sign is wrong wherever the codes' rounding carries a value across zero -- a whole gradient let through or lost, not a rounding of one.
+// part [gridDim.x][2][cols]: sums of u h and u over the block's rows.
 // A row group walks its rows with the next row's loads in flight; gamma and beta wait in LDS (G < 256), which the column sums reuse at the end.
 // blocks of the backward kernel per CU, by the values a lane holds (registers); the grid is as many as run at once
 __host__ __device__ constexpr int ln_bwd_occupancy(int nv, bool fp32, bool rag) {
@@ -147,11 +159,11 @@ __host__ __device__ constexpr int ln_bwd_occupancy(int nv, bool fp32, bool rag) 
   return nv <= 1 ? 6 : nv <= 2 ? (rag ? 3 : 4) : nv <= 4 ? 2 : 1;
 }
 
-template <typename T, int G, int NV, bool A8, int RAG, bool GATE>
+template <typename T, int G, int NV, bool A8, int RAG, int GATE>
 __global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG != 0)) void layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
                                                              const uint8_t* __restrict__ exps, const float* __restrict__ gamma,
                                                              const float* __restrict__ beta, const float* __restrict__ mean,
-                                                             const float* __restrict__ rstd, T* __restrict__ dx,
+                                                             const float* __restrict__ rstd, const uint8_t* __restrict__ gate, T* __restrict__ dx,
                                                              float* __restrict__ part, long long rows, int cols) {
   constexpr int VE = Vec16<T>::N, RB = 256 / G, W8 = VE / 4;
   constexpr bool GLOBAL = G == 256;  // wide rows: gamma / beta come from the caches
@@ -176,6 +188,7 @@ __global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG != 0)
   uint4 qd[NV], qx[A8 ? 1 : NV];
   unsigned qc[A8 ? NV : 1][W8];
   unsigned qe[A8 ? NV : 1];  // exponents of the vector's first and last column
+  unsigned qg[GATE == 2 ? NV : 1];
   float qm, qr;
   auto fetch = [&](long long row) __attribute__((always_inline)) {
     const bool live = row < rows;
@@ -187,6 +200,7 @@ __global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG != 0)
       const LnVec<VE, RAG> w((i * G + t) * VE, cols);
       if (!w.on) continue;
       qd[i] = w.template load<T>(dy + rr * cols);
+      if constexpr (GATE == 2) qg[i] = gate[rr * ((cols + VE - 1) / VE) + i * G + t];
       if constexpr (A8) {
         act8_ld_codes<VE>(codes + rr * cols + w.at, RAG == 2 ? w.hi : VE, qc[i]);
         const uint8_t* ex = exps + rr * eb;
@@ -210,6 +224,10 @@ __global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG != 0)
       const LnVec<VE, RAG> w((i * G + t) * VE, cols);
       if (!w.on) continue;
       unpack16<T>(qd[i], u[i]);
+      if constexpr (GATE == 2) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) u[i][e] = qg[i] >> e & 1u ? u[i][e] : 0.f;
+      }
       if constexpr (A8) {
         const float s0 = act8_scale(qe[i] & 0xffu);
 #pragma unroll
@@ -240,17 +258,17 @@ __global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG != 0)
       float ga[VE], be[VE];
       if constexpr (GLOBAL) {
         w.load_f32(gamma, ga);
-        if constexpr (GATE) w.load_f32(beta, be);
+        if constexpr (GATE == 1) w.load_f32(beta, be);
       } else {
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           ga[e] = fold[0][w.at + e];
-          if constexpr (GATE) be[e] = fold[1][w.at + e];
+          if constexpr (GATE == 1) be[e] = fold[1][w.at + e];
         }
       }
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        if constexpr (GATE) {
+        if constexpr (GATE == 1) {
           if (!(ln_affine(h[i][e], m, r, ga[e], be[e], h[i][e]) > 0.f)) u[i][e] = 0.f;
         } else {
           h[i][e] = fmaf(h[i][e], r, -mr);  // off by U of |m r| more than (x - m) r, which the mean's own rounding costs already
@@ -380,11 +398,17 @@ extern "C" {
 
 int simhand_layer_norm_fwd(const void* x, const float* gamma, const float* beta, float eps, int relu, void* y, float* mean, float* rstd, int64_t rows,
                            int cols, int dtype, sh_stream_t stream) {
+  return simhand_layer_norm_fwd_ex(x, gamma, beta, eps, relu, y, nullptr, mean, rstd, rows, cols, dtype, stream);
+}
+
+int simhand_layer_norm_fwd_ex(const void* x, const float* gamma, const float* beta, float eps, int relu, void* y, uint8_t* gate, float* mean, float* rstd,
+                              int64_t rows, int cols, int dtype, sh_stream_t stream) {
   SH_REQUIRE(dtype == SH_F32 || dtype == SH_BF16, "layer_norm_fwd: dtype %d", dtype);
   SH_REQUIRE(rows >= 0 && cols >= 1 && ln_nvec(cols, dtype) <= kLnMaxVec, "layer_norm_fwd: rows=%lld cols=%d (at most %d columns)", (long long)rows, cols,
              kLnMaxVec * (dtype == SH_F32 ? 4 : 8));
   SH_REQUIRE(gamma && beta && (rows == 0 || (x && y && mean && rstd)), "layer_norm_fwd: NULL argument");
   SH_REQUIRE(eps >= 0.f, "layer_norm_fwd: eps < 0");
+  SH_REQUIRE(!gate || relu, "layer_norm_fwd: a gate without the ReLU");
   if (rows == 0) return 0;
   const int nvec = ln_nvec(cols, dtype);
   const int rpb = ln_rows_per_block(nvec);
@@ -393,7 +417,8 @@ int simhand_layer_norm_fwd(const void* x, const float* gamma, const float* beta,
   ProfScope ps(SH_PROF_BN, s, 0, 2.0 * rows * cols * (dtype == SH_F32 ? 4 : 2));
   const int rag = ln_rag(cols, dtype);
 #define SH_ONE(T, G, NV, RAG) \
-  layer_norm_fwd_kernel<T, G, NV, RAG><<<grid, 256, 0, s>>>((const T*)x + r * cols, gamma, beta, eps, relu, (T*)y + r * cols, mean + r, rstd + r, n, cols)
+  layer_norm_fwd_kernel<T, G, NV, RAG><<<grid, 256, 0, s>>>((const T*)x + r * cols, gamma, beta, eps, relu, (T*)y + r * cols, \
+                                                      gate ? gate + r * nvec : nullptr, mean + r, rstd + r, n, cols)
 #define SH_CALL(G, NV)                       \
   if (dtype == SH_F32) {                     \
     if (rag) SH_ONE(float, G, NV, 1);        \
@@ -426,11 +451,18 @@ size_t simhand_layer_norm_bwd_workspace_bytes(int64_t rows, int cols, int dtype)
 int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, const float* gamma, const float* beta,
                            const float* mean, const float* rstd, int relu, void* dx, float* dgamma_dbeta, int64_t rows, int cols, int dtype,
                            void* workspace, size_t workspace_bytes, sh_stream_t stream) {
+  return simhand_layer_norm_bwd_ex(dy, x, x_codes, x_exps, gamma, beta, mean, rstd, relu, nullptr, dx, dgamma_dbeta, rows, cols, dtype, workspace, workspace_bytes, stream);
+}
+
+int simhand_layer_norm_bwd_ex(const void* dy, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, const float* gamma, const float* beta,
+                              const float* mean, const float* rstd, int relu, const uint8_t* gate, void* dx, float* dgamma_dbeta, int64_t rows, int cols,
+                              int dtype, void* workspace, size_t workspace_bytes, sh_stream_t stream) {
   SH_REQUIRE(dtype == SH_F32 || dtype == SH_BF16, "layer_norm_bwd: dtype %d", dtype);
   SH_REQUIRE(rows >= 0 && cols >= 1 && ln_nvec(cols, dtype) <= kLnMaxVec, "layer_norm_bwd: rows=%lld cols=%d (at most %d columns)", (long long)rows, cols,
              kLnMaxVec * (dtype == SH_F32 ? 4 : 8));
   const bool a8 = x_codes != nullptr;
   SH_REQUIRE(!a8 || (x_exps && !x), "layer_norm_bwd: pass either x or its codes and exponents");
+  SH_REQUIRE(!gate || relu, "layer_norm_bwd: a gate without the ReLU");
   SH_REQUIRE(gamma && beta && dgamma_dbeta && (rows == 0 || (dy && (x || a8) && mean && rstd && dx)), "layer_norm_bwd: NULL argument");
   const int nvec = ln_nvec(cols, dtype);
   const int grid = ln_bwd_blocks(rows, cols, dtype);
@@ -441,11 +473,12 @@ int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes
   float* part = grid == 1 ? dgamma_dbeta : (float*)workspace;
   const int rag = ln_rag(cols, dtype);
 #define SH_LAUNCH(T, G, NV, A8, RAG, GATE)                                                                                                           \
-  layer_norm_bwd_kernel<T, G, NV, A8, RAG, GATE><<<grid, 256, 0, s>>>((const T*)dy, (const T*)x, x_codes, x_exps, gamma, beta, mean, rstd, (T*)dx, part, \
+  layer_norm_bwd_kernel<T, G, NV, A8, RAG, GATE><<<grid, 256, 0, s>>>((const T*)dy, (const T*)x, x_codes, x_exps, gamma, beta, mean, rstd, gate, (T*)dx, part, \
                                                                       rows, cols)
-#define SH_ONE(T, G, NV, A8, RAG)               \
-  if (relu) SH_LAUNCH(T, G, NV, A8, RAG, true); \
-  else SH_LAUNCH(T, G, NV, A8, RAG, false)
+#define SH_ONE(T, G, NV, A8, RAG)                 \
+  if (gate) SH_LAUNCH(T, G, NV, A8, RAG, 2);      \
+  else if (relu) SH_LAUNCH(T, G, NV, A8, RAG, 1); \
+  else SH_LAUNCH(T, G, NV, A8, RAG, 0)
 #define SH_TYPE(T, G, NV)                       \
   if (a8) {                                     \
     if (rag) { SH_ONE(T, G, NV, true, 1); }     \

@@ -141,16 +141,17 @@ class _LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, gamma, beta, eps, relu, act8):
         x = x.contiguous()
         g, b = gamma.detach().float().contiguous(), beta.detach().float().contiguous()
-        y, mean, rstd = ops.layer_norm_fwd(x, g, b, eps, relu)
-        _keep(ctx, x, act8, g, b, mean, rstd)
+        # from the codes alone the backward pass could not tell what the ReLU let through (a rounding may cross zero): its gate is kept, one bit a value
+        y, *stats = ops.layer_norm_fwd(x, g, b, eps, relu, want_gate=relu and act8)
+        _keep(ctx, x, act8, g, b, *stats)
         ctx.relu, ctx.dtypes = relu, (gamma.dtype, beta.dtype)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, (g, b, mean, rstd) = _kept(ctx)
-        dx, dg, db = ops.layer_norm_bwd(dy.to(ctx.x_dtype).contiguous(), x, g, b, mean, rstd, ctx.relu)
+        x, (g, b, mean, rstd, *gate) = _kept(ctx)
+        dx, dg, db = ops.layer_norm_bwd(dy.to(ctx.x_dtype).contiguous(), x, g, b, mean, rstd, ctx.relu, *gate)
         return dx, dg.to(ctx.dtypes[0]), db.to(ctx.dtypes[1]), None, None, None
 
 

@@ -269,24 +269,38 @@ def _scratch(nbytes: int, x) -> torch.Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=x.device)
 
 
-def layer_norm_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps: float = 1e-5, relu: bool = False):
+def layer_norm_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps: float = 1e-5, relu: bool = False, want_gate: bool = False):
     """(y, mean, rstd): y = (x - mean) * rstd * gamma + beta over the last dimension (relu: max(y, 0)); gamma, beta fp32 [cols]; mean, rstd fp32,
-    one per row, for layer_norm_bwd."""
+    one per row, for layer_norm_bwd.  want_gate (with relu): (y, mean, rstd, gate), the ReLU's gate as one bit a value (uint8 [rows][ceil(cols / 8)], fp32: / 4)
+    for a backward pass that has x in 8 bits only."""
     rows, cols = _rows_of(x, "layer_norm_fwd")
+    if want_gate and not relu:
+        raise _lib.SimhandHipError("layer_norm_fwd: a gate needs relu=True")
     lib = _lib_dev()
     px, shape = _at(x), (cols,)
     y = torch.empty_like(x)
     mean = torch.empty(rows, dtype=_F32, device=x.device)
     rstd = torch.empty_like(mean)
-    check(lib.simhand_layer_norm_fwd(px, _like(gamma, x, shape, _F32, "layer_norm_fwd (gamma)"), _like(beta, x, shape, _F32, "layer_norm_fwd (beta)"), eps,
-                                     1 if relu else 0, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), rows, cols, dt(x.dtype), _row_stream(x)), "layer_norm_fwd")
-    return y, mean, rstd
+    gate = torch.empty(_gate_shape(rows, cols, x.dtype), dtype=torch.uint8, device=x.device) if want_gate else None
+    check(lib.simhand_layer_norm_fwd_ex(px, _like(gamma, x, shape, _F32, "layer_norm_fwd (gamma)"), _like(beta, x, shape, _F32, "layer_norm_fwd (beta)"), eps,
+                                        1 if relu else 0, y.data_ptr(), gate.data_ptr() if want_gate else 0, mean.data_ptr(), rstd.data_ptr(), rows, cols, dt(x.dtype),
+                                        _row_stream(x)), "layer_norm_fwd")
+    return (y, mean, rstd, gate) if want_gate else (y, mean, rstd)
 
 
-def layer_norm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, beta: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, relu: bool = False):
-    """(dx, dgamma, dbeta) of layer_norm_fwd.  x: its input, or the input's 8-bit checkpoint (act8_pack); mean, rstd: as returned there.  With relu the gate
-    is recomputed from x (bit for bit the forward's when x is the tensor itself)."""
+def _gate_shape(rows: int, cols: int, dtype: torch.dtype) -> Tuple[int, int]:
+    v = 4 if dtype is _F32 else 8  # values of a 16-byte vector
+    return rows, (cols + v - 1) // v
+
+
+def layer_norm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, beta: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, relu: bool = False,
+                   gate: Optional[torch.Tensor] = None):
+    """(dx, dgamma, dbeta) of layer_norm_fwd.  x: its input, or the input's 8-bit checkpoint (act8_pack); mean, rstd: as returned there.  With relu the gate is the one that
+    the forward pass kept (gate), or without it recomputed from x: bit for bit the forward's when x is the tensor itself, but from a checkpoint only what the
+    codes' values give -- a value whose rounding crosses the gate then passes or loses its whole gradient."""
     rows, cols = _rows_of(dy, "layer_norm_bwd")
+    if gate is not None and not relu:
+        raise _lib.SimhandHipError("layer_norm_bwd: a gate needs relu=True")
     lib = _lib_dev()
     what, shape, stats = "layer_norm_bwd", (cols,), (rows,)
     pdy = _at(dy)
@@ -296,9 +310,10 @@ def layer_norm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, beta: torch.Tensor,
     d = dt(dy.dtype)
     nb = lib.simhand_layer_norm_bwd_workspace_bytes(rows, cols, d)
     ws = _scratch(nb, dy) if nb else None
-    check(lib.simhand_layer_norm_bwd(pdy, px, pc, pe, _like(gamma, dy, shape, _F32, what + " (gamma)"), _like(beta, dy, shape, _F32, what + " (beta)"),
-                                     _like(mean, dy, stats, _F32, what + " (mean)"), _like(rstd, dy, stats, _F32, what + " (rstd)"), 1 if relu else 0,
-                                     dx.data_ptr(), dgb.data_ptr(), rows, cols, d, ws.data_ptr() if nb else 0, nb, _row_stream(dy)), what)
+    pg = _like(gate, dy, _gate_shape(rows, cols, dy.dtype), torch.uint8, what + " (gate)") if gate is not None else 0
+    check(lib.simhand_layer_norm_bwd_ex(pdy, px, pc, pe, _like(gamma, dy, shape, _F32, what + " (gamma)"), _like(beta, dy, shape, _F32, what + " (beta)"),
+                                        _like(mean, dy, stats, _F32, what + " (mean)"), _like(rstd, dy, stats, _F32, what + " (rstd)"), 1 if relu else 0, pg,
+                                        dx.data_ptr(), dgb.data_ptr(), rows, cols, d, ws.data_ptr() if nb else 0, nb, _row_stream(dy)), what)
     dgamma, dbeta = dgb.unbind(0)
     return dx, dgamma, dbeta
 
