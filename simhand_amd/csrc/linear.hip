@@ -348,10 +348,11 @@ template <typename T> __global__ __launch_bounds__(256) void linear_transpose_ke
 // ---- dz = dy act'(pre), db ----------------------------------------------------------------------------------------------------
 // One pass, bound by HBM: 100352 x 2048 bf16 with gelu 254 us (4.9 TB/s) and 5 for the fold of the blocks' sums.
 // A block covers TX 16-byte vectors of columns (TX = 8 .. 64, the power of two at or above a narrow row's vectors) and 256 / TX rows at a time over its range of rows;
-// part [row blocks][cols] = its column sums.
+// part [row blocks][cols] = its column sums.  dz may be dy's buffer (no __restrict__ between them): a value is read before the same thread stores it, and what a moved-back vector reads of
+// its neighbour's columns is dropped.
 template <typename T, int TX>
-__global__ __launch_bounds__(256) void linear_act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ pre, int act, T* __restrict__ dz,
-                                                             float* __restrict__ part, long long rows, int cols, long long per_block) {
+__global__ __launch_bounds__(256) void linear_act_bwd_kernel(const T* dy, const T* __restrict__ pre, int act, T* dz, float* __restrict__ part,
+                                                             long long rows, int cols, long long per_block) {
   constexpr int VE = Vec16<T>::N, TY = 256 / TX;
   __shared__ float red[TY][TX * VE + 1];
   const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
