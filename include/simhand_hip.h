@@ -631,7 +631,7 @@ int simhand_layer_norm_bwd_ex(const void* dy, const void* x, const uint8_t* x_co
 size_t simhand_linear_fwd_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int aligned);
 int simhand_linear_fwd(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, void* pre, int64_t rows, int in_dim,
                        int out_dim, int dtype, void* workspace, size_t workspace_bytes, sh_stream_t stream);
-/* dz = dy act'(pre), db [cols] fp32 = sum_rows dz (before dz is rounded).  SH_ACT_NONE: pre and dz may be NULL (dz = dy; only db is computed).  dz may be dy's buffer. */
+/* dz = dy act'(pre), db [cols] fp32 = sum_rows dz (before dz is rounded).  ReLU: dz = dy where pre > 0, 0 where pre <= 0 whatever dy is, NaN where pre is.  SH_ACT_NONE: pre and dz may be NULL (dz = dy; only db is computed).  dz may be dy's buffer. */
 size_t simhand_linear_act_bwd_workspace_bytes(int64_t rows, int cols, int dtype);
 int simhand_linear_act_bwd(const void* dy, const void* pre, int act, void* dz, float* db, int64_t rows, int cols, int dtype, void* workspace,
                            size_t workspace_bytes, sh_stream_t stream);

@@ -372,8 +372,13 @@ __global__ __launch_bounds__(256) void linear_act_bwd_kernel(const T* dy, const 
       if (act != SH_ACT_NONE) {
         float z[VE];
         unpack16<T>(cols >= VE ? ld16_any(pre + at - gone) : ld_chunk<T>(pre + at, left), z);
+        if (act == SH_ACT_RELU) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) d[e] *= act_slope(z[e], act);
+          for (int e = 0; e < VE; ++e) d[e] = relu_grad(d[e], z[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) d[e] *= act_slope(z[e], act);
+        }
       }
 #pragma unroll
       for (int e = 0; e < VE; ++e) s[e] += d[e];

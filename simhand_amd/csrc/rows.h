@@ -222,8 +222,8 @@ __device__ __forceinline__ float act_value(float z, int act) {
   if (act == SH_ACT_SILU) return z * logistic(z);
   return z;
 }
+// (ReLU: relu_grad below)
 __device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == SH_ACT_RELU) return z > 0.f ? 1.f : 0.f;
   if (act == SH_ACT_GELU) {
     float e;
     const float c = normal_cdf(z, e);
@@ -235,6 +235,8 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   }
   return 1.f;
 }
+// dz = dy relu'(z).  A gate, not a product: what it closes is 0 also where dy is infinite or NaN (as behind the layer norm); a NaN z stays NaN.
+__device__ __forceinline__ float relu_grad(float dy, float z) { return z > 0.f ? dy : z <= 0.f ? 0.f : z; }
 
 // ---- column sums: part [nblk][n] -> out [n], folded in 64 bits in the order of the blocks (rows.hip) -----------------------------------
 int fold_columns(const float* part, int nblk, int n, float* out, hipStream_t s);
