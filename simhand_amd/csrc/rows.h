@@ -194,9 +194,9 @@ __device__ __forceinline__ unsigned xcd_order(unsigned bid, unsigned nblk) {
 
 // ---- activations of the linear operator (enum sh_act) and their derivatives, fp32.  NaN stays NaN (also through ReLU). ------------------------
 // exp(-z^2 / 2) and the normal distribution function Phi(z) = erfc(-z / sqrt 2) / 2.  erfc(x) = t P(t) exp(-x^2), t = 1 / (1 + x / 2), x >= 0, with P the degree-8
-// Chebyshev fit of exp(x^2) erfc(x) / t over t in [1/16, 1] (x <= 30; exp(-x^2) is zero in fp32 long before): 4e-7 relative in fp32 arithmetic over the whole
-// range, on both tails, in 17 instructions.  The library's erff costs about three times that, and an epilogue of 256 x 256 of them took as long as the
-// product it follows.
+// Chebyshev fit of exp(x^2) erfc(x) / t over t in [1/16, 1] (x <= 30; exp(-x^2) is zero in fp32 long before), in 17 instructions.  Off by at most (8 + z^2) 2^-24 of Phi below zero (4e-7
+// near zero, 8e-7 at -3, 7e-6 at -12: z^2 is rounded before exp2, which the product carries over) and by 4e-7 above; exp2's and the reciprocal's last bit come on top.  The library's erff costs
+// about three times that, and an epilogue of 256 x 256 of them took as long as the product it follows.  logistic, below, likewise: (3 + 1.2 |z|) 2^-24 of its value.
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
   e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
   const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.35355339059327376f, 1.f));
@@ -238,6 +238,6 @@ __device__ __forceinline__ float act_slope(float z, int act) {
 // dz = dy relu'(z).  A gate, not a product: what it closes is 0 also where dy is infinite or NaN (as behind the layer norm); a NaN z stays NaN.
 __device__ __forceinline__ float relu_grad(float dy, float z) { return z > 0.f ? dy : z <= 0.f ? 0.f : z; }
 
-// ---- column sums: part [nblk][n] -> out [n], folded in 64 bits in the order of the blocks (rows.hip) -----------------------------------
+// ---- column sums: part [nblk][n] -> out [n], folded in 64 bits in the order of the blocks (layernorm.hip) -----------------------------------
 int fold_columns(const float* part, int nblk, int n, float* out, hipStream_t s);
 }  // namespace sh
