@@ -93,11 +93,10 @@ def projection_stats(head_out_view: Tensor, name: str) -> dict:
 # --------------------------------------------------------------------------
 # row operators with their gradients: linear, layer norm, 8-bit checkpoints
 # --------------------------------------------------------------------------
-def _keep(ctx, x: Tensor, act8: bool, *others):
-    """Saves x -- as it is, or its 8-bit codes -- and whatever else the backward pass reads."""
-    ctx.x_dtype = x.dtype
-    ctx.act8 = act8
-    if act8:
+def _keep(ctx, x: Optional[Tensor], act8: bool, *others):
+    """Saves x -- as it is, or its 8-bit codes; None: nothing reads it -- and whatever else the backward pass reads."""
+    ctx.act8 = act8 and x is not None
+    if ctx.act8:
         c = ops.act8_pack(x)
         ctx.save_for_backward(c.codes, c.exps, *others)
     else:
@@ -111,38 +110,44 @@ def _kept(ctx):
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, act, residual, act8):
+    def forward(ctx, x, w, bias, act, residual, act8, grad):
         x = x.contiguous()
         wc = w.detach().to(x.dtype).contiguous()
         b = None if bias is None else bias.detach().float().contiguous()
-        plain = act in (None, "none")
-        out = ops.linear_fwd(x, wc, b, act=act, residual=None if residual is None else residual.contiguous(), want_pre=not plain)
-        y, pre = (out, None) if plain else out
-        _keep(ctx, x, act8, wc, *(() if plain else (pre,)))
+        # kept is what a gradient that was asked for reads: x for w's, w for x's, the pre-activation for either and the bias's
+        need_x, need_w, need_b = (grad and n for n in ctx.needs_input_grad[:3])
+        want_pre = act not in (None, "none") and (need_x or need_w or need_b)
+        out = ops.linear_fwd(x, wc, b, act=act, residual=None if residual is None else residual.contiguous(), want_pre=want_pre)
+        y, pre = out if want_pre else (out, None)
+        ctx.x_dtype = x.dtype
+        _keep(ctx, x if need_w else None, act8, wc if need_x else None, pre)
         ctx.act, ctx.dtypes = act, (w.dtype, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, rest = _kept(ctx)
-        need_x, need_w, need_b, _, need_r, _ = ctx.needs_input_grad
+        x, (w, pre) = _kept(ctx)
+        need_x, need_w, need_b, _, need_r, _, _ = ctx.needs_input_grad
         dy = dy.to(ctx.x_dtype).contiguous()
-        pre = rest[1] if len(rest) > 1 else None
         dz, db = ops.linear_act_bwd(dy, pre, ctx.act) if (need_b or pre is not None) else (dy, None)
         dx = dw = None
-        if need_x or need_w:
-            dx, dw = ops.linear_bwd(dz, x, rest[0], need_dx=need_x)
-        return (dx, dw.to(ctx.dtypes[0]) if need_w else None, db.to(ctx.dtypes[1]) if need_b else None, None, dy if need_r else None, None)
+        if need_x:
+            dx, dw = ops.linear_bwd(dz, x, w, need_dw=need_w)
+        elif need_w:
+            dw = ops.linear_wgrad(dz, x)
+        return (dx, dw.to(ctx.dtypes[0]) if need_w else None, db.to(ctx.dtypes[1]) if need_b else None, None, dy if need_r else None, None, None)
 
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gamma, beta, eps, relu, act8):
+    def forward(ctx, x, gamma, beta, eps, relu, act8, grad):
         x = x.contiguous()
+        act8 = act8 and grad and any(ctx.needs_input_grad[:3])
         g, b = gamma.detach().float().contiguous(), beta.detach().float().contiguous()
         # from the codes alone the backward pass could not tell what the ReLU let through (a rounding may cross zero): its gate is kept, one bit a value
         y, *stats = ops.layer_norm_fwd(x, g, b, eps, relu, want_gate=relu and act8)
+        ctx.x_dtype = x.dtype
         _keep(ctx, x, act8, g, b, *stats)
         ctx.relu, ctx.dtypes = relu, (gamma.dtype, beta.dtype)
         return y
@@ -152,19 +157,20 @@ class _LayerNormFn(torch.autograd.Function):
     def backward(ctx, dy):
         x, (g, b, mean, rstd, *gate) = _kept(ctx)
         dx, dg, db = ops.layer_norm_bwd(dy.to(ctx.x_dtype).contiguous(), x, g, b, mean, rstd, ctx.relu, *gate)
-        return dx, dg.to(ctx.dtypes[0]), db.to(ctx.dtypes[1]), None, None, None
+        return dx, dg.to(ctx.dtypes[0]), db.to(ctx.dtypes[1]), None, None, None, None
 
 
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: Optional[str] = None, residual: Optional[Tensor] = None,
            act8: bool = False) -> Tensor:
     """act(x weight^T + bias) + residual (act: none, relu, gelu, silu) with gradients of every tensor argument; x [..., in] in fp32 or the library's 16-bit type, weight
-    [out][in] (a fp32 master is rounded to x's type for the product, its gradient stays fp32).  act8: x is kept for the backward pass in 8 bits."""
-    return _LinearFn.apply(x, weight, bias, act, residual, bool(act8) and torch.is_grad_enabled())
+    [out][in] (a fp32 master is rounded to x's type for the product, its gradient stays fp32).  act8: x is kept for the backward pass in 8 bits.  What no gradient that is asked for
+    reads is neither kept nor computed (a frozen weight: no weight gradient, x not kept)."""
+    return _LinearFn.apply(x, weight, bias, act, residual, bool(act8), torch.is_grad_enabled())
 
 
 def layer_norm(x: Tensor, weight: Tensor, bias: Tensor, eps: float = 1e-5, relu: bool = False, act8: bool = False) -> Tensor:
     """Layer norm over the last dimension (relu: with the ReLU behind it) with gradients of x, weight and bias.  act8: x is kept in 8 bits."""
-    return _LayerNormFn.apply(x, weight, bias, eps, bool(relu), bool(act8) and torch.is_grad_enabled())
+    return _LayerNormFn.apply(x, weight, bias, eps, bool(relu), bool(act8), torch.is_grad_enabled())
 
 
 # --------------------------------------------------------------------------

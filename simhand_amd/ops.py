@@ -361,9 +361,9 @@ def linear_act_bwd(dy: torch.Tensor, pre: Optional[torch.Tensor] = None, act: Op
     return dz, db
 
 
-def linear_bwd(dz: torch.Tensor, x, w: torch.Tensor, need_dx: bool = True):
-    """(dx, dw) of z = x w^T: dx = dz w in dz's type (None with need_dx=False), dw = dz^T x fp32 [out][in].  x: the forward's input, or its 8-bit
-    checkpoint (act8_pack) -- the weight gradient then reads the codes."""
+def linear_bwd(dz: torch.Tensor, x, w: torch.Tensor, need_dx: bool = True, need_dw: bool = True):
+    """(dx, dw) of z = x w^T: dx = dz w in dz's type (None with need_dx=False), dw = dz^T x fp32 [out][in] (None with need_dw=False: x may then be None too).  x: the forward's
+    input, or its 8-bit checkpoint (act8_pack) -- the weight gradient then reads the codes."""
     rows, cout = _rows_of(dz, "linear_bwd")
     lib = _lib_dev()
     if w.dim() != 2:
@@ -372,17 +372,20 @@ def linear_bwd(dz: torch.Tensor, x, w: torch.Tensor, need_dx: bool = True):
     d = dt(dz.dtype)
     pw = _like(w, dz, (cout, cin), dz.dtype, "linear_bwd (w)")
     xshape = dz.shape[:-1] + (cin,)
-    if x.shape != xshape:
-        raise _lib.SimhandHipError(f"linear_bwd: x must be {tuple(xshape)}, got {tuple(x.shape)}")
     pz = _at(dz)
-    px, pc, pe = _saved(x, dz, xshape, "linear_bwd (x)")
+    if x is None and need_dw:
+        raise _lib.SimhandHipError("linear_bwd: the weight gradient needs x")
+    if x is not None:
+        if x.shape != xshape:
+            raise _lib.SimhandHipError(f"linear_bwd: x must be {tuple(xshape)}, got {tuple(x.shape)}")
+        px, pc, pe = _saved(x, dz, xshape, "linear_bwd (x)")
     dx = None
     if need_dx:
         dx = torch.empty(xshape, dtype=dz.dtype, device=dz.device)
         nb = lib.simhand_linear_dgrad_workspace_bytes(rows, cin, cout, d, 1 if (pz | pw) & 15 == 0 else 0)
         ws = _scratch(nb, dz) if nb else None
         check(lib.simhand_linear_dgrad(pz, pw, dx.data_ptr(), rows, cin, cout, d, ws.data_ptr() if nb else 0, nb, _row_stream(dz)), "linear_dgrad")
-    return dx, _wgrad(lib, dz, pz, px, pc, pe, rows, cin, cout, d)
+    return dx, _wgrad(lib, dz, pz, px, pc, pe, rows, cin, cout, d) if need_dw else None
 
 
 def _wgrad(lib, dz, pz, px, pc, pe, rows, cin, cout, d) -> torch.Tensor:
