@@ -107,7 +107,7 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
             if constexpr (!RAG) {
               a[mi][ks][kk] = k < p.K ? ld16_any(row + k) : make_uint4(0u, 0u, 0u, 0u);
             } else {  // the ragged last chunk: the row's last 8 elements, moved into place below -- no branch between the loads
-              a[mi][ks][kk] = ld16_any(row + (k + 8 <= p.K ? k : p.K - 8));
+              a[mi][ks][kk] = ld16_any(row + (ks < KS2 * 2 - 2 || k + 8 <= p.K ? k : p.K - 8));  // (K > 128 (KS2 - 1): only the last two can end it)
             }
           }
       }
