@@ -6,7 +6,8 @@ name=$1; src=$2; shift 2
 cd "$(dirname "$0")/../simhand_amd/csrc"
 mkdir -p ../../scripts/abl build
 base=${src%.hip}
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC "$@" -c $src -o build/var_${name}.o
+flags=$(sed -n 's/^CXXFLAGS := //p' Makefile | sed 's/\$(ARCH)/gfx950/')  # the Makefile's own
+/opt/rocm/bin/hipcc $flags "$@" -c $src -o build/var_${name}.o
 objs=$(ls build/*.o | grep -v "/${base}.o" | grep -v "/var_" | grep -v "/v_" | grep -v abl)
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC $objs build/var_${name}.o -ldl -o ../../scripts/abl/lib${name}.so
 ls -la ../../scripts/abl/lib${name}.so

@@ -4,7 +4,7 @@
 // kernel's ratio (24 ds_read_b128 per 64 MFMAs per wave); + the LDS-DMA refill from L2 (8 global_load_lds_dwordx4 per 64 MFMAs per wave);
 // + both with the loop's two barriers -- and the same FLOPs arranged as 4 waves x (128 x 128) (32 reads + 16 DMAs per 128 MFMAs), each
 // for ~2 s with the socket power and gfx clock sampled from sysfs: TFLOP/s at the cap = FLOP per joule of that arrangement.
-// build: hipcc --offload-arch=gfx950 -O3 -o scripts/probes/energy_parts scripts/probes/energy_parts.hip -lpthread ; run on the GPU box.
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o scripts/probes/energy_parts scripts/probes/energy_parts.hip -lpthread ; run on the GPU box.
 #include <hip/hip_runtime.h>
 #include <atomic>
 #include <cstdio>

@@ -4,7 +4,7 @@
 // dependent chain even on zeros, so its column said nothing about the instruction.  Now 8 INDEPENDENT 32x32 accumulators per wave (128 acc registers,
 // 16 waves' worth of independent MFMAs per SIMD with 2 waves), one MFMA each per iteration; 16x16x32 keeps its 16 independent accumulators.  A host
 // thread samples the amdgpu hwmon power node while each shape runs ~1.5 s at the cap; pJ/FLOP = mean socket power / rate (idle power NOT subtracted).
-// build: hipcc --offload-arch=gfx950 -O3 -o scripts/probes/mfma_power scripts/probes/mfma_power.hip -lpthread ; run on the GPU box.
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o scripts/probes/mfma_power scripts/probes/mfma_power.hip -lpthread ; run on the GPU box.
 #include <hip/hip_runtime.h>
 #include <dirent.h>
 #include <limits.h>

@@ -8,7 +8,7 @@
 //   acc     lane (li, g): row li, bytes 16 g (+ 64)            two instructions per 16 rows x 128 B, 4 NON-adjacent lanes per 64-B segment
 //   line8   lane l: row l >> 3 (+ 8), bytes 16 (l & 7)         two instructions, 8 adjacent lanes per 128-B line
 //   linear  lane l: bytes 16 l (+ 1024) of the 2-KB block      only meaningful for row_bytes == 128 (the block is contiguous)
-// build: hipcc --offload-arch=gfx950 -O3 request_shape.hip -o request_shape      run: ./request_shape [GiB = 3]
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops request_shape.hip -o request_shape      run: ./request_shape [GiB = 3]
 #include <hip/hip_runtime.h>
 
 #include <cstdio>

@@ -6,7 +6,7 @@
 //   P1  linear: lane l writes 16 B at l*16: two whole 512-B tile rows per instruction (needs an LDS transpose in the kernel)
 //   P2  lane pairs trade a chunk (abl53): 8 rows x 128 B, lanes 2a / 2a+1 of a quarter-wave write bytes g*16 and 64 + g*16 of row a
 //   P3  8 lanes per row: lane l writes row l >> 3, byte (l & 7)*16: 8 rows x 128 B with whole lines per 8 consecutive lanes
-// build: hipcc --offload-arch=gfx950 -O3 -o scripts/probes/store_pattern scripts/probes/store_pattern.hip ; run on the GPU box.
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o scripts/probes/store_pattern scripts/probes/store_pattern.hip ; run on the GPU box.
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

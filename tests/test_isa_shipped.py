@@ -48,3 +48,15 @@ def test_no_scratch_traffic_inside_the_shipped_dma_loops():
         assert not re.search(r"\bv_pk_(add|mul|fma)_f32\b", asm), f"{src}: packed fp32 arithmetic"
     assert all(seen[s] > 4 for s in ROWS), "the scan found no LDS-DMA kernels: the sources or the pattern moved"
     assert not bad, "scratch traffic inside a hand-counted DMA loop (hipcc waits vmcnt(0) behind it):\n" + "\n".join(map(str, bad))
+
+
+def test_every_recipe_builds_with_those_flags():
+    """Variants and probes are timed and compared against the shipped kernels: their compile lines leave packed fp32 arithmetic out as well."""
+    scripts = os.path.join(ROOT, "scripts")
+    for d, _, files in os.walk(scripts):
+        for f in files:
+            if f.endswith((".sh", ".hip", ".py")):
+                for line in open(os.path.join(d, f), errors="replace"):
+                    if re.search(r"hipcc\b.*(-c|-O3|\$src)\b", line) and "-shared" not in line:
+                        assert "-packed-fp32-ops" in line or "$flags" in line, (f, line)
+    assert "CXXFLAGS" in open(os.path.join(scripts, "build_variant.sh")).read()
