@@ -1,6 +1,6 @@
 // Activation checkpoints in 8 bits: what a backward pass needs of an activation, kept as e4m3 codes with one power of two for every 32 consecutive
 // columns of a row (1.03 bytes a value).  The scale is local -- no amax history, no state, no pass over the tensor before the codes are made -- and a power of two,
-// so x 2^-e is exact and the one rounding is the code's own (at most 2^-4 relative).
+// so x 2^-e is exact and the one rounding is the code's own: at most 2^-4 of the value, or 2^-10 2^e where that is more (codes below the grid's normal range).
 //
 //   A = largest finite |x| of the 32, e = floor(log2 A) - 8, one more where A > 1.75 * 2^floor(log2 A) (so that A 2^-e <= 448, e4m3's largest), e >= -126
 //   code = e4m3(x 2^-e) to nearest even; exp byte = e + 127;  x^ = code 2^e, rounded to the tensor's type

@@ -1,5 +1,5 @@
 // Layer norm over the last dimension, forward and backward (the BatchNorm of the projection head with statistics per ROW instead of per batch: the
-// result of a row depends on no other row, so it is the same on any number of ranks and needs no collective).
+// result of a row depends on no other row: bit for bit the same in any batch, on any number of ranks, without a collective).
 //
 //   m = sum x / C, v = sum (x - m)^2 / C, r = 1 / sqrt(v + eps), h = (x - m) r, y = h gamma + beta, optionally max(y, 0)
 //   backward, u = dy (ReLU: where h gamma + beta > 0), g = u gamma:  dx = r (g - mean(g) - h mean(g h)), dgamma = sum_rows u h, dbeta = sum_rows u

@@ -94,7 +94,7 @@ class SimCLR(BaseModel):
         # nothing in the reference fixes it -> follow the encoder's width
         in_dim = getattr(self.encoder, "out_features", self.config.projection_head_input_dim)
         # projection_head_norm (not in the reference; default "batch" = its head): "layer" normalises every row by itself -- the projections of an image
-        # then depend on no other image, so they are the same on any number of ranks without a collective
+        # then depend on no other image: the same on any number of ranks without a collective, up to the rounding of the products around the norm (their order of sums goes by the number of rows)
         norm = getattr(self.config, "projection_head_norm", None) or "batch"
         if norm not in ("batch", "layer"):
             raise ValueError(f"projection_head_norm must be 'batch' or 'layer', got {norm!r}")
