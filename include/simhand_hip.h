@@ -598,7 +598,8 @@ int simhand_augment_batch_ex(const uint8_t* images, const float* joints, const f
 /* ===========================================================================
  * Row operators of an MLP / projection head: layer norm, linear (matrix product with bias, activation and residual in its epilogue) and 8-bit
  * activation checkpoints, forward and backward.  All tensors are dense rows ([rows][cols], cols contiguous) in `dtype` = SH_F32 or SH_BF16 (the
- * build's 16-bit type) unless a parameter says fp32; rows >= 0 and cols >= 1 are arbitrary (no multiple, element alignment suffices); sums,
+ * build's 16-bit type) unless a parameter says fp32; rows >= 0 and cols >= 1 are arbitrary (no multiple, element alignment suffices) up to
+ * what each call names, beyond which it is refused; sums,
  * statistics and products accumulate in fp32, column sums over rows are folded in a fixed order (bit-reproducible).  Nothing is written beside the
  * outputs and the workspace (a 16-byte address; a query of 0: NULL will do).  The reference has no such operators (its head is Linear -> BatchNorm1d -> ReLU -> Linear,
  * src/models/unsupervised/simclr_model.py:22-39): parity is held against the formulas in 64 bits.
@@ -626,7 +627,8 @@ int simhand_layer_norm_bwd_ex(const void* dy, const void* x, const uint8_t* x_co
                               int dtype, void* workspace, size_t workspace_bytes, sh_stream_t stream);
 
 /* z = x w^T + bias, y = act(z) + residual; x [rows][in_dim], w [out_dim][in_dim], bias fp32 [out_dim] or NULL, residual [rows][out_dim] or NULL,
- * pre [rows][out_dim] or NULL receives z (what simhand_linear_act_bwd takes).  residual may be y's own buffer.  Workspace query, here and below: aligned = every operand (x, w,
+ * pre [rows][out_dim] or NULL receives z (what simhand_linear_act_bwd takes).  residual may be y's own buffer.  The linear calls take rows < 2^31 and
+ * up to 2^20 columns on either side.  Workspace query, here and below: aligned = every operand (x, w,
  * residual; dz, w) lies at a 16-byte address. */
 size_t simhand_linear_fwd_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int aligned);
 int simhand_linear_fwd(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, void* pre, int64_t rows, int in_dim,
@@ -646,7 +648,8 @@ int simhand_linear_wgrad(const void* dz, const void* x, const uint8_t* x_codes, 
 
 /* 8-bit activation checkpoint: codes [rows][cols] (OCP e4m3) and exps [rows][ceil(cols / 32)], value = e4m3(code) 2^(exp - 127) with one exponent for 32
  * consecutive columns of a row: the least one with which the block's largest finite magnitude is at most 448 (never below 2^-126).  Rounded to nearest even;
- * Inf and NaN are stored as NaN.  unpack rounds the values to dtype. */
+ * Inf and NaN are stored as NaN; a finite value whose code would round past dtype's range is held at the last one that does not (61440 in fp16, 1.875 2^127 else).  unpack rounds the
+ * values to dtype.  At most 2^24 columns. */
 int simhand_act8_pack(const void* x, uint8_t* codes, uint8_t* exps, int64_t rows, int cols, int dtype, sh_stream_t stream);
 int simhand_act8_unpack(const uint8_t* codes, const uint8_t* exps, void* x, int64_t rows, int cols, int dtype, sh_stream_t stream);
 
