@@ -147,6 +147,10 @@ int simhand_test_wgrad_plain_kpm(int kpm);
  * (< 64 restores the default) */
 int simhand_test_wgrad_target_blocks(int n, int n3x3);
 
+/* the kernel that simhand_linear_fwd multiplies with (rows beyond one launch's tiles: each range is looked at by itself); aligned as in its workspace query, residual: with one */
+enum sh_linear_kernel { SH_LIN_SKINNY = 0, SH_LIN_ROWS = 1, SH_LIN_TILES256 = 2, SH_LIN_DMA = 3, SH_LIN_STAGED = 4 };
+int simhand_test_linear_kernel(int64_t rows, int in_dim, int out_dim, int dtype, int aligned, int residual);
+
 #ifdef __cplusplus
 }
 #endif

@@ -160,6 +160,7 @@ SIGNATURES = {
     "simhand_conv2d_wgrad_bnbwd": (_I, [C.POINTER(ConvDesc), _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P, _S, _P]),
     "simhand_bn_bwd_coefs": (_I, [_P, _P, _P, _P, _P, _L, _I, _P, _P, _P, _P]),
     "simhand_test_wgrad_set_tr": (_I, [_I]),
+    "simhand_test_linear_kernel": (_I, [_L, _I, _I, _I, _I, _I]),
     "simhand_test_wgrad_plain_kpm": (_I, [_I]),
     "simhand_test_wgrad_target_blocks": (_I, [_I, _I]),
     "simhand_test_wgrad3x3_enable": (_I, [_I]),

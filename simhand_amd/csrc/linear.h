@@ -99,6 +99,7 @@ struct WgradArgsL {
 bool linear256_takes(const LinearArgs& p, int dtype);
 int linear256_launch(const LinearArgs& p, hipStream_t s, const char* what);
 // rows in registers, K <= 512 (linear_rows.hip)
+bool linear_rows_fits(const LinearArgs& p, int dtype);
 bool linear_rows_takes(const LinearArgs& p, int dtype);
 size_t linear_rows_workspace_bytes(const LinearArgs& p);
 int linear_rows_launch(const LinearArgs& p, bool b_padded, void* workspace, hipStream_t s, const char* what);

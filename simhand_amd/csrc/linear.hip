@@ -675,9 +675,17 @@ template <typename F> static int by_row_ranges(const LinearArgs& p, int dtype, F
 
 // Which kernel: few rows -> the skinny one (rows <= 64 and so little work that tiles would leave most CUs idle); many -> rows in registers or the 256-wide tiles, as their rules say; whole
 // chunks -> the DMA tiles; anything else staged through registers.
+static int linear_kernel_of(const LinearArgs& p, int dtype) {
+  if (p.M <= 64 && ceil_div(p.N, 64) < 256) return SH_LIN_SKINNY;
+  if (linear_rows_takes(p, dtype)) return SH_LIN_ROWS;
+  if (linear256_takes(p, dtype)) return SH_LIN_TILES256;
+  const int ve = dtype == SH_F32 ? 4 : 8;
+  return p.K % ve == 0 && p.ldb % ve == 0 && !(((size_t)p.a | (size_t)p.b) & 15) ? SH_LIN_DMA : SH_LIN_STAGED;
+}
 static int gemm_launch(const LinearArgs& base, bool b_padded, void* workspace, int dtype, hipStream_t s, const char* what) {
   LinearArgs p = base;
-  if (p.M <= 64 && ceil_div(p.N, 64) < 256) {
+  const int kernel = linear_kernel_of(p, dtype);
+  if (kernel == SH_LIN_SKINNY) {
     const int mt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
     const dim3 grid(ceil_div(p.N, 16), 1);
 #define SH_SKINNY(T, MT) linear_skinny_kernel<T, MT><<<grid, 512, 0, s>>>(p)
@@ -693,10 +701,9 @@ static int gemm_launch(const LinearArgs& base, bool b_padded, void* workspace, i
 #undef SH_SKINNY
     return check_launch(what);
   }
-  if (linear_rows_takes(p, dtype)) return linear_rows_launch(p, b_padded, workspace, s, what);
-  if (linear256_takes(p, dtype)) return linear256_launch(p, s, what);
-  const int ve = dtype == SH_F32 ? 4 : 8;
-  if (p.K % ve == 0 && p.ldb % ve == 0 && !(((size_t)p.a | (size_t)p.b) & 15)) return dma_launch<false>(p, dtype, s, what);
+  if (kernel == SH_LIN_ROWS) return linear_rows_launch(p, b_padded, workspace, s, what);
+  if (kernel == SH_LIN_TILES256) return linear256_launch(p, s, what);
+  if (kernel == SH_LIN_DMA) return dma_launch<false>(p, dtype, s, what);
   // the tile whose rounds over the CUs cost least, each with its ends (1.2 and 4 us): 128 for 100000 x 777 -> 333 (16 bits 113 us, 64: 173; fp32 532 and 546), 64 for 400000 x 65 -> 63 (43 and
   // 53; fp32 61 and 113) and, for its last round, 5001 x 2047 -> 2047 in fp32 (393 and 515)
   auto cost = [&](int t) {
@@ -769,12 +776,18 @@ using namespace sh;
 
 extern "C" {
 
+int simhand_test_linear_kernel(int64_t rows, int in_dim, int out_dim, int dtype, int aligned, int residual) {
+  const void* at = (const void*)(size_t)(aligned ? 16 : 2);
+  const LinearArgs p = {at, at, nullptr, nullptr, nullptr, residual ? at : nullptr, rows, out_dim, in_dim, in_dim, SH_ACT_NONE, 0};
+  return linear_kernel_of(p, dtype);
+}
+
 size_t simhand_linear_fwd_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int aligned) {
   if (rows < 1 || in_dim < 1 || out_dim < 1 || dtype != SH_BF16) return 0;
-  // the padded copy of w, where the rows-in-registers kernel takes rows that are no whole 16-byte chunks, by length or by address (with a residual it takes more cases)
+  // the padded copy of w, wherever the rows-in-registers kernel may be given rows that are no whole 16-byte chunks, by length or by address
   const void* at = (const void*)(size_t)(aligned ? 16 : 2);
   LinearArgs p = {at, at, nullptr, nullptr, nullptr, at, rows, out_dim, in_dim, in_dim, SH_ACT_NONE, 0};
-  return linear_rows_takes(p, dtype) ? linear_rows_workspace_bytes(p) : 0;
+  return linear_rows_fits(p, dtype) ? linear_rows_workspace_bytes(p) : 0;
 }
 
 int simhand_linear_fwd(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, void* pre, int64_t rows, int in_dim,

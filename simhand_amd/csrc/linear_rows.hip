@@ -223,17 +223,24 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the DMAs past the end have landed before the LDS is given back
 }
 
-// K in registers, at least four units a CU; and where it pays.  Whole chunks and 64-column units: with a residual (100352 x 512 -> 2048: 260 us, the 256 x 256 kernel 325; 1605632 x 128
-// -> 512: 732 and 826), without one for K of 256 to 512 (401408 x 256 -> 1024: 272 and 319; but 1605632 x 128 -> 512: 452 and 435).  Rows that are no whole chunks, which the other
-// kernel stages through registers once per column tile: with a residual (with gelu, 100000 x 333 -> 777: 218 and 280, 200000 x 129 -> 130: 104 and 117), without one from three units
-// a row tile (300000 x 77 -> 192: 59 and 84, 100000 x 333 -> 777: 124 and 170; but 200000 x 129 -> 130: 85 and 65).
 static bool rows_whole(const LinearArgs& p) {
   return p.K % 8 == 0 && p.N % 64 == 0 && p.ldb % 8 == 0 && !(((size_t)p.a | (size_t)p.b | (size_t)p.residual) & 15);
 }
-bool linear_rows_takes(const LinearArgs& p, int dtype) {
+// What the kernel can take: K in registers, at least four units a CU.  (Ragged columns alone are the LDS-DMA tiles' business.)
+bool linear_rows_fits(const LinearArgs& p, int dtype) {
   if (dtype != SH_BF16 || p.K > 512 || p.N > kRowsMaxN || p.K < 32 || (int64_t)ceil_div(p.M, 256) * ceil_div(p.N, 64) < 1024) return false;
-  if (rows_whole(p)) return p.residual != nullptr || p.K >= 256;
-  return (p.K % 8 != 0 || (((size_t)p.a) & 15) != 0) && (p.residual != nullptr || p.N >= 192);  // (ragged columns alone: the LDS-DMA tiles take them)
+  return rows_whole(p) || p.K % 8 != 0 || (((size_t)p.a) & 15) != 0;
+}
+// ... and where it pays; us of this kernel and of what takes the call otherwise (the tiles of linear256.hip and linear.hip), over N from 50 to 2048 by K from 32 to 512, rows for 2e8 values.
+// Whole chunks and 64-column units: with a residual (100352 x 512 -> 2048: 257 and 331, 1605632 x 128 -> 512: 734 and 765, 568064 x 32 -> 320: 164 and 258; within 10 % either way at N = 64);
+// without one for K and N from 256 (401408 x 256 -> 1024: 280 and 326, 347136 x 256 -> 320: 92 and 112; but 1605632 x 128 -> 512: 452 and 435, 446208 x 256 -> 192: 94 and 87).
+// Rows that are no whole chunks, which the other kernels stage through registers: without a residual from three units a row tile (300000 x 77 -> 192: 47 and 55, 100000 x 333 -> 777: 109 and
+// 152; but 622848 x 129 -> 192: 204 and 184); with one, read in the epilogue row by row, where K is long enough to pay for that (with gelu, 100000 x 333 -> 777: 207 and 270, 314880 x 505
+// -> 130: 185 and 284, 443392 x 201 -> 250: 262 and 305; but 361472 x 33 -> 520: 333 and 258, 200000 x 129 -> 130: 92 and 61, 503552 x 333 -> 64: 138 and 131).
+bool linear_rows_takes(const LinearArgs& p, int dtype) {
+  if (!linear_rows_fits(p, dtype)) return false;
+  if (rows_whole(p)) return p.residual != nullptr || (p.K >= 256 && p.N >= 256);
+  return p.residual != nullptr ? p.K >= 192 && p.N >= 128 : p.N >= 192;
 }
 size_t linear_rows_workspace_bytes(const LinearArgs& p) { return rows_whole(p) ? 0 : (size_t)p.N * ((p.K + 7) / 8 * 8) * 2; }
 
@@ -258,17 +265,18 @@ int linear_rows_launch(const LinearArgs& base, bool b_padded, void* workspace, h
   p.n_tiles = (unsigned)ceil_div(p.N, 64);
   const unsigned units = (unsigned)ceil_div(p.M, 256) * p.n_tiles, per_cu = (units + 255) / 256;
 #define SH_ROWS(KS2, RES, PRE, RAG) linear_rows_kernel<KS2, RES, PRE, RAG><<<256, 512, 0, s>>>(p, units, per_cu)
+  // (K <= 128: ragged rows without a residual and whole ones with it, as linear_rows_takes says)
 #define SH_ROWS_K(RES, PRE)                                                                      \
   if (rag) {                                                                                     \
     switch ((p.K + 127) / 128) {                                                                 \
-      case 1: SH_ROWS(1, RES, PRE, true); break;                                              \
+      case 1: if constexpr (!RES) SH_ROWS(1, RES, PRE, true); break;                          \
       case 2: SH_ROWS(2, RES, PRE, true); break;                                              \
       case 3: SH_ROWS(3, RES, PRE, true); break;                                              \
       default: SH_ROWS(4, RES, PRE, true); break;                                             \
     }                                                                                            \
   } else {                                                                                       \
     switch ((p.K + 127) / 128) {                                                                 \
-      case 1: SH_ROWS(1, RES, PRE, false); break;                                             \
+      case 1: if constexpr (RES) SH_ROWS(1, RES, PRE, false); break;                          \
       case 2: SH_ROWS(2, RES, PRE, false); break;                                             \
       case 3: SH_ROWS(3, RES, PRE, false); break;                                             \
       default: SH_ROWS(4, RES, PRE, false); break;                                            \
