@@ -7,7 +7,7 @@
 //
 // Infinities and NaN become NaN (e4m3 has no infinity): an overflow stays visible in the gradient instead of turning into a large number.  |x| beyond
 // the last value whose code does not round past the type's range is held there (61440 for fp16, 1.875 * 2^127 else).
-// Bound by HBM: 3.03 (fp32: 5.03) bytes per value each way.  401408 x 1024 bf16: pack 221 us, unpack 209 (5.8 TB/s).
+// Bound by HBM: 3.03 (fp32: 5.03) bytes per value each way.  401408 x 1024 bf16: pack 214 us, unpack 211 (5.9 TB/s).
 #include "rows.h"
 
 namespace sh {

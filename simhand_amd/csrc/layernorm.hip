@@ -7,8 +7,9 @@
 // One pass over the data each way: a group of G lanes holds a whole row in registers (NV 16-byte vectors per lane), so the variance is summed about
 // the finished mean (no E[x^2] - m^2 cancellation) and nothing is read twice.  Statistics and sums are fp32, the column sums over row blocks are
 // folded in 64 bits in a fixed order (bit-reproducible).  Bound by HBM: 2 (3) elements of traffic per element forward (backward).
-// Measured: forward 100352 x 2048 bf16 154 us (5.3 TB/s; a large copy reaches 4.9), 256 x 512 fp32 3.1 (11 with the call around it); backward 33001 x 777 fp16 from codes 34 + 4 for the
-// fold (2.9 TB/s: a ragged row costs more arithmetic than its bytes take), 2048 x 512 fp32 with ReLU 5.8 + 3.4.
+// Measured: forward 100352 x 2048 bf16 154 us (5.3 TB/s; a large copy reaches 4.8), 256 x 512 fp32 3.0 (10 with the call around it); backward 100352 x 2048 bf16 230 (5.4 TB/s), 33001 x 777
+// fp16 from codes 35 + 4 for the fold (HBM moves 139 MB at 4.0 TB/s, the vector units are 40 % and the LDS 36 % busy, the waves, three a SIMD, wait two thirds of their time: latency),
+// 2048 x 512 fp32 with ReLU 5.8 + 3.2.
 #include "rows.h"
 
 namespace sh {
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(256, ln_bwd_occupancy(NV, sizeof(T) == 4, RAG != 0)
     }
     if (row0 + stride < rows) fetch(row + stride);
     float s1 = 0.f, s2 = 0.f;
-    // The pass is bound by its arithmetic once the loads are hidden (25 instructions a value took 35 us of 33001 x 777 alone): the gate is a variant of its own, and
+    // Three waves a SIMD hide no instruction that need not be there: the gate is a variant of its own (33001 x 777 from codes 38 us, the recomputed one 45), and
     // only a row's ragged last vector -- never in the first half of the lane's vectors -- masks what its neighbour counts.
 #pragma unroll
     for (int i = 0; i < NV; ++i) {

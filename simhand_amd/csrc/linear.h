@@ -31,7 +31,7 @@ struct LinearArgs {
 __device__ __forceinline__ int lin_col(int ni, int m) { return (ni >> 1) * 32 + (m >> 2) * 8 + (ni & 1) * 4 + (m & 3); }
 
 // A wave's finished sums, rows row0 + 16 mi, columns n0 + 32 j .. + 7 of a lane: z = acc + bias, pre <- z, out <- act(z) + residual.  The residual is read for the whole tile before
-// the first value is used (chunk after chunk, each waited for: 300000 x 77 -> 256 fp32 with gelu 333 us, like this 293).
+// the first value is used (chunk after chunk, each waited for: 300000 x 77 -> 256 fp32 with gelu 333 us, like this 293; 231 since its tiles are 64 wide).
 template <typename T, int QM, int QN>
 __device__ __forceinline__ void linear_store_tile(const LinearArgs& p, long long row0, int n0, const f32x4 (&acc)[QM][QN]) {
   constexpr int VE = Vec16<T>::N, H = 8 / VE;

@@ -6,11 +6,11 @@
 //
 // linear_gemm_kernel (forward, and dx with w transposed first; rows at any element address): out [M][N] = a [M][K] b[N][K]^T, tiles of 128 x 128 or 64 x 64, 128 bytes of K a step, both
 // operands global -> registers -> LDS with the next step's loads in flight under the MFMAs (a second step in flight and a second buffer: no faster).
-// 100000 x 777 -> 333: bf16 125 us, fp32 535 (336 at the fp32 rate of a large matrix product).  The operands are swapped (b is the MFMA's first one), and b's rows are permuted inside
+// 100000 x 777 -> 333: bf16 113 to 119 us (HBM 2 TB/s, matrix cores 22 % busy: two barriers a step), fp32 532 (336 at the fp32 rate of a large matrix product).  The operands are swapped (b is the MFMA's first one), and b's rows are permuted inside
 // the tile, so that a lane ends with 8 consecutive columns of one row: bias, residual, pre-activation and output move as 16-byte vectors.
 // linear_wgrad_kernel: dw [N][K] = dz^T x, the reduction runs over rows: tiles of 64 or 128 squared over a range of rows (split), 16-bit operands are read transposed from LDS
-// (ds_read_b64_tr_b16); the splits' fp32 partial sums are added in a fixed order by a second launch.  100000 x 777 -> 333: bf16 113 us, fp32 608; 400000 x 64 -> 64 bf16 27;
-// 2048 x 2048 -> 512 fp32 53 (28 at that rate).
+// (ds_read_b64_tr_b16); the splits' fp32 partial sums are added in a fixed order by a second launch.  100000 x 777 -> 333: bf16 109 us, fp32 608; 400000 x 64 -> 64 bf16 26;
+// from codes 6422528 x 256 -> 64 603 (4.2 TB/s), 1605632 x 512 -> 128 362 (3.5 TB/s); 2048 x 2048 -> 512 fp32 53 (28 at that rate).
 #include "linear.h"
 
 namespace sh {
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_gemm_kernel(L
 
 // The same product with both operands by LDS-DMA, for rows of whole 16-byte chunks: several k-steps ahead, one barrier per step and nothing staged in registers.  Waves as 2 x 2, each
 // QM x QN MFMA tiles: 128 x 128 (80 KB of LDS: activations two steps ahead, weights one), 128 x 64 (72 KB, two steps), 64 x 64 (80 KB, four steps: so small a tile is all
-// latency).  One block's epilogue runs under the other's k-loop.  5001 x 1000 -> 333 fp16 11 us, 16 with gelu and the pre-activation; 2048 x 512 -> 2048 fp32 40 (28 at the fp32 rate
+// latency).  One block's epilogue runs under the other's k-loop.  5001 x 1000 -> 333 fp16 12 us, 16 with gelu and the pre-activation; 2048 x 512 -> 2048 fp32 43 (28 at the fp32 rate
 // of a large matrix product).  Twice the stages for grids of one block a CU: slower (13.9 us for 11.2); barrier in mid-step with the next fragments read ahead: 12.3.
 // BT: b is stored [K][N] (dx = dz w reads w as it is, without a transposed copy): its tile is sub-tiles of 64 columns by K rows, 16-bit operands are read transposed
 // (ds_read_b64_tr_b16; the activations' chunks are then read in the halves that match its row order), fp32 ones element by element.
@@ -705,7 +705,7 @@ static int gemm_launch(const LinearArgs& base, bool b_padded, void* workspace, i
   if (kernel == SH_LIN_TILES256) return linear256_launch(p, s, what);
   if (kernel == SH_LIN_DMA) return dma_launch<false>(p, dtype, s, what);
   // the tile whose rounds over the CUs cost least, each with its ends (1.2 and 4 us): 128 for 100000 x 777 -> 333 (16 bits 113 us, 64: 173; fp32 532 and 546), 64 for 400000 x 65 -> 63 (43 and
-  // 53; fp32 61 and 113) and, for its last round, 5001 x 2047 -> 2047 in fp32 (393 and 515)
+  // 53; fp32 63 and 113) and, for its last round, 5001 x 2047 -> 2047 in fp32 (382 and 515)
   auto cost = [&](int t) {
     const int64_t blocks = (int64_t)ceil_div(p.M, t) * ceil_div(p.N, t), round = 256 * staged_on_cu(t), full = blocks / round, rest = blocks % round;
     const bool h = dtype != SH_F32;
@@ -743,7 +743,7 @@ static void act_bwd_plan(int64_t rows, int cols, int dtype, int* gx, int* gy, in
 }
 
 // Tile and splits of the rows: the pair whose estimate is least; the join of the splits reads and writes their sums at 4 TB/s and is a launch more.  It takes 64 without a split for 1000 x
-// 1000 -> 1000 in 16 bits (13.7 us; in four 20.8), 64 in 8 splits for 5001 x 1000 -> 333 (21; 128 in 20: 26), 128 in 24 for 100000 x 777 -> 333 (113; 64: 180), and 64 in 4 for 2048 x 2048
+// 1000 -> 1000 in 16 bits (13.7 us; in four 20.8), 64 in 8 splits for 5001 x 1000 -> 333 (21; 128 in 20: 26), 128 in 24 for 100000 x 777 -> 333 (109; 64: 180), and 64 in 4 for 2048 x 2048
 // -> 512 in fp32 (53; 128 in 8: 56).
 static int linear_wgrad_plan(int64_t rows, int in, int out, int dtype, int* splits, int64_t* per) {
   const bool h = dtype != SH_F32;

@@ -5,8 +5,8 @@
 // form one sequence across them: the first steps of the next tile are already on their way while the finished one is scaled, activated, added to its residual and stored, and
 // the stores drain under the next tile's MFMAs.  These layers are short in K (256 .. 512 for the wide outputs: 4 .. 8 steps) and bound by memory, so a kernel that fills
 // and drains its pipeline for every tile pays for both ends each time.
-// Measured, bf16: 1605632 x 128 -> 512 445 us (2.1 GB: 4.6 TB/s), 1605632 x 64 -> 256 193 us (1.03 GB: 5.3 TB/s); 100352 x 512 -> 2048 240 us, where its operand traffic binds (the
-// rows-in-registers kernel takes that one).
+// Measured, bf16: 1605632 x 128 -> 512 436 us (2.1 GB: 4.7 TB/s), 1605632 x 64 -> 256 199 us (1.03 GB: 5.2 TB/s); 100352 x 512 -> 2048 with a residual 331 us, where its operand traffic
+// binds (the rows-in-registers kernel takes that one: 257).
 #include "linear.h"
 
 namespace sh {

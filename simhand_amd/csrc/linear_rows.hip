@@ -5,7 +5,8 @@
 // and only b streams through LDS -- half the traffic.  The work is a list of units (256 rows x 64 columns), dealt out evenly over the CUs in contiguous ranges; b's steps (64 columns x
 // 128 of K, 16 KB, four stages, fetched three steps ahead by LDS-DMA) form one sequence across the units, and the residual's tile of the next unit arrives by LDS-DMA as well, so
 // nothing in the loop waits for memory but the counted waits below; the stores drain behind them.
-// Measured, bf16: 100352 x 512 -> 2048 with a residual 256 us (0.93 GB: 3.6 TB/s; multiplying, storing and fetching rows do not overlap inside a block), 401408 x 256 -> 1024 283.
+// Measured, bf16: 100352 x 512 -> 2048 with a residual 255 us (0.93 GB; HBM moves 1.12 at 4.5 TB/s, the matrix cores are 39 % busy: inside a block they wait while it stores and fetches
+// rows), 401408 x 256 -> 1024 282 (1.33 GB at 4.8 TB/s, of which 1.09 are written where 0.82 are due; matrix cores 34 %).  Between runs and beside other work both move by 10 %.
 // RAG: rows of a (any K) and of out (any N) at element alignment -- a goes straight to registers, so only b, which is copied into padded rows first, needs whole chunks; the residual is then read in the epilogue, and the waits are not counted past stores that may be missing.
 #include "linear.h"
 
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
 #pragma unroll
     for (int i = 0; i < 2 * RM; ++i) {
       const long long m = m0 + 8 * i < p.M ? m0 + 8 * i : p.M - 1;
-      // read once: past the caches where K is long (100352 x 512 -> 2048: 263 -> 251 us; 383 -> 389 at K = 256)
+      // read once: past the caches where K is long (100352 x 512 -> 2048: 258 -> 246 us, 200704 x 512 -> 1024 263 -> 256; 401408 x 256 -> 1024 382 -> 388)
       if constexpr (KS2 >= 3) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(dst + i * 1024), "v"((const T*)p.residual + m * p.N + col));
       else dma16((const T*)p.residual + m * p.N + col, dst + i * 1024);
     }
@@ -204,7 +205,7 @@ __global__ __launch_bounds__(512, 1) void linear_rows_kernel(LinearArgs p, unsig
             for (int e = 0; e < 8; ++e) z[e] += r8[e];
           }
           if (!in) continue;
-          // without a residual the stores go past the caches (401408 x 256 -> 1024: 285 -> 272 us); with one that costs a fifth (383 -> 469)
+          // without a residual the stores go past the caches (401408 x 256 -> 1024: 302 -> 280 us, 300032 x 384 -> 512 165 -> 145; but 600064 x 256 -> 320 171 -> 193); with one that costs a fifth (381 -> 463)
           if constexpr (RAG) {
             st_chunk<T>((T*)((char*)p.out + at), left, pack16<T>(z));
           } else {

@@ -5,7 +5,8 @@
 // each other's banks.  The operands arrive by LDS-DMA several steps ahead, one barrier per step.
 // A8: the codes (8 KB a step instead of 16) and their exponents arrive by LDS-DMA too; every thread decodes the 16 codes it fetched itself -- no barrier in between -- into the
 // 16-bit sub-tile of the NEXT step while the matrix cores work on this one.  What the layer reads of x halves, and the product is memory-bound: the decoding hides.
-// Measured, 401408 x 1024 -> 256 bf16 (1.03 GB, 210 GFLOP): 212 us, from codes 203 (0.63 GB; 159 us at the rate of a large matrix product), and 12 us for the join of the splits.
+// Measured, 401408 x 1024 -> 256 bf16 (1.03 GB, 210 GFLOP): 207 to 213 us (HBM 5.3 TB/s), from codes 201 to 209 (0.63 GB; 133 us at the rate of
+// a large matrix product, itself 63 % of the dense peak; the matrix cores are 46 % busy either way), and 12 us for the join of the splits.
 #include "linear.h"
 
 namespace sh {
