@@ -611,7 +611,8 @@ enum sh_act { SH_ACT_NONE = 0, SH_ACT_RELU = 1, SH_ACT_GELU = 2 /* z Phi(z), by 
 int simhand_layer_norm_fwd(const void* x, const float* gamma, const float* beta, float eps, int relu, void* y, float* mean, float* rstd,
                            int64_t rows, int cols, int dtype, sh_stream_t stream);
 /* u = dy (relu: where h gamma + beta > 0), g = u gamma: dx = rstd (g - mean_c(g) - h mean_c(g h)); dgamma_dbeta [2][cols] fp32 = sum_rows u h, sum_rows u.
- * x is given as it is, or (x = NULL) as its 8-bit checkpoint x_codes / x_exps (simhand_act8_pack). */
+ * x is given as it is, or (x = NULL) as its 8-bit checkpoint x_codes / x_exps (simhand_act8_pack): its rounding, up to 2^-4 |x|, stands in h as up to 2^-4 |x| rstd -- little for rows about
+ * zero, much where a row's mean is large against its spread. */
 size_t simhand_layer_norm_bwd_workspace_bytes(int64_t rows, int cols, int dtype);
 int simhand_layer_norm_bwd(const void* dy, const void* x, const uint8_t* x_codes, const uint8_t* x_exps, const float* gamma, const float* beta,
                            const float* mean, const float* rstd, int relu, void* dx, float* dgamma_dbeta, int64_t rows, int cols, int dtype,

@@ -169,7 +169,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: Option
 
 
 def layer_norm(x: Tensor, weight: Tensor, bias: Tensor, eps: float = 1e-5, relu: bool = False, act8: bool = False) -> Tensor:
-    """Layer norm over the last dimension (relu: with the ReLU behind it) with gradients of x, weight and bias.  act8: x is kept in 8 bits."""
+    """Layer norm over the last dimension (relu: with the ReLU behind it) with gradients of x, weight and bias.  act8: x is kept in 8 bits (behind a ReLU with
+    the gate beside it): h = (x - mean) rstd is then off by up to 2^-4 |x| rstd in the gradients -- for rows about zero, not for rows whose mean is large against their spread."""
     return _LayerNormFn.apply(x, weight, bias, eps, bool(relu), bool(act8), torch.is_grad_enabled())
 
 
