@@ -256,6 +256,8 @@ __global__ __launch_bounds__(256) void linear_pad_kernel(const bf16_t* __restric
 int linear_rows_launch(const LinearArgs& base, bool b_padded, void* workspace, hipStream_t s, const char* what) {
   LinearArgs p = base;
   const bool rag = !rows_whole(base);
+  // K <= 128: ragged rows without a residual and whole ones with it are all that linear_rows_takes lets through
+  SH_REQUIRE(p.K > 128 || rag == (p.residual == nullptr), "%s: rows in registers: K = %d", what, p.K);
   if (rag && !b_padded) {
     const int kp = (p.K + 7) / 8 * 8;
     linear_pad_kernel<<<(unsigned)(((int64_t)p.N * (kp / 8) + 255) / 256), 256, 0, s>>>((const bf16_t*)p.b, (bf16_t*)workspace, p.N, p.K, p.ldb, kp);
@@ -266,7 +268,6 @@ int linear_rows_launch(const LinearArgs& base, bool b_padded, void* workspace, h
   p.n_tiles = (unsigned)ceil_div(p.N, 64);
   const unsigned units = (unsigned)ceil_div(p.M, 256) * p.n_tiles, per_cu = (units + 255) / 256;
 #define SH_ROWS(KS2, RES, PRE, RAG) linear_rows_kernel<KS2, RES, PRE, RAG><<<256, 512, 0, s>>>(p, units, per_cu)
-  // (K <= 128: ragged rows without a residual and whole ones with it, as linear_rows_takes says)
 #define SH_ROWS_K(RES, PRE)                                                                      \
   if (rag) {                                                                                     \
     switch ((p.K + 127) / 128) {                                                                 \

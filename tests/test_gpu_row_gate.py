@@ -137,3 +137,33 @@ def test_gate_refusals():
               lambda: ops.layer_norm_bwd(x, x, g, g, m, r, True, gate=gate.cpu())):
         with pytest.raises(_lib.SimhandHipError):
             f()
+
+
+def test_other_shapes_no_rows_and_two_streams(dtype):
+    """Leading dimensions, no rows at all, and the same call on two streams at once."""
+    from simhand_amd import ops
+    from simhand_amd.host import model_utils as mu
+
+    x, dy = (randn(6, 7, 45) + 1).to(dtype), randn(6, 7, 45, seed=3, dtype=dtype)
+    gamma, beta = (1 + 0.1 * randn(45, seed=1)).cuda(), (0.1 * randn(45, seed=2)).cuda()
+
+    def run(shape):
+        t = [v.clone().requires_grad_() for v in (x.cuda().view(shape), gamma, beta)]
+        y = mu.layer_norm(*t, relu=True, act8=True)
+        y.backward(dy.cuda().view(shape))
+        return [y.detach().view(-1), t[0].grad.view(-1), t[1].grad, t[2].grad]
+
+    want = run((42, 45))
+    assert all(torch.equal(a, b) for a, b in zip(want, run((6, 7, 45))))
+    e = torch.empty(0, 45, dtype=dtype, device="cuda")
+    y, m, r, gate = ops.layer_norm_fwd(e, gamma, beta, relu=True, want_gate=True)
+    assert gate.shape[0] == 0
+    dx, dg, db = ops.layer_norm_bwd(e, ops.act8_pack(e), gamma, beta, m, r, True, gate=gate)
+    assert dx.shape == (0, 45) and not bool(dg.any()) and not bool(db.any())
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [None, None]
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            got[i] = run((42, 45))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(want, g))
